@@ -480,6 +480,154 @@ WAL_API int wal_decode_attention_static(const uint16_t* q, int64_t ld_q, const u
                          int64_t cache_len, int64_t n, float scale, uint16_t* out, int64_t ld_out,
                          void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged 8-bit KV cache and speculative decoding.  No reference counterpart:
+ * the reference runs Hugging Face attention over a dense 16-bit cache and
+ * decodes one token at a time.
+ *
+ * A cache holds `layers` x (K, V) pools of num_pages pages.  A page keeps
+ * page_size consecutive positions of one sequence for every kv head; a value
+ * is code * scale, with one fp32 scale for each (page, kv head) of K and of V.
+ * A sequence's pages are a row of a table int32 [B, max_pages] (rows ld_table
+ * apart): position j lives in page table[b][j / page_size].  An entry outside
+ * [0, num_pages) names no page: nothing is written there and attention leaves
+ * those positions out.  Lengths, tables and every other int32 array live on
+ * the device, so a decoding loop needs no host synchronisation; a kernel
+ * bounds every index it reads from them.
+ *
+ * Contract of the lengths: lens[b] is the number of positions that sequence b
+ * holds BEFORE this call's new tokens.  new_lens[b] (NULL: T for all) is how
+ * many of the T new rows of sequence b are real; the others are padding.
+ * ------------------------------------------------------------------------ */
+typedef enum wal_kv_kind {
+  WAL_KV_INT8 = 0, /* codes -127..127, scale = largest magnitude / 127   */
+  WAL_KV_E4M3 = 1  /* 8-bit floats up to 448, scale = largest magnitude / 448 */
+} wal_kv_kind;
+
+typedef struct wal_kv8_cache {
+  void* codes;        /* [layers][2 (K, V)][num_pages][kv_heads][page_size][head_dim] bytes, 16-byte aligned */
+  float* scales;      /* [layers][2][num_pages][kv_heads]                                                   */
+  int64_t num_pages;
+  int32_t layers;
+  int32_t kv_heads;
+  int32_t page_size;  /* 16, 32 or 64                                                                        */
+  int32_t head_dim;   /* 64 or 128                                                                           */
+  int32_t kind;       /* wal_kv_kind                                                                         */
+} wal_kv8_cache;
+
+/*
+ * Rotary positions and store of T new tokens per sequence.  qkv: bf16
+ * [B * T, ld_qkv], row b * T + t holding q (hq heads), k, v (kv_heads each) of
+ * the token at position lens[b] + t.  cos/sin: fp32 [max_pos][head_dim / 2]
+ * contiguous (rotate-half pairs i, i + head_dim / 2), or both NULL for no
+ * rotation.  q_out: bf16 rows ld_q apart, zeros for padding rows.
+ * Products and sums of the rotation are rounded one by one in fp32; q is
+ * rounded to bf16, k and v from fp32 to their codes.
+ * For each (page, kv head) that new tokens enter, of K and of V: a = largest
+ * finite magnitude of the new values there, s0 = the block's scale if it holds
+ * earlier positions of the sequence, else 0; the scale becomes s = max(s0, a
+ * times the fp32 number next to 1 / Q) and a new code is round-to-nearest-even of x / s clamped to [-Q, Q] (an
+ * infinity saturates, a NaN and every value of a block with s = 0 becomes 0);
+ * where s > s0 the earlier codes c become the codes of c * (s0 / s).  Tokens
+ * whose position has no page, or is max_pos or more, are not stored.  Pages
+ * written here must belong to one sequence alone (wal_kv_pages_assign).
+ * qkv, q_out, cos, sin 16-byte aligned; ld_qkv, ld_q multiples of 8.
+ */
+WAL_API int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qkv, int64_t ld_qkv, int64_t B,
+                   int64_t T, int32_t hq, const int32_t* table, int64_t ld_table, int64_t max_pages,
+                   const int32_t* lens, const int32_t* new_lens, const float* cos, const float* sin,
+                   int64_t max_pos, uint16_t* q_out, int64_t ld_q, void* stream);
+
+/*
+ * Values of positions first[b] + l, l < count[b], l < L, as out_dtype (WAL_F32
+ * or WAL_BF16) into k_out and v_out [B][kv_heads][L][head_dim] (contiguous,
+ * 16-byte aligned); zeros for l >= count[b] and where there is no page.
+ */
+WAL_API int wal_kv8_read(const wal_kv8_cache* cache, int32_t layer, int64_t B, const int32_t* table, int64_t ld_table,
+                 int64_t max_pages, const int32_t* first, const int32_t* count, int64_t L, void* k_out,
+                 void* v_out, int out_dtype, void* stream);
+
+/*
+ * Attention of T new tokens per sequence, already stored, over the cache:
+ * row b * T + t, head h attends to positions j <= lens[b] + t:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  G = hq / kv_heads heads share
+ * a kv head.  Rows with t >= new_lens[b], and rows without a position that has
+ * a page, are zeros.  q, out: bf16 rows ld_q / ld_out apart, heads contiguous,
+ * 16-byte aligned, ld multiples of 8; any hq that is a multiple of kv_heads.
+ * workspace: at least wal_kv8_attention_workspace bytes (0 = invalid shape),
+ * 256-byte aligned and zero-filled before its first use; calls leave it ready
+ * for the next one, whatever its lengths, and calls that share one must not
+ * overlap in time.
+ */
+WAL_API size_t wal_kv8_attention_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq);
+WAL_API int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t* q, int64_t ld_q, int64_t B,
+                      int64_t T, int32_t hq, const int32_t* table, int64_t ld_table, int64_t max_pages,
+                      const int32_t* lens, const int32_t* new_lens, float scale, uint16_t* out, int64_t ld_out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Tables of the next step.  Row b of the new table keeps the first keep[b]
+ * tokens of row parent[b] of the old one (parent outside [0, rows_in): an empty
+ * row) and gets room for add[b] more: forking, beam reordering, truncation
+ * (rejected drafts), freeing (keep = add = 0) and reserving are all cases of
+ * it.  Pages that no kept prefix names are free; nothing else is remembered.
+ * A row that will write into a partly filled last page (add > 0, keep not a
+ * multiple of page_size) shared with another reference gets a page of its own
+ * and a pair (copy_src, copy_dst) for wal_kv_pages_copy; where every reference
+ * to the page is such a row, the lowest keeps it.  Rows in rising order (the
+ * copy first, then new pages) take the free pages in rising order.
+ *   table_out [rows][width], -1 past a row's pages; ref_out [num_pages]
+ *   references after the call; copy_src / copy_dst [rows], -1 where none;
+ *   info[0] pages left free, info[1] pages that were wanted but not given (the
+ *   pool or the row's width was exhausted; their entries are -1).
+ * The old table stays as it is and must not overlap the new one, so a caller
+ * who finds info[1] > 0 can make room and call again.  rows <= 16383; a row
+ * names a page at most once.
+ */
+WAL_API int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in, const int32_t* parent,
+                        const int32_t* keep, const int32_t* add, int64_t rows, int64_t width,
+                        int64_t num_pages, int32_t page_size, int32_t* table_out, int64_t ld_out,
+                        int32_t* ref_out, int32_t* copy_src, int32_t* copy_dst, int32_t* info, void* stream);
+
+/*
+ * Compaction: with n pages named by the rows' first lens[b] tokens, the used
+ * pages >= n move to the free pages < n, both in rising order.  table_out (may
+ * be the table itself): renamed, -1 past a row's pages; remap [num_pages]: new
+ * page of each used page, else -1; move_src / move_dst [num_pages]: the moves
+ * for wal_kv_pages_copy, then -1; info[0] = n, info[1] = number of moves.
+ */
+WAL_API int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* lens, int64_t rows,
+                         int64_t width, int64_t num_pages, int32_t page_size, int32_t* table_out,
+                         int64_t ld_out, int32_t* remap, int32_t* move_src, int32_t* move_dst,
+                         int32_t* info, void* stream);
+
+/* Page src[i] -> dst[i], i < n, in every layer, K, V and scales; pairs with an
+ * entry outside [0, num_pages) are skipped.  No dst may be another pair's src
+ * or dst. */
+WAL_API int wal_kv_pages_copy(const wal_kv8_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                      void* stream);
+
+/*
+ * Verification of drafted tokens.  target: fp32 probabilities of T + 1 rows per
+ * sequence (row strides target_row, sequences target_seq elements apart);
+ * draft: the drafting distributions, T rows, or NULL where drafts were chosen
+ * without one (each counts as probability 1); drafts int32 [B, T];
+ * draft_lens[b] <= T drafts are real (NULL: T); uniforms fp32 [B, T + 1] in
+ * [0, 1).  With P = round(2^38 p), Q likewise (p clamped to [0, 1], NaN as 0)
+ * and U = floor(2^24 u):
+ *   draft t is kept while U_t Q_t(x_t) < 2^24 P_t(x_t); accepted[b] = a kept;
+ *   the next token is drawn from W = max(P_a - Q_a, 0) after a rejection (P_a
+ *   itself where that is empty), from P_a after a = draft_lens[b]: the first i
+ *   with W_0 + .. + W_i > floor(U_T sum(W) / 2^24); -1 where P_a is empty.
+ * All of it is in whole numbers: the outcome does not depend on the order of
+ * summation.  tokens [B, T + 1]: the kept drafts, the drawn token, then -1.
+ * A draft outside [0, V) is rejected.  B <= 65535, T <= 4096, V <= 2^22.
+ */
+WAL_API int wal_verify_drafts(const float* target, int64_t target_seq, int64_t target_row, const float* draft,
+                      int64_t draft_seq, int64_t draft_row, const int32_t* drafts, int64_t ld_drafts,
+                      const int32_t* draft_lens, const float* uniforms, int64_t ld_uniforms, int64_t B,
+                      int64_t T, int64_t V, int32_t* accepted, int32_t* tokens, int64_t ld_tokens, void* stream);
+
 /*
  * Device memory shared with peer processes: create (cudaMalloc, zero-filled,
  * IPC handle of WAL_IPC_HANDLE_BYTES written to handle_out), open a peer's

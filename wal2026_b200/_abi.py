@@ -31,6 +31,9 @@ WAL_BF16 = 0
 WAL_F32 = 1
 WAL_F16 = 2
 
+WAL_KV_INT8 = 0
+WAL_KV_E4M3 = 1
+
 WAL_SUM_EXACT = 0
 WAL_SUM_FAST = 1
 
@@ -112,8 +115,24 @@ class IDRouteLayer(ctypes.Structure):
     ]
 
 
+class KV8Cache(ctypes.Structure):
+    """``wal_kv8_cache``: device buffers and shape of a paged 8-bit KV cache."""
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("layers", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("kind", ctypes.c_int32),
+    ]
+
+
 _GP = ctypes.POINTER(Geometry)
 _LP = ctypes.POINTER(Layer)
+_CP = ctypes.POINTER(KV8Cache)
+_c_i32 = ctypes.c_int32
 
 SIGNATURES: dict[str, tuple] = {
     "wal_status_string": (ctypes.c_char_p, [_c_int]),
@@ -157,6 +176,19 @@ SIGNATURES: dict[str, tuple] = {
     "wal_rope_kv_append": (_c_int, [_vp, _c_i64, _c_i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp, _vp,
                                     _c_i64, _vp, _vp, _vp, _c_i64, _vp]),
     "wal_silu_mul": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp]),
+    "wal_kv8_append": (_c_int, [_CP, _c_i32, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
+                                _c_i64, _vp, _c_i64, _vp]),
+    "wal_kv8_read": (_c_int, [_CP, _c_i32, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _c_int, _vp]),
+    "wal_kv8_attention_workspace": (ctypes.c_size_t, [_CP, _c_i64, _c_i64, _c_i32]),
+    "wal_kv8_attention": (_c_int, [_CP, _c_i32, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _c_i64, _vp, _vp,
+                                   ctypes.c_float, _vp, _c_i64, _vp, ctypes.c_size_t, _vp]),
+    "wal_kv_pages_assign": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64,
+                                     _vp, _vp, _vp, _vp, _vp]),
+    "wal_kv_pages_compact": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _vp, _vp, _vp, _vp,
+                                      _vp]),
+    "wal_kv_pages_copy": (_c_int, [_CP, _vp, _vp, _c_i64, _vp]),
+    "wal_verify_drafts": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
+                                   _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
     "wal_peer_region_create": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "wal_peer_region_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),
     "wal_peer_region_close": (_c_int, [_vp]),

@@ -1,0 +1,334 @@
+// Store and read-back of the paged 8-bit KV cache.
+//
+//   kv8_append_kernel  rotary positions of q and k, and the new tokens of every
+//                      sequence into their pages.  A CTA owns one (sequence,
+//                      touched page, kv head) of K or of V: it reads its new
+//                      values, takes their largest magnitude a, sets the block's
+//                      scale to max(old, a * (1 / Q)), re-rounds the earlier codes of
+//                      the block where the scale grew, and stores the codes.
+//                      Further CTAs rotate q.  Rotation rounds each product and
+//                      sum in fp32; K is rounded once, from fp32 to its code.
+//   kv8_read_kernel    values code * scale of a range of positions.
+#include "wal_kv8.cuh"
+
+namespace {
+
+using namespace wal_kv8;
+
+struct AppendParams {
+  const uint16_t* qkv;
+  long long ld;
+  int B, T, hq, hkv, pages, max_pages, touched;
+  const int* table;
+  long long ld_table;
+  const int* lens;
+  const int* new_lens;
+  const float* cos;
+  const float* sin;
+  int max_pos;
+  uint16_t* q_out;
+  long long ld_q;
+  LayerView kv;
+  unsigned kv_ctas;  // CTAs of the K/V part, before those of q
+};
+
+// 16 values of one token and head: dims [8c, 8c + 8) and their rotation partners hd/2 later.
+struct Pair {
+  float a[8], b[8];
+};
+
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+  f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+  f[4] = bf16_lo(v.z); f[5] = bf16_hi(v.z); f[6] = bf16_lo(v.w); f[7] = bf16_hi(v.w);
+}
+
+template <int HD>
+__device__ __forceinline__ Pair load_pair(const uint16_t* src, int c) {
+  Pair p;
+  unpack(__ldg(reinterpret_cast<const uint4*>(src + 8 * c)), p.a);
+  unpack(__ldg(reinterpret_cast<const uint4*>(src + HD / 2 + 8 * c)), p.b);
+  return p;
+}
+
+template <int HD>
+__device__ __forceinline__ void rotate(Pair& p, const float* cos, const float* sin, int pos, int c) {
+  const float4* cp = reinterpret_cast<const float4*>(cos + (long long)pos * (HD / 2) + 8 * c);
+  const float4* sp = reinterpret_cast<const float4*>(sin + (long long)pos * (HD / 2) + 8 * c);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float4 cv = __ldg(cp + h), sv = __ldg(sp + h);
+    const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, ss[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = p.a[4 * h + i], y = p.b[4 * h + i];
+      p.a[4 * h + i] = __fadd_rn(__fmul_rn(x, cc[i]), __fmul_rn(-y, ss[i]));
+      p.b[4 * h + i] = __fadd_rn(__fmul_rn(y, cc[i]), __fmul_rn(x, ss[i]));
+    }
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float s) {
+  uint32_t w[2] = {0u, 0u};
+  if (s > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= encode<KIND>(__fdiv_rn(x[i], s)) << (8 * (i & 3));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+
+constexpr int kThreads = 128;
+
+template <int HD, int P, int KIND>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int C = HD / 16;                              // 16-value pieces per token and head
+  constexpr int IT = (P * C + kThreads - 1) / kThreads;   // pieces per thread of a whole page
+  const int tid = threadIdx.x;
+  if (blockIdx.x >= p.kv_ctas) {  // q rows
+    const long long i = (long long)(blockIdx.x - p.kv_ctas) * kThreads + tid;
+    const int c = (int)(i % C);
+    const long long mh = i / C;
+    const int h = (int)(mh % p.hq);
+    const long long m = mh / p.hq;
+    if (m >= (long long)p.B * p.T) return;
+    const int b = (int)(m / p.T), t = (int)(m - (long long)b * p.T);
+    const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
+    const long long pos = (long long)max(p.lens[b], 0) + t;
+    uint16_t* dst = p.q_out + m * p.ld_q + (long long)h * HD + 8 * c;
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (t < nn && (!p.cos || pos < p.max_pos)) {
+      Pair x = load_pair<HD>(p.qkv + m * p.ld + (long long)h * HD, c);
+      if (p.cos) rotate<HD>(x, p.cos, p.sin, (int)pos, c);
+      lo = make_uint4(pack_bf16(x.a[0], x.a[1]), pack_bf16(x.a[2], x.a[3]), pack_bf16(x.a[4], x.a[5]), pack_bf16(x.a[6], x.a[7]));
+      hi = make_uint4(pack_bf16(x.b[0], x.b[1]), pack_bf16(x.b[2], x.b[3]), pack_bf16(x.b[4], x.b[5]), pack_bf16(x.b[6], x.b[7]));
+    }
+    *reinterpret_cast<uint4*>(dst) = lo;
+    *reinterpret_cast<uint4*>(dst + HD / 2) = hi;
+    return;
+  }
+  const int kv = blockIdx.x & 1;
+  unsigned u = blockIdx.x >> 1;
+  const int h = (int)(u % p.hkv);
+  u /= p.hkv;
+  const int j = (int)(u % p.touched), b = (int)(u / p.touched);
+  const int len = max(p.lens[b], 0);
+  int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
+  const long long pg = (long long)(len / P) + j;  // page of the sequence
+  if (pg >= p.max_pages) return;
+  const long long start = pg * P;
+  // new tokens t in [t0, t1) fall into this page, at slots start + ...
+  long long t0 = start > len ? start - len : 0, t1 = start + P - len;
+  if (t1 > nn) t1 = nn;
+  if (p.cos && t1 > (long long)p.max_pos - len) t1 = (long long)p.max_pos - len;
+  if (t0 >= t1) return;
+  const int page = valid_page(p.table[(long long)b * p.ld_table + pg], p.pages);
+  if (page < 0) return;
+  const int slot0 = (int)(len + t0 - start), cnt = (int)(t1 - t0);  // slots [slot0, slot0 + cnt)
+  const uint16_t* src = p.qkv + ((long long)b * p.T + t0) * p.ld + (long long)(p.hq + kv * p.hkv + h) * HD;
+  Pair x[IT];
+  float a = 0.f;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * kThreads + tid, t = i / C, c = i % C;
+    if (t < cnt) {
+      x[it] = load_pair<HD>(src + (long long)t * p.ld, c);
+      if (kv == 0 && p.cos) rotate<HD>(x[it], p.cos, p.sin, (int)(len + t0) + t, c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = fmaxf(a, fmaxf(finite_abs(x[it].a[e]), finite_abs(x[it].b[e])));
+    }
+  }
+  __shared__ float red[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if ((tid & 31) == 0) red[tid >> 5] = a;
+  float* scale = (kv == 0 ? p.kv.ks : p.kv.vs) + (long long)page * p.hkv + h;
+  const float s0 = slot0 > 0 ? *scale : 0.f;
+  __syncthreads();  // every thread has read the old scale
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) a = fmaxf(a, red[w]);
+  const float s = fmaxf(s0, __fmul_rn(a, 1.f / qmax<KIND>()));
+  uint8_t* blk = (kv == 0 ? p.kv.k : p.kv.v) + ((long long)page * p.hkv + h) * (P * HD);
+  if (s > s0 && slot0 > 0) {  // the scale grew: earlier codes in units of the new one
+    const float r = __fdiv_rn(s0, s);
+    for (int i = tid; i < slot0 * (HD / 4); i += kThreads) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(blk) + i;
+      const uint32_t v = *w;
+      uint32_t n = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n |= encode<KIND>(__fmul_rn(decode<KIND>((v >> (8 * e)) & 0xffu), r)) << (8 * e);
+      *w = n;
+    }
+  }
+  if (tid == 0) *scale = s;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * kThreads + tid, t = i / C, c = i % C;
+    if (t < cnt) {
+      uint8_t* row = blk + (slot0 + t) * HD + 8 * c;
+      *reinterpret_cast<uint2*>(row) = encode8<KIND>(x[it].a, s);
+      *reinterpret_cast<uint2*>(row + HD / 2) = encode8<KIND>(x[it].b, s);
+    }
+  }
+}
+
+struct ReadParams {
+  LayerView kv;
+  int B, hkv, pages, max_pages;
+  long long L;
+  const int* table;
+  long long ld_table;
+  const int* first;
+  const int* count;
+  void* k_out;
+  void* v_out;
+};
+
+template <int HD, int P, int KIND, bool F32>
+__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ ReadParams p) {
+  constexpr int C = HD / 8;  // 8-value pieces per row
+  const long long total = (long long)p.B * p.hkv * p.L * C;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < 2 * total; i += (long long)gridDim.x * kThreads) {
+    const int kv = i >= total;
+    long long r = kv ? i - total : i;
+    const int c = (int)(r % C);
+    r /= C;  // (b, h, position)
+    const long long l = r % p.L, bh = r / p.L;
+    const int h = (int)(bh % p.hkv), b = (int)(bh / p.hkv);
+    const long long pos = (long long)max(p.first[b], 0) + l;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (l < p.count[b] && pos / P < p.max_pages) {
+      const int page = valid_page(p.table[(long long)b * p.ld_table + pos / P], p.pages);
+      if (page >= 0) {
+        const long long blk = (long long)page * p.hkv + h;
+        const float s = (kv ? p.kv.vs : p.kv.ks)[blk];
+        const uint2 w = *reinterpret_cast<const uint2*>((kv ? p.kv.v : p.kv.k) + (blk * P + pos % P) * HD + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(decode<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu), s);
+      }
+    }
+    if (F32) {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(kv ? p.v_out : p.k_out) + r * HD + 8 * c);
+      dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+      dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(kv ? p.v_out : p.k_out) + r * HD + 8 * c);
+      *dst = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    }
+  }
+}
+
+template <int HD, int P, int KIND>
+int launch_append(const AppendParams& p, unsigned grid, cudaStream_t st) {
+  kv8_append_kernel<HD, P, KIND><<<grid, kThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+template <int HD, int P, int KIND>
+int launch_read(const ReadParams& p, bool f32, unsigned grid, cudaStream_t st) {
+  if (f32) kv8_read_kernel<HD, P, KIND, true><<<grid, kThreads, 0, st>>>(p);
+  else kv8_read_kernel<HD, P, KIND, false><<<grid, kThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+// Calls F<HD, P, KIND>(args...) for the cache's shape (check_cache has passed).
+#define WAL_KV8_DISPATCH(c, F, ...)                                                                   \
+  do {                                                                                                \
+    const int key_ = ((c)->head_dim == 128 ? 6 : 0) + ((c)->page_size == 16 ? 0 : (c)->page_size == 32 ? 2 : 4) + \
+                     ((c)->kind == WAL_KV_E4M3 ? 1 : 0);                                              \
+    switch (key_) {                                                                                   \
+      case 0: return F<64, 16, WAL_KV_INT8>(__VA_ARGS__);                                             \
+      case 1: return F<64, 16, WAL_KV_E4M3>(__VA_ARGS__);                                             \
+      case 2: return F<64, 32, WAL_KV_INT8>(__VA_ARGS__);                                             \
+      case 3: return F<64, 32, WAL_KV_E4M3>(__VA_ARGS__);                                             \
+      case 4: return F<64, 64, WAL_KV_INT8>(__VA_ARGS__);                                             \
+      case 5: return F<64, 64, WAL_KV_E4M3>(__VA_ARGS__);                                             \
+      case 6: return F<128, 16, WAL_KV_INT8>(__VA_ARGS__);                                            \
+      case 7: return F<128, 16, WAL_KV_E4M3>(__VA_ARGS__);                                            \
+      case 8: return F<128, 32, WAL_KV_INT8>(__VA_ARGS__);                                            \
+      case 9: return F<128, 32, WAL_KV_E4M3>(__VA_ARGS__);                                            \
+      case 10: return F<128, 64, WAL_KV_INT8>(__VA_ARGS__);                                           \
+      default: return F<128, 64, WAL_KV_E4M3>(__VA_ARGS__);                                           \
+    }                                                                                                 \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qkv, int64_t ld_qkv, int64_t B, int64_t T,
+                   int32_t hq, const int32_t* table, int64_t ld_table, int64_t max_pages, const int32_t* lens,
+                   const int32_t* new_lens, const float* cos, const float* sin, int64_t max_pos, uint16_t* q_out,
+                   int64_t ld_q, void* stream) {
+  int st = check_cache(cache, layer);
+  if (st != WAL_OK) return st;
+  if (!qkv || !table || !lens || !q_out || !cos != !sin) return WAL_ERR_INVALID_ARGUMENT;
+  if (B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads || max_pages <= 0 || ld_table < max_pages) return WAL_ERR_SHAPE;
+  if (B > 0x7fffffff || T > 0x7fffffff || max_pages > 0x7fffffff / cache->page_size) return WAL_ERR_SHAPE;
+  if (cos && (max_pos <= 0 || max_pos > 0x7fffffff)) return WAL_ERR_SHAPE;
+  const int hd = cache->head_dim, P = cache->page_size;
+  if (ld_qkv < (int64_t)(hq + 2 * cache->kv_heads) * hd || ld_q < (int64_t)hq * hd) return WAL_ERR_SHAPE;
+  if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)cos & 15) || ((uintptr_t)sin & 15) || (ld_qkv % 8) ||
+      (ld_q % 8))
+    return WAL_ERR_ALIGNMENT;
+  AppendParams p = {};
+  p.qkv = qkv;
+  p.ld = ld_qkv;
+  p.B = (int)B;
+  p.T = (int)T;
+  p.hq = hq;
+  p.hkv = cache->kv_heads;
+  p.pages = (int)cache->num_pages;
+  p.max_pages = (int)max_pages;
+  p.touched = (int)((T + P - 2) / P + 1);  // T tokens from any slot of a page
+  p.table = table;
+  p.ld_table = ld_table;
+  p.lens = lens;
+  p.new_lens = new_lens;
+  p.cos = cos;
+  p.sin = sin;
+  p.max_pos = (int)max_pos;
+  p.q_out = q_out;
+  p.ld_q = ld_q;
+  p.kv = layer_view(*cache, layer);
+  const long long kv_ctas = 2LL * B * p.touched * p.hkv;
+  const long long q_ctas = (B * T * hq * (hd / 16) + kThreads - 1) / kThreads;
+  if (kv_ctas + q_ctas > 0x7fffffff) return WAL_ERR_SHAPE;
+  p.kv_ctas = (unsigned)kv_ctas;
+  const unsigned grid = (unsigned)(kv_ctas + q_ctas);
+  WAL_KV8_DISPATCH(cache, launch_append, p, grid, static_cast<cudaStream_t>(stream));
+}
+
+int wal_kv8_read(const wal_kv8_cache* cache, int32_t layer, int64_t B, const int32_t* table, int64_t ld_table,
+                 int64_t max_pages, const int32_t* first, const int32_t* count, int64_t L, void* k_out, void* v_out,
+                 int out_dtype, void* stream) {
+  int st = check_cache(cache, layer);
+  if (st != WAL_OK) return st;
+  if (!table || !first || !count || !k_out || !v_out) return WAL_ERR_INVALID_ARGUMENT;
+  if (out_dtype != WAL_F32 && out_dtype != WAL_BF16) return WAL_ERR_UNSUPPORTED;
+  if (B <= 0 || L <= 0 || max_pages <= 0 || ld_table < max_pages) return WAL_ERR_SHAPE;
+  if (B > 0x7fffffff || L > 0x7fffffff || max_pages > 0x7fffffff / cache->page_size) return WAL_ERR_SHAPE;
+  if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15)) return WAL_ERR_ALIGNMENT;
+  ReadParams p = {};
+  p.kv = layer_view(*cache, layer);
+  p.B = (int)B;
+  p.hkv = cache->kv_heads;
+  p.pages = (int)cache->num_pages;
+  p.max_pages = (int)max_pages;
+  p.L = L;
+  p.table = table;
+  p.ld_table = ld_table;
+  p.first = first;
+  p.count = count;
+  p.k_out = k_out;
+  p.v_out = v_out;
+  const long long ctas = (2LL * B * p.hkv * L * (cache->head_dim / 8) + kThreads - 1) / kThreads;
+  const unsigned grid = (unsigned)(ctas < 148 * 16 ? ctas : 148 * 16);
+  WAL_KV8_DISPATCH(cache, launch_read, p, out_dtype == WAL_F32, grid, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
