@@ -88,7 +88,7 @@ def _check_attention(cache, q, table, lens, news=None, scale=None, layer=0, ws=N
     nl = None if news is None else _i32(news)
     kv8_attention(cache, layer, q, table, _i32(lens), out, ws, new_lens=nl, scale=scale)
     want, mag = _attention64(cache, layer, q, table, lens, news or [T] * B, hd ** -0.5 if scale is None else scale)
-    bad = (out.double() - want).abs() > 2 * (2.0 ** -8 * want.abs() + 2.0 ** -11 * mag) + 1e-30
+    bad = ~((out.double() - want).abs() <= 2 * (2.0 ** -8 * want.abs() + 2.0 ** -11 * mag) + 1e-30)  # a NaN is bad too
     assert not bool(bad.any()), (int(bad.sum()), float((out.double() - want).abs().max()))
     again = torch.empty_like(out)
     kv8_attention(cache, layer, q, table, _i32(lens), again, ws, new_lens=nl, scale=scale)

@@ -2,21 +2,59 @@
 //
 //   out[b, t, h] = sum_j softmax_j(scale * q[b, t, h] . k_j) v_j,  j <= lens[b] + t
 //
-// One CTA per query row; its warps take positions in turn, each with a running
-// maximum and sum (softmax in one pass), joined at the end.
+// The cache is read once per kv head and row tile; everything else is small, so
+// the kernel is built to keep loads in flight and bytes per value at one.
+//
+// Work split.  The rows that share a kv head (T tokens x G heads, row t * G + g)
+// form tiles of 8, 16, 32 or 64 rows; a unit is one (sequence, row tile, kv head)
+// over its positions in tiles of 32.  The position tiles of all units, in
+// order, are cut into equal runs, one per CTA of a grid that fills the GPU
+// once, whatever the mix of lengths: every CTA reads the lengths, sums the tile
+// counts and finds its run.  A unit that one CTA covers is written by it; one
+// that several cover leaves (max, sum, un-normalised output) per row in the
+// workspace, and the last of its CTAs to arrive joins them in CTA order, so
+// results do not depend on timing.  Calls of more than kMaxEntries (sequence,
+// row tile) pairs have units enough to give each CTA whole ones.
+//
+// Within a CTA.  One warp group (one warp for 8 rows, or for each 16) takes every NS-th
+// position tile through its own ring of stages in shared memory (16-byte
+// asynchronous copies, page by page; pieces swizzled so that the matrix loads
+// below meet no bank conflict), with its own running maximum and sum.  Codes
+// become 16-bit floats in registers (each int8 and e4m3 code is exact in f16
+// and in bf16) and feed mma.sync m16n8k16 with fp32 accumulators.  K fragments
+// come from ldmatrix (four dims of a token per register), V fragments from the
+// transposing 8-bit ldmatrix (four tokens of a dim per register); the order of
+// k within a fragment is free, so Q and P are laid out to match.
+//
+// Numerics.  q is scaled by a power of two per row into f16's range: elements
+// down to 2^-31 of the row's largest keep all of bf16's bits.  Scores, maxima,
+// sums and outputs are fp32.  P, times the block's V scale over the largest V
+// scale seen so far (which moves with the running maximum), enters the second
+// product as the sum of two bf16 numbers: 2^-17 of each weight and fp32's
+// range, where one f16 would lose weights below 2^-24 of the largest and one
+// bf16 would add an error the size of the output's own rounding.  With up to 8
+// rows the second number costs nothing: it takes the unused half of the A tile.
 #include "wal_kv8.cuh"
+
+#include <cuda_fp16.h>
 
 namespace {
 
 using namespace wal_kv8;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTile = 32;          // positions of a tile
+constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced call
+constexpr int kCtasPerSm = 2;
+constexpr int kMinTiles = 4;       // least position tiles of a run: one per warp
 
 struct AttnParams {
   const uint16_t* q;
   long long ld_q;
   LayerView kv;
-  int T, hq, hkv, P, pages, max_pages;
+  int B, T, hq, hkv, G, P, pages, max_pages;
+  int row_tiles;  // per (sequence, kv head)
   const int* table;
   long long ld_table;
   const int* lens;
@@ -24,54 +62,604 @@ struct AttnParams {
   float qscale;  // scale * log2(e)
   uint16_t* out;
   long long ld_out;
+  unsigned* counter;  // [grid] of the unit that starts in a CTA's run and goes on past it
+  float* part;        // [grid][2][rows][HD]
+  float2* stats;      // [grid][2][rows] (max, sum)
+  bool balanced;
 };
 
-template <int HD, int KIND>
-__global__ void __launch_bounds__(kThreads) kv8_attention_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int NW = kThreads / 32, E = HD / 32;
-  __shared__ float sm[NW], sl[NW], so[NW][HD];
-  const int h = blockIdx.x % p.hq, m = blockIdx.x / p.hq, b = m / p.T, t = m - b * p.T;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = h / (p.hq / p.hkv);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&m)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+               : "r"(addr));
+}
+// Two 16 x 16 byte matrices, transposed: register 2i holds column lane / 4 of
+// matrix i, rows 4 * (lane % 4) .. + 3; register 2i + 1 column 8 + lane / 4.
+__device__ __forceinline__ void ldsm_t8_x2(uint32_t addr, uint32_t (&m)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t v;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+
+// Which of a register's four codes share a 16-bit pair: bytes (0, 2) and (1, 3),
+// as masks split even from odd bytes, but (0, 1) and (2, 3) where e4m3 becomes
+// f16 by the conversion that takes neighbours.
+__host__ __device__ constexpr int split_at(int pair, int e) { return 2 * e + pair; }
+template <int KIND>
+__host__ __device__ constexpr int k_at(int pair, int e) {
+  return KIND == WAL_KV_INT8 ? split_at(pair, e) : 2 * pair + e;
+}
+
+// K codes as f16.
+template <int KIND>
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if (KIND == WAL_KV_INT8) {
+    // 0x6400 | u is 1024 + u; u = code + 128
+    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));  // 1152
+    const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    p0 = *reinterpret_cast<const uint32_t*>(&x);
+    p1 = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{.reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n cvt.rn.f16x2.e4m3x2 %1, hi;\n}"
+        : "=r"(p0), "=r"(p1)
+        : "r"(w));
+  }
+}
+
+// V codes as bf16, divided by v_unit.
+template <int KIND>
+__host__ __device__ constexpr float v_unit() {
+  return KIND == WAL_KV_INT8 ? 1.f : 1.329227995784916e36f;  // 2^120
+}
+template <int KIND>
+__device__ __forceinline__ void to_bf16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if (KIND == WAL_KV_INT8) {
+    // 0x4300 | low seven bits is 128 + them; 0x4300 | sign bit is 128 or 256
+    const uint32_t w1 = w >> 8;
+    const uint32_t a = (w & 0x007f007fu) | 0x43004300u, b = (w & 0x00800080u) | 0x43004300u;
+    const uint32_t c = (w1 & 0x007f007fu) | 0x43004300u, d = (w1 & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(&d));
+    p0 = *reinterpret_cast<const uint32_t*>(&x);
+    p1 = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    // exponent and fraction bits moved to bf16's: the value times 2^(7 - 127),
+    // subnormals included, and finite for every byte
+    p0 = ((w << 8) & 0x80008000u) | ((w << 4) & 0x07f007f0u);
+    p1 = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);
+  }
+}
+
+// Byte offset of 16-byte piece c of row r of a tile.  Lines of 128 bytes hold
+// one row (HD 128) or two; the pieces of a line are permuted by a key that
+// differs among the eight rows one matrix load reads together.
+template <int HD>
+__device__ __forceinline__ uint32_t k_offset(int r, int c) {
+  const int line = HD == 128 ? r : r >> 1, piece = HD == 128 ? c : ((r & 1) << 2) | c;
+  return (uint32_t)(line * 128 + ((piece ^ ((r >> 1) & 7)) << 4));
+}
+template <int HD>
+__device__ __forceinline__ uint32_t v_offset(int r, int c) {
+  if (HD == 128) return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+  const int line = r >> 1;
+  return (uint32_t)(line * 128 + (((((r & 1) << 2) | c) ^ (line & 3)) << 4));
+}
+
+// RW rows per warp (8 or 16), WM warps per group.
+template <int HD, int RW, int WM>
+struct Shape {
+  static constexpr int kRows = RW * WM;         // query rows of a unit
+  static constexpr int NS = kWarps / WM;        // warp groups
+  static constexpr int kStages = WM == 4 ? 4 : 3;
+  static constexpr int kStageBytes = 2 * kTile * HD;  // K rows, then V rows
+  static constexpr int kRing = NS * kStages * kStageBytes;
+  static constexpr int LDO = HD + 8;            // padded row of the join buffer
+  static constexpr int kJoin = kWarps * RW * LDO * 4;
+  static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kSmem = kMain + NS * kStages * 32;  // then, per stage: 4 scales and the block mask
+};
+
+struct Segment {
+  int b, rt, kvh;    // unit
+  int tile0, tile1;  // position tiles
+};
+
+// Attended positions of sequence b by its last real token of row tile rt; 0 where the tile has none.
+template <int RT>
+__device__ __forceinline__ int positions(const AttnParams& p, int b, int rt, int* news, int* len) {
   const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
-  uint16_t* orow = p.out + (long long)m * p.ld_out + (long long)h * HD;
-  const long long cap = (long long)p.max_pages * p.P;
-  const int n = t < nn ? (int)min((long long)max(p.lens[b], 0) + t + 1, cap) : 0;
-  float q[E], o[E], mx = -INFINITY, l = 0.f;
+  const int ln = max(p.lens[b], 0);
+  *news = nn;
+  *len = ln;
+  if (nn <= 0 || (long long)rt * RT >= (long long)nn * p.G) return 0;
+  const int last = (int)min(((long long)rt * RT + RT - 1) / p.G, (long long)nn - 1);
+  return (int)min((long long)ln + last + 1, (long long)p.max_pages * p.P);
+}
+
+template <int HD, int KIND, int RW, int WM>
+__device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& sg, bool whole, int slot, uint8_t* smem) {
+  using S = Shape<HD, RW, WM>;
+  constexpr int KT = HD / 16, NT = HD / 8, C = HD / 16, RT = S::kRows, LDO = S::LDO;
+  constexpr int HH = RW / 8;  // rows of a lane: r and, of 16, r + 8
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grp = warp / WM, wm = warp % WM, r = lane >> 2, q4 = lane & 3;
+  int news, len;
+  const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(grp * S::kStages * S::kStageBytes);
+  float* const side = reinterpret_cast<float*>(smem + S::kMain) + grp * S::kStages * 8;
+  const int* trow = p.table + (long long)sg.b * p.ld_table;
+  const int psh = p.P == 16 ? 4 : p.P == 32 ? 5 : 6;
+  const long long page_codes = (long long)p.hkv * p.P * HD;
+  const uint8_t* kbase = p.kv.k + (long long)sg.kvh * p.P * HD;
+  const uint8_t* vbase = p.kv.v + (long long)sg.kvh * p.P * HD;
+
+  auto group_sync = [&]() {
+    if (WM == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(32 * WM) : "memory");
+  };
+  // pages of a tile's two blocks of 16 positions, -1 past the unit's positions
+  auto pages_of = [&](int tile, int& a, int& b) {
+    const int t0 = tile * kTile;
+    a = t0 < n ? valid_page(__ldg(trow + (t0 >> psh)), p.pages) : -1;
+    b = t0 + 16 < n ? valid_page(__ldg(trow + ((t0 + 16) >> psh)), p.pages) : -1;
+  };
+  auto load = [&](int stage, int tile, int pa, int pb) {
+    const int t0 = tile * kTile;
+    const uint32_t ks = ring + (uint32_t)(stage * S::kStageBytes), vs = ks + kTile * HD;
+    constexpr int PER = kTile * C / (32 * WM);  // pieces of K per lane
+    const int l = wm * 32 + lane;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __uint_as_float((uint32_t)p.q[(long long)m * p.ld_q + (long long)h * HD + e * 32 + lane] << 16);
-    o[e] = 0.f;
+    for (int i = 0; i < PER; ++i) {
+      const int x = i * 32 * WM + l, row = x / C, c = x % C;
+      const int page = row < 16 ? pa : pb;
+      const bool in = page >= 0;
+      const long long off = in ? page * page_codes + (long long)((t0 + row) & (p.P - 1)) * HD + c * 16 : 0;
+      const uint32_t sz = in ? 16u : 0u;  // absent blocks read as zeros
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(ks + k_offset<HD>(row, c)), "l"(kbase + off), "r"(sz));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(vs + v_offset<HD>(row, c)), "l"(vbase + off), "r"(sz));
+    }
+    float* sd = side + stage * 8;
+    if (l < 4) {
+      const int page = l & 1 ? pb : pa;
+      const float* src = (l < 2 ? p.kv.ks : p.kv.vs) + (page >= 0 ? (long long)page * p.hkv + sg.kvh : 0);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(sd + l)), "l"(src), "r"(page >= 0 ? 4u : 0u));
+    }
+    if (l == 4) sd[4] = __int_as_float((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
+  };
+
+  // fill the ring
+  const int first = sg.tile0 + grp;
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) {
+    const int tile = first + s * S::NS;
+    if (tile < sg.tile1) {
+      int pa, pb;
+      pages_of(tile, pa, pb);
+      load(s, tile, pa, pb);
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
   }
-  for (int j = warp; j < n; j += NW) {
-    const int page = valid_page(p.table[(long long)b * p.ld_table + j / p.P], p.pages);
-    if (page < 0) continue;
-    const long long blk = (long long)page * p.hkv + kvh, row = (blk * p.P + j % p.P) * HD;
-    float s = 0.f;
+  int npa = -1, npb = -1;  // pages of the next tile to load
+  if (first + (S::kStages - 1) * S::NS < sg.tile1) pages_of(first + (S::kStages - 1) * S::NS, npa, npb);
+
+  // q: rows r and r + 8 of this warp's, scaled by powers of two into f16
+  const int row0 = sg.rt * RT + wm * RW + r;
+  uint32_t qa[KT][4];
+  float unscale[HH];
+  int lim[HH];  // positions each row attends to
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], decode<KIND>(p.kv.k[row + e * 32 + lane]), s);
+  for (int hh = 0; hh < HH; ++hh) {
+    const int row = row0 + 8 * hh, t = row / p.G, g = row - t * p.G;
+    const bool real = t < news;
+    lim[hh] = real ? (int)min((long long)len + t + 1, (long long)n) : 0;
+    const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + g) * HD;
+    uint2 w[KT];
+    float mx = 0.f;
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    s *= p.kv.ks[blk] * p.qscale;
-    const float mn = fmaxf(mx, s), al = mx == -INFINITY ? 0.f : exp2f(mx - mn), w = exp2f(s - mn);
-    const float wv = w * p.kv.vs[blk];
-    l = fmaf(l, al, w);
+    for (int kt = 0; kt < KT; ++kt) {
+      w[kt] = real ? __ldg(reinterpret_cast<const uint2*>(src + kt * 16 + 4 * q4)) : make_uint2(0u, 0u);
+      mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(w[kt].x)), fabsf(bf16_hi(w[kt].x))), fmaxf(fabsf(bf16_lo(w[kt].y)), fabsf(bf16_hi(w[kt].y)))));
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // 2^e with mx * 2^e in [2^14, 2^15), kept within normal floats
+    const int e = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    unscale[hh] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], al, wv * decode<KIND>(p.kv.v[row + e * 32 + lane]));
-    mx = mn;
+    for (int kt = 0; kt < KT; ++kt) {
+      const float x[4] = {bf16_lo(w[kt].x) * up, bf16_hi(w[kt].x) * up, bf16_lo(w[kt].y) * up, bf16_hi(w[kt].y) * up};
+      qa[kt][hh] = pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]);
+      qa[kt][2 + hh] = pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]);
+      if (HH == 1) qa[kt][1] = qa[kt][3] = 0u;
+    }
   }
-  if (lane == 0) sm[warp] = mx, sl[warp] = l;
+  const int lim_min = HH == 2 ? min(lim[0], lim[HH - 1]) : lim[0];
+
+  float m[HH], l[HH], vref = 1e-30f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][e * 32 + lane] = o[e];
+  for (int hh = 0; hh < HH; ++hh) m[hh] = -INFINITY, l[hh] = 0.f;
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+  int stage = 0;
+  for (int tile = first; tile < sg.tile1; tile += S::NS) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(S::kStages - 2) : "memory");
+    group_sync();  // this stage has landed for the group, and the previous one is free
+    const int ahead = tile + (S::kStages - 1) * S::NS;
+    if (ahead < sg.tile1) {
+      load(stage == 0 ? S::kStages - 1 : stage - 1, ahead, npa, npb);
+      if (ahead + S::NS < sg.tile1) pages_of(ahead + S::NS, npa, npb);
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+    const uint32_t ks = ring + (uint32_t)(stage * S::kStageBytes), vs = ks + kTile * HD;
+    const float4 sc = *reinterpret_cast<const float4*>(side + stage * 8);  // K scales, V scales of the two blocks
+    const int have = __float_as_int(side[stage * 8 + 4]);
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+
+    // scores: n-tile 2j + s, column c is position 16j + 4 * (c / 2) + split_at(s, c % 2)
+    float s[4][4];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      const int i = lane & 7, row = (nt >> 1) * 16 + 4 * (i >> 1) + split_at(nt & 1, i & 1);
+#pragma unroll
+      for (int c = 0; c < C; c += 4) {
+        uint32_t w[4];
+        ldsm_x4(ks + k_offset<HD>(row, c + (lane >> 3)), w);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t b0, b1;
+          to_f16<KIND>(w[x], b0, b1);
+          mma_f16(s[nt], qa[c + x], b0, b1);
+        }
+      }
+    }
+    const int t0 = tile * kTile;
+    const bool edge = have != 3 || t0 + kTile > lim_min;
+    float mn[HH];
+    bool grew = false;
+#pragma unroll
+    for (int hh = 0; hh < HH; ++hh) {
+      mn[hh] = m[hh];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[nt][2 * hh + e];
+          x *= unscale[hh] * (nt < 2 ? sc.x : sc.y);
+          if (edge) {
+            const int pos = t0 + (nt >> 1) * 16 + 4 * q4 + split_at(nt & 1, e);
+            if (!((have >> (nt >> 1)) & 1) || pos >= lim[hh]) x = -INFINITY;
+          }
+          mn[hh] = fmaxf(mn[hh], x);
+        }
+      mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 1));
+      mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 2));
+      grew |= mn[hh] > m[hh];
+    }
+    const float vnew = fmaxf(vref, fmaxf(sc.z, sc.w));
+    if (__any_sync(0xffffffffu, grew || vnew > vref)) {
+      const float vr = vref / vnew;
+      vref = vnew;
+#pragma unroll
+      for (int hh = 0; hh < HH; ++hh) {
+        const float al = mn[hh] == -INFINITY ? 0.f : ex2(m[hh] - mn[hh]);
+        m[hh] = mn[hh];
+        l[hh] *= al;
+        const float av = al * vr;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          o[i][2 * hh] *= av;
+          o[i][2 * hh + 1] *= av;
+          if (HH == 1) o[i][2] *= av, o[i][3] *= av;
+        }
+      }
+    }
+    const float vinv = 1.f / vref, vf[2] = {sc.z * vinv * v_unit<KIND>(), sc.w * vinv * v_unit<KIND>()};
+#pragma unroll
+    for (int hh = 0; hh < HH; ++hh) {
+      const float base = m[hh] == -INFINITY ? 0.f : m[hh];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = ex2(s[nt][2 * hh + e] - base);
+          l[hh] += x;
+          s[nt][2 * hh + e] = x * vf[nt >> 1];
+        }
+    }
+    // P.V, 16 positions at a time; each weight as a bf16 number and the rest of it
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t hi[2 * HH], lo[2 * HH];
+#pragma unroll
+      for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float u = s[2 * j + x][2 * hh], v = s[2 * j + x][2 * hh + 1];
+          const uint32_t w = pack_bf16(u, v);
+          hi[x * HH + hh] = w;
+          lo[x * HH + hh] = pack_bf16(u - bf16_lo(w), v - bf16_hi(w));
+        }
+#pragma unroll
+      for (int c = 0; c < C; c += 2) {
+        uint32_t w[4];
+        ldsm_t8_x2(vs + v_offset<HD>(16 * j + (lane & 15), c + (lane >> 4)), w);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t b0, b1;
+          to_bf16<KIND>(w[x], b0, b1);
+          if constexpr (HH == 1) {
+            const uint32_t a[4] = {hi[0], lo[0], hi[1], lo[1]};
+            mma_bf16(o[2 * c + x], a, b0, b1);
+          } else {
+            const uint32_t a[4] = {hi[0], hi[1], hi[2], hi[3]}, b[4] = {lo[0], lo[1], lo[2], lo[3]};
+            mma_bf16(o[2 * c + x], a, b0, b1);
+            mma_bf16(o[2 * c + x], b, b0, b1);
+          }
+        }
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+#pragma unroll
+  for (int hh = 0; hh < HH; ++hh) {
+    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+  }
+
+  // join the warp groups: outputs and (max, sum) of every warp's rows
+  __shared__ float2 wstat[kWarps][RW];
+  __syncthreads();  // the ring is free
+  float* po = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int hh = 0; hh < HH; ++hh) {
+    if (lim[hh] > 0) {
+      float* dst = po + (warp * RW + r + 8 * hh) * LDO + 2 * q4;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float x = o[i][2 * hh], y = o[i][2 * hh + 1];
+        if (HH == 1) x += o[i][2], y += o[i][3];
+        *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(x * vref, y * vref);
+      }
+    }
+    if (q4 == 0) wstat[warp][r + 8 * hh] = make_float2(m[hh], l[hh]);
+  }
   __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w]);
-  for (int w = 0; w < NW; ++w)
-    if (sm[w] != -INFINITY) L = fmaf(exp2f(sm[w] - M), sl[w], L);
-  for (int d = threadIdx.x; d < HD; d += kThreads) {
-    float a = 0.f;
-    for (int w = 0; w < NW; ++w)
-      if (sm[w] != -INFINITY) a = fmaf(exp2f(sm[w] - M), so[w][d], a);
-    orow[d] = __bfloat16_as_ushort(__float2bfloat16_rn(L > 0.f ? a / L : 0.f));
+  const int rows = min(RT, news * p.G - sg.rt * RT);
+  for (int i = tid; i < rows * (HD / 4); i += kThreads) {
+    const int row = i / (HD / 4), c = i % (HD / 4), w0 = row / RW, rr = row % RW;
+    float M = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < S::NS; ++g) M = fmaxf(M, wstat[g * WM + w0][rr].x);
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < S::NS; ++g) {
+      const float2 st = wstat[g * WM + w0][rr];
+      if (st.y == 0.f) continue;  // no position seen
+      const float f = ex2(st.x - M);
+      const float4 v = *reinterpret_cast<const float4*>(po + ((g * WM + w0) * RW + rr) * LDO + 4 * c);
+      L = fmaf(f, st.y, L);
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    }
+    if (whole) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const int grow = sg.rt * RT + row, t = grow / p.G, g = grow - t * p.G;
+      uint16_t* dst = p.out + ((long long)sg.b * p.T + t) * p.ld_out + (long long)(sg.kvh * p.G + g) * HD + 4 * c;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    } else {
+      reinterpret_cast<float4*>(p.part)[((long long)slot * RT + row) * (HD / 4) + c] = acc;
+      if (c == 0) p.stats[(long long)slot * RT + row] = make_float2(M, L);
+    }
+  }
+  __syncthreads();  // the join buffer becomes the ring again
+}
+
+// Joins the runs c0 .. c1 of a unit, in order, by the last CTA that finished one.
+template <int HD, int RW, int WM>
+__device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg, int c0, int c1, int slot0) {
+  constexpr int RT = Shape<HD, RW, WM>::kRows;
+  int news, len;
+  positions<RT>(p, sg.b, sg.rt, &news, &len);
+  const int rows = min(RT, news * p.G - sg.rt * RT);
+  for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+    const int row = i / (HD / 4), c = i % (HD / 4);
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = c0; k <= c1; ++k) {
+      const long long slot = k == c0 ? slot0 : 2 * k;
+      const float2 st = __ldcg(p.stats + slot * RT + row);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part) + (slot * RT + row) * (HD / 4) + c);
+      if (st.y == 0.f) continue;  // no position seen
+      const float mn = fmaxf(M, st.x), a = ex2(M - mn), f = ex2(st.x - mn);
+      M = mn;
+      L = fmaf(L, a, f * st.y);
+      acc.x = fmaf(acc.x, a, f * v.x);
+      acc.y = fmaf(acc.y, a, f * v.y);
+      acc.z = fmaf(acc.z, a, f * v.z);
+      acc.w = fmaf(acc.w, a, f * v.w);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int grow = sg.rt * RT + row, t = grow / p.G, g = grow - t * p.G;
+    uint16_t* dst = p.out + ((long long)sg.b * p.T + t) * p.ld_out + (long long)(sg.kvh * p.G + g) * HD + 4 * c;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+}
+
+template <int HD, int KIND, int RW, int WM>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const __grid_constant__ AttnParams p) {
+  using S = Shape<HD, RW, WM>;
+  constexpr int RT = S::kRows;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long prefix[kMaxEntries + 1];  // position tiles of one kv head before each entry
+  __shared__ long long wsum[kWarps];
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // rows without a position are zeros: each CTA takes its share of the batch's rows
+  for (long long m = blockIdx.x; m < (long long)p.B * p.T; m += gridDim.x) {
+    const int b = (int)(m / p.T), t = (int)(m - (long long)b * p.T);
+    const int nn = p.new_lens ? p.new_lens[b] : p.T;
+    if (t >= nn)
+      for (int i = tid; i < p.hq * HD / 8; i += kThreads)
+        *reinterpret_cast<uint4*>(p.out + m * p.ld_out + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  const long long entries = (long long)p.B * p.row_tiles;
+  if (!p.balanced) {  // whole units
+    for (long long u = blockIdx.x; u < entries * p.hkv; u += gridDim.x) {
+      Segment sg;
+      sg.kvh = (int)(u % p.hkv);
+      const long long e = u / p.hkv;
+      sg.b = (int)(e / p.row_tiles);
+      sg.rt = (int)(e % p.row_tiles);
+      int news, len;
+      const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
+      sg.tile0 = 0;
+      sg.tile1 = (n + kTile - 1) / kTile;
+      if (n > 0) run_segment<HD, KIND, RW, WM>(p, sg, true, 0, smem);
+    }
+    return;
+  }
+  // tiles of each entry and their running sum
+  {
+    const int ne = (int)entries, per = (ne + kThreads - 1) / kThreads, e0 = min(tid * per, ne), e1 = min(e0 + per, ne);
+    long long mine = 0;
+    for (int e = e0; e < e1; ++e) {
+      int news, len;
+      mine += (positions<RT>(p, e / p.row_tiles, e % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    long long at = inc - mine;
+    for (int w = 0; w < warp; ++w) at += wsum[w];
+    for (int e = e0; e < e1; ++e) {
+      int news, len;
+      prefix[e] = at;
+      at += (positions<RT>(p, e / p.row_tiles, e % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+    }
+    if (e1 == ne && e0 < e1) prefix[ne] = at;
+    __syncthreads();
+  }
+  const int ne = (int)entries;
+  const long long total = prefix[ne] * p.hkv;
+  long long per = (total + gridDim.x - 1) / gridDim.x;
+  if (per < kMinTiles) per = kMinTiles;
+  long long at = blockIdx.x * per;
+  const long long end = min(at + per, total);
+  if (at >= end) return;
+  int lo = 0, hi = ne - 1;  // the entry that holds tile `at`: the last with hkv * prefix <= at
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] * p.hkv <= at) lo = mid;
+    else hi = mid - 1;
+  }
+  for (int e = lo; at < end; ++e) {
+    const long long cost = prefix[e + 1] - prefix[e];
+    if (cost == 0) continue;
+    for (int kvh = (int)((at - prefix[e] * p.hkv) / cost); kvh < p.hkv && at < end; ++kvh) {
+      const long long u0 = prefix[e] * p.hkv + kvh * cost, u1 = u0 + cost;
+      Segment sg;
+      sg.b = e / p.row_tiles;
+      sg.rt = e % p.row_tiles;
+      sg.kvh = kvh;
+      sg.tile0 = (int)(at - u0);
+      sg.tile1 = (int)(min(end, u1) - u0);
+      const bool whole = at == u0 && end >= u1;
+      const int slot = 2 * blockIdx.x + (at == blockIdx.x * per ? 0 : 1);
+      run_segment<HD, KIND, RW, WM>(p, sg, whole, slot, smem);
+      if (!whole) {
+        const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          last = atomicAdd(p.counter + c0, 1u) == (unsigned)(c1 - c0);
+          if (last) p.counter[c0] = 0u;  // ready for the next call
+        }
+        __syncthreads();
+        if (last) {
+          __threadfence();
+          join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (u0 == c0 * per ? 0 : 1));
+        }
+        __syncthreads();
+      }
+      at = min(end, u1);
+    }
+  }
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 148;
+}
+
+// Row tile of a call: the smallest of 8, 16, 32, 64 that holds the rows of a kv head, else 64.
+int row_tile(int64_t T, int G) {
+  const int64_t rows = T * G;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+size_t counter_bytes(int grid) { return ((size_t)grid * sizeof(unsigned) + 255) & ~(size_t)255; }
+
+template <int HD, int KIND, int RW, int WM>
+int launch(const AttnParams& p, int grid, cudaStream_t st) {
+  auto kern = kv8_attention_kernel<HD, KIND, RW, WM>;
+  constexpr int smem = Shape<HD, RW, WM>::kSmem;
+  static_assert(smem <= 110 * 1024, "two CTAs per SM");
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return WAL_ERR_CUDA;
+  kern<<<grid, kThreads, smem, st>>>(p);
+  return launch_status();
+}
+
+template <int HD, int KIND>
+int launch_rows(const AttnParams& p, int rows, int grid, cudaStream_t st) {
+  switch (rows) {
+    case 8: return launch<HD, KIND, 8, 1>(p, grid, st);
+    case 16: return launch<HD, KIND, 16, 1>(p, grid, st);
+    case 32: return launch<HD, KIND, 16, 2>(p, grid, st);
+    default: return launch<HD, KIND, 16, 4>(p, grid, st);
   }
 }
 
@@ -80,8 +668,10 @@ __global__ void __launch_bounds__(kThreads) kv8_attention_kernel(const __grid_co
 extern "C" {
 
 size_t wal_kv8_attention_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq) {
-  if (!cache || cache->kv_heads <= 0 || B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads) return 0;
-  return 256;
+  if (!cache || cache->kv_heads <= 0 || B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads || T > 0x7fffffff) return 0;
+  const int grid = sm_count() * kCtasPerSm;
+  const int64_t rows = row_tile(T, hq / cache->kv_heads);
+  return counter_bytes(grid) + (size_t)grid * 2 * rows * (cache->head_dim * sizeof(float) + sizeof(float2));
 }
 
 int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t* q, int64_t ld_q, int64_t B, int64_t T,
@@ -97,18 +687,37 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   if (ld_q < (int64_t)hq * hd || ld_out < (int64_t)hq * hd) return WAL_ERR_SHAPE;
   if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 255) || (ld_q % 8) || (ld_out % 8)) return WAL_ERR_ALIGNMENT;
   if (workspace_bytes < wal_kv8_attention_workspace(cache, B, T, hq)) return WAL_ERR_BUFFER_TOO_SMALL;
-  AttnParams p = {q, ld_q, layer_view(*cache, layer), (int)T, hq, cache->kv_heads, cache->page_size, (int)cache->num_pages,
-                  (int)max_pages, table, ld_table, lens, new_lens, scale * 1.4426950408889634f, out, ld_out};
-  const unsigned grid = (unsigned)(B * T * hq);
+  const int grid = sm_count() * kCtasPerSm;
+  AttnParams p = {};
+  p.q = q;
+  p.ld_q = ld_q;
+  p.kv = layer_view(*cache, layer);
+  p.B = (int)B;
+  p.T = (int)T;
+  p.hq = hq;
+  p.hkv = cache->kv_heads;
+  p.G = hq / cache->kv_heads;
+  p.P = cache->page_size;
+  p.pages = (int)cache->num_pages;
+  p.max_pages = (int)max_pages;
+  const int rows = row_tile(T, p.G);
+  p.row_tiles = (int)((T * p.G + rows - 1) / rows);
+  p.table = table;
+  p.ld_table = ld_table;
+  p.lens = lens;
+  p.new_lens = new_lens;
+  p.qscale = scale * 1.4426950408889634f;  // log2(e)
+  p.out = out;
+  p.ld_out = ld_out;
+  p.balanced = B * p.row_tiles <= kMaxEntries;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.counter = reinterpret_cast<unsigned*>(ws);
+  p.part = reinterpret_cast<float*>(ws + counter_bytes(grid));
+  p.stats = reinterpret_cast<float2*>(p.part + (size_t)grid * 2 * rows * hd);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (hd == 128) {
-    if (cache->kind == WAL_KV_INT8) kv8_attention_kernel<128, WAL_KV_INT8><<<grid, kThreads, 0, s>>>(p);
-    else kv8_attention_kernel<128, WAL_KV_E4M3><<<grid, kThreads, 0, s>>>(p);
-  } else {
-    if (cache->kind == WAL_KV_INT8) kv8_attention_kernel<64, WAL_KV_INT8><<<grid, kThreads, 0, s>>>(p);
-    else kv8_attention_kernel<64, WAL_KV_E4M3><<<grid, kThreads, 0, s>>>(p);
-  }
-  return launch_status();
+  if (hd == 128)
+    return cache->kind == WAL_KV_INT8 ? launch_rows<128, WAL_KV_INT8>(p, rows, grid, s) : launch_rows<128, WAL_KV_E4M3>(p, rows, grid, s);
+  return cache->kind == WAL_KV_INT8 ? launch_rows<64, WAL_KV_INT8>(p, rows, grid, s) : launch_rows<64, WAL_KV_E4M3>(p, rows, grid, s);
 }
 
 }  // extern "C"
