@@ -42,12 +42,16 @@ namespace {
 
 using namespace wal_kv8;
 
+#ifndef CTAS8
+#define CTAS8 3
+#define STAGES8 2
+#endif
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 32;          // positions of a tile
 constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced call
-constexpr int kCtasPerSm = 2;
 constexpr int kMinTiles = 4;       // least position tiles of a run: one per warp
+constexpr float kSlack = 8.f;      // weights may reach 2^8 before the running maximum moves
 
 struct AttnParams {
   const uint16_t* q;
@@ -75,14 +79,14 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -158,19 +162,15 @@ __device__ __forceinline__ void to_bf16(uint32_t w, uint32_t& p0, uint32_t& p1) 
   }
 }
 
-// Byte offset of 16-byte piece c of row r of a tile.  Lines of 128 bytes hold
-// one row (HD 128) or two; the pieces of a line are permuted by a key that
-// differs among the eight rows one matrix load reads together.
+// A tile's rows stand HD bytes apart; their 16-byte pieces are permuted within
+// 128-byte lines by xor with a key of the row, distinct among the eight rows
+// that one matrix load reads together (K: rows 4 * (i / 2) + 2 * (i % 2) + s,
+// V: eight in a row).  Keys are linear in the bits of the row, so that offsets
+// of a lane's rows differ by an xor and an addition of constants.
+__device__ __forceinline__ constexpr uint32_t k_key(int r) { return (uint32_t)((r >> 1) & 7) << 4; }
 template <int HD>
-__device__ __forceinline__ uint32_t k_offset(int r, int c) {
-  const int line = HD == 128 ? r : r >> 1, piece = HD == 128 ? c : ((r & 1) << 2) | c;
-  return (uint32_t)(line * 128 + ((piece ^ ((r >> 1) & 7)) << 4));
-}
-template <int HD>
-__device__ __forceinline__ uint32_t v_offset(int r, int c) {
-  if (HD == 128) return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
-  const int line = r >> 1;
-  return (uint32_t)(line * 128 + (((((r & 1) << 2) | c) ^ (line & 3)) << 4));
+__device__ __forceinline__ constexpr uint32_t v_key(int r) {
+  return (uint32_t)(HD == 128 ? r & 7 : (r >> 1) & 3) << 4;
 }
 
 // RW rows per warp (8 or 16), WM warps per group.
@@ -178,10 +178,11 @@ template <int HD, int RW, int WM>
 struct Shape {
   static constexpr int kRows = RW * WM;         // query rows of a unit
   static constexpr int NS = kWarps / WM;        // warp groups
-  static constexpr int kStages = WM == 4 ? 4 : 3;
+  static constexpr int kCtas = RW == 8 ? CTAS8 : 2;  // per SM
+  static constexpr int kStages = WM == 4 ? 4 : RW == 8 ? STAGES8 : 3;
   static constexpr int kStageBytes = 2 * kTile * HD;  // K rows, then V rows
   static constexpr int kRing = NS * kStages * kStageBytes;
-  static constexpr int LDO = HD + 8;            // padded row of the join buffer
+  static constexpr int LDO = HD + 4;            // padded row of the join buffer
   static constexpr int kJoin = kWarps * RW * LDO * 4;
   static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
   static constexpr int kSmem = kMain + NS * kStages * 32;  // then, per stage: 4 scales and the block mask
@@ -207,7 +208,7 @@ __device__ __forceinline__ int positions(const AttnParams& p, int b, int rt, int
 template <int HD, int KIND, int RW, int WM>
 __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& sg, bool whole, int slot, uint8_t* smem) {
   using S = Shape<HD, RW, WM>;
-  constexpr int KT = HD / 16, NT = HD / 8, C = HD / 16, RT = S::kRows, LDO = S::LDO;
+  constexpr int KT = HD / 16, MT = HD / 16, C = HD / 16, RT = S::kRows, LDO = S::LDO;
   constexpr int HH = RW / 8;  // rows of a lane: r and, of 16, r + 8
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = warp / WM, wm = warp % WM, r = lane >> 2, q4 = lane & 3;
@@ -229,31 +230,41 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   auto pages_of = [&](int tile, int& a, int& b) {
     const int t0 = tile * kTile;
     a = t0 < n ? valid_page(__ldg(trow + (t0 >> psh)), p.pages) : -1;
-    b = t0 + 16 < n ? valid_page(__ldg(trow + ((t0 + 16) >> psh)), p.pages) : -1;
+    b = a;
+    if (p.P == 16 || t0 + 16 >= n) b = t0 + 16 < n ? valid_page(__ldg(trow + ((t0 + 16) >> psh)), p.pages) : -1;
   };
+  constexpr int STEP = 32 * WM / C, PER = kTile / STEP;  // rows that the group copies at once, and how often
+  const int gl = wm * 32 + lane, lrow = gl / C, lpiece = gl % C;
+  const uint32_t kdst = ring + ((uint32_t)(lrow * HD + lpiece * 16) ^ k_key(lrow));
+  const uint32_t vdst = ring + kTile * HD + ((uint32_t)(lrow * HD + lpiece * 16) ^ v_key<HD>(lrow));
+  const int lsrc = lrow * HD + lpiece * 16;
   auto load = [&](int stage, int tile, int pa, int pb) {
     const int t0 = tile * kTile;
-    const uint32_t ks = ring + (uint32_t)(stage * S::kStageBytes), vs = ks + kTile * HD;
-    constexpr int PER = kTile * C / (32 * WM);  // pieces of K per lane
-    const int l = wm * 32 + lane;
+    const uint32_t ks = kdst + (uint32_t)(stage * S::kStageBytes), vs = vdst + (uint32_t)(stage * S::kStageBytes);
+    // source of row 0 of the tile, were it in the page of block 0 or 1; absent blocks read as zeros
+    const long long oa = max(pa, 0) * page_codes + (t0 & (p.P - 1)) * HD + lsrc;
+    const long long ob = max(pb, 0) * page_codes + ((t0 + 16) & (p.P - 1)) * HD - 16 * HD + lsrc;
+    const uint8_t *ka = kbase + oa, *kb = kbase + ob, *va = vbase + oa, *vb = vbase + ob;
+    const uint32_t za = pa >= 0 ? 16u : 0u, zb = pb >= 0 ? 16u : 0u;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int x = i * 32 * WM + l, row = x / C, c = x % C;
-      const int page = row < 16 ? pa : pb;
-      const bool in = page >= 0;
-      const long long off = in ? page * page_codes + (long long)((t0 + row) & (p.P - 1)) * HD + c * 16 : 0;
-      const uint32_t sz = in ? 16u : 0u;  // absent blocks read as zeros
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(ks + k_offset<HD>(row, c)), "l"(kbase + off), "r"(sz));
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(vs + v_offset<HD>(row, c)), "l"(vbase + off), "r"(sz));
+      const bool second = STEP == 32 ? lrow >= 16 : i * STEP >= 16;
+      const uint32_t z = second ? zb : za;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((ks ^ k_key(i * STEP)) + i * STEP * HD), "l"((second ? kb : ka) + i * STEP * HD), "r"(z) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((vs ^ v_key<HD>(i * STEP)) + i * STEP * HD), "l"((second ? vb : va) + i * STEP * HD), "r"(z) : "memory");
     }
     float* sd = side + stage * 8;
-    if (l < 4) {
-      const int page = l & 1 ? pb : pa;
-      const float* src = (l < 2 ? p.kv.ks : p.kv.vs) + (page >= 0 ? (long long)page * p.hkv + sg.kvh : 0);
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(sd + l)), "l"(src), "r"(page >= 0 ? 4u : 0u));
+    if (gl < 4) {
+      const int page = gl & 1 ? pb : pa;
+      const float* src = (gl < 2 ? p.kv.ks : p.kv.vs) + (long long)max(page, 0) * p.hkv + sg.kvh;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(sd + gl)), "l"(src), "r"(page >= 0 ? 4u : 0u) : "memory");
     }
-    if (l == 4) sd[4] = __int_as_float((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
+    if (gl == 4) sd[4] = __int_as_float((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
   };
+  // what this lane addresses for the matrix loads of stage 0
+  const int krow = 4 * ((lane & 7) >> 1) + 2 * (lane & 1);
+  const uint32_t kld = ring + ((uint32_t)(krow * HD + (lane >> 3) * 16) ^ k_key(krow));
+  const uint32_t vld = ring + kTile * HD + ((uint32_t)((lane & 15) * HD + (lane >> 4) * 16) ^ v_key<HD>(lane & 15));
 
   // fill the ring
   const int first = sg.tile0 + grp;
@@ -279,7 +290,7 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   for (int hh = 0; hh < HH; ++hh) {
     const int row = row0 + 8 * hh, t = row / p.G, g = row - t * p.G;
     const bool real = t < news;
-    lim[hh] = real ? (int)min((long long)len + t + 1, (long long)n) : 0;
+    lim[hh] = real ? (int)min((long long)len + t + 1, (long long)n) : n;  // rows that are not there compute something unread
     const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + g) * HD;
     uint2 w[KT];
     float mx = 0.f;
@@ -302,14 +313,16 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
       if (HH == 1) qa[kt][1] = qa[kt][3] = 0u;
     }
   }
-  const int lim_min = HH == 2 ? min(lim[0], lim[HH - 1]) : lim[0];
+  const int lim_min = (int)min((long long)len + sg.rt * RT / p.G + 1, (long long)n);  // the unit's first row's
 
   float m[HH], l[HH], vref = 1e-30f;
 #pragma unroll
   for (int hh = 0; hh < HH; ++hh) m[hh] = -INFINITY, l[hh] = 0.f;
-  float o[NT][4];
+  float o[MT][HH][4];  // output, transposed: dims 16i + r (+ 8), rows 8hh + 2 * q4 (+ 1)
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int hh = 0; hh < HH; ++hh) o[i][hh][0] = o[i][hh][1] = o[i][hh][2] = o[i][hh][3] = 0.f;
 
   int stage = 0;
   for (int tile = first; tile < sg.tile1; tile += S::NS) {
@@ -321,7 +334,7 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
       if (ahead + S::NS < sg.tile1) pages_of(ahead + S::NS, npa, npb);
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
-    const uint32_t ks = ring + (uint32_t)(stage * S::kStageBytes), vs = ks + kTile * HD;
+    const uint32_t ks = kld + (uint32_t)(stage * S::kStageBytes), vs = vld + (uint32_t)(stage * S::kStageBytes);
     const float4 sc = *reinterpret_cast<const float4*>(side + stage * 8);  // K scales, V scales of the two blocks
     const int have = __float_as_int(side[stage * 8 + 4]);
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -331,11 +344,12 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
       s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-      const int i = lane & 7, row = (nt >> 1) * 16 + 4 * (i >> 1) + split_at(nt & 1, i & 1);
+      // the next row of HD 64 is the other half of the line
+      const uint32_t at = (HD == 128 ? ks + (nt & 1) * HD : ks ^ ((nt & 1) * HD)) + (nt >> 1) * 16 * HD;
 #pragma unroll
       for (int c = 0; c < C; c += 4) {
         uint32_t w[4];
-        ldsm_x4(ks + k_offset<HD>(row, c + (lane >> 3)), w);
+        ldsm_x4(at ^ (uint32_t)(c << 4), w);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           uint32_t b0, b1;
@@ -346,42 +360,48 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     }
     const int t0 = tile * kTile;
     const bool edge = have != 3 || t0 + kTile > lim_min;
+#pragma unroll
+    for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s[nt][2 * hh + e] *= unscale[hh] * (nt < 2 ? sc.x : sc.y);
+    if (edge) {
+#pragma unroll
+      for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!((have >> (nt >> 1)) & 1) || t0 + (nt >> 1) * 16 + 4 * q4 + split_at(nt & 1, e) >= lim[hh])
+              s[nt][2 * hh + e] = -INFINITY;
+    }
     float mn[HH];
     bool grew = false;
 #pragma unroll
     for (int hh = 0; hh < HH; ++hh) {
-      mn[hh] = m[hh];
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = s[nt][2 * hh + e];
-          x *= unscale[hh] * (nt < 2 ? sc.x : sc.y);
-          if (edge) {
-            const int pos = t0 + (nt >> 1) * 16 + 4 * q4 + split_at(nt & 1, e);
-            if (!((have >> (nt >> 1)) & 1) || pos >= lim[hh]) x = -INFINITY;
-          }
-          mn[hh] = fmaxf(mn[hh], x);
-        }
+      mn[hh] = fmaxf(fmaxf(s[0][2 * hh], s[0][2 * hh + 1]), fmaxf(s[1][2 * hh], s[1][2 * hh + 1]));
+      mn[hh] = fmaxf(mn[hh], fmaxf(fmaxf(s[2][2 * hh], s[2][2 * hh + 1]), fmaxf(s[3][2 * hh], s[3][2 * hh + 1])));
       mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 1));
       mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 2));
-      grew |= mn[hh] > m[hh];
+      grew |= mn[hh] > m[hh] + kSlack;
     }
-    const float vnew = fmaxf(vref, fmaxf(sc.z, sc.w));
-    if (__any_sync(0xffffffffu, grew || vnew > vref)) {
-      const float vr = vref / vnew;
-      vref = vnew;
+    const float vmax = fmaxf(sc.z, sc.w);
+    if (__any_sync(0xffffffffu, grew || vmax > vref)) {
+      const float vr = vmax > vref ? vref / vmax : 1.f;
+      vref = fmaxf(vref, vmax);
 #pragma unroll
       for (int hh = 0; hh < HH; ++hh) {
-        const float al = mn[hh] == -INFINITY ? 0.f : ex2(m[hh] - mn[hh]);
-        m[hh] = mn[hh];
+        const float top = fmaxf(m[hh], mn[hh]), al = top == -INFINITY ? 0.f : ex2(m[hh] - top), av = al * vr;
+        m[hh] = top;
         l[hh] *= al;
-        const float av = al * vr;
+        const float a0 = __shfl_sync(0xffffffffu, av, 8 * q4), a1 = __shfl_sync(0xffffffffu, av, 8 * q4 + 4);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          o[i][2 * hh] *= av;
-          o[i][2 * hh + 1] *= av;
-          if (HH == 1) o[i][2] *= av, o[i][3] *= av;
+        for (int i = 0; i < MT; ++i) {
+          o[i][hh][0] *= a0;
+          o[i][hh][1] *= a1;
+          o[i][hh][2] *= a0;
+          o[i][hh][3] *= a1;
         }
       }
     }
@@ -398,34 +418,31 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
           s[nt][2 * hh + e] = x * vf[nt >> 1];
         }
     }
-    // P.V, 16 positions at a time; each weight as a bf16 number and the rest of it
+    // V^T P^T, 16 positions at a time; each weight as a bf16 number and the rest of it
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t hi[2 * HH], lo[2 * HH];
+      uint32_t hi[HH][2], lo[HH][2];
 #pragma unroll
       for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float u = s[2 * j + x][2 * hh], v = s[2 * j + x][2 * hh + 1];
-          const uint32_t w = pack_bf16(u, v);
-          hi[x * HH + hh] = w;
-          lo[x * HH + hh] = pack_bf16(u - bf16_lo(w), v - bf16_hi(w));
+          hi[hh][x] = pack_bf16(u, v);
+          lo[hh][x] = pack_bf16(u - bf16_lo(hi[hh][x]), v - bf16_hi(hi[hh][x]));
         }
 #pragma unroll
       for (int c = 0; c < C; c += 2) {
         uint32_t w[4];
-        ldsm_t8_x2(vs + v_offset<HD>(16 * j + (lane & 15), c + (lane >> 4)), w);
+        ldsm_t8_x2((vs ^ (uint32_t)(c << 4)) + j * 16 * HD, w);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t b0, b1;
-          to_bf16<KIND>(w[x], b0, b1);
-          if constexpr (HH == 1) {
-            const uint32_t a[4] = {hi[0], lo[0], hi[1], lo[1]};
-            mma_bf16(o[2 * c + x], a, b0, b1);
-          } else {
-            const uint32_t a[4] = {hi[0], hi[1], hi[2], hi[3]}, b[4] = {lo[0], lo[1], lo[2], lo[3]};
-            mma_bf16(o[2 * c + x], a, b0, b1);
-            mma_bf16(o[2 * c + x], b, b0, b1);
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a[4];
+          to_bf16<KIND>(w[2 * x], a[0], a[2]);
+          to_bf16<KIND>(w[2 * x + 1], a[1], a[3]);
+#pragma unroll
+          for (int hh = 0; hh < HH; ++hh) {
+            mma_bf16(o[c + x][hh], a, hi[hh][0], hi[hh][1]);
+            mma_bf16(o[c + x][hh], a, lo[hh][0], lo[hh][1]);
           }
         }
       }
@@ -444,14 +461,13 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   float* po = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int hh = 0; hh < HH; ++hh) {
-    if (lim[hh] > 0) {
-      float* dst = po + (warp * RW + r + 8 * hh) * LDO + 2 * q4;
+    float* dst = po + (warp * RW + 8 * hh + 2 * q4) * LDO + r;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float x = o[i][2 * hh], y = o[i][2 * hh + 1];
-        if (HH == 1) x += o[i][2], y += o[i][3];
-        *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(x * vref, y * vref);
-      }
+    for (int i = 0; i < MT; ++i) {
+      dst[16 * i] = o[i][hh][0] * vref;
+      dst[16 * i + LDO] = o[i][hh][1] * vref;
+      dst[16 * i + 8] = o[i][hh][2] * vref;
+      dst[16 * i + 8 + LDO] = o[i][hh][3] * vref;
     }
     if (q4 == 0) wstat[warp][r + 8 * hh] = make_float2(m[hh], l[hh]);
   }
@@ -522,7 +538,7 @@ __device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg
 }
 
 template <int HD, int KIND, int RW, int WM>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attention_kernel(const __grid_constant__ AttnParams p) {
   using S = Shape<HD, RW, WM>;
   constexpr int RT = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -540,28 +556,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         *reinterpret_cast<uint4*>(p.out + m * p.ld_out + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
   }
   const long long entries = (long long)p.B * p.row_tiles;
-  if (!p.balanced) {  // whole units
-    for (long long u = blockIdx.x; u < entries * p.hkv; u += gridDim.x) {
-      Segment sg;
-      sg.kvh = (int)(u % p.hkv);
-      const long long e = u / p.hkv;
-      sg.b = (int)(e / p.row_tiles);
-      sg.rt = (int)(e % p.row_tiles);
-      int news, len;
-      const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
-      sg.tile0 = 0;
-      sg.tile1 = (n + kTile - 1) / kTile;
-      if (n > 0) run_segment<HD, KIND, RW, WM>(p, sg, true, 0, smem);
-    }
-    return;
-  }
-  // tiles of each entry and their running sum
-  {
-    const int ne = (int)entries, per = (ne + kThreads - 1) / kThreads, e0 = min(tid * per, ne), e1 = min(e0 + per, ne);
+  const int ne = (int)min(entries, (long long)kMaxEntries);
+  long long per = 0, at = 0, end = 0;  // this CTA's run of position tiles, or of whole units
+  long long e = 0;
+  int kvh = 0;
+  if (p.balanced) {
+    // tiles of each entry and their running sum
+    const int each = (ne + kThreads - 1) / kThreads, e0 = min(tid * each, ne), e1 = min(e0 + each, ne);
     long long mine = 0;
-    for (int e = e0; e < e1; ++e) {
+    for (int i = e0; i < e1; ++i) {
       int news, len;
-      mine += (positions<RT>(p, e / p.row_tiles, e % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+      mine += (positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len) + kTile - 1) / kTile;
     }
     long long inc = mine;
 #pragma unroll
@@ -571,60 +576,81 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    long long at = inc - mine;
-    for (int w = 0; w < warp; ++w) at += wsum[w];
-    for (int e = e0; e < e1; ++e) {
+    long long sum = inc - mine;
+    for (int w = 0; w < warp; ++w) sum += wsum[w];
+    for (int i = e0; i < e1; ++i) {
       int news, len;
-      prefix[e] = at;
-      at += (positions<RT>(p, e / p.row_tiles, e % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+      prefix[i] = sum;
+      sum += (positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len) + kTile - 1) / kTile;
     }
-    if (e1 == ne && e0 < e1) prefix[ne] = at;
+    if (e1 == ne && e0 < e1) prefix[ne] = sum;
     __syncthreads();
+    const long long total = prefix[ne] * p.hkv;
+    per = max((total + gridDim.x - 1) / gridDim.x, (long long)kMinTiles);
+    at = blockIdx.x * per;
+    end = min(at + per, total);
+    if (at >= end) return;
+    int lo = 0, hi = ne - 1;  // the entry that holds tile `at`: the last with hkv * prefix <= at
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] * p.hkv <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    e = lo;
+    kvh = (int)((at - prefix[e] * p.hkv) / (prefix[e + 1] - prefix[e]));
+  } else {
+    at = blockIdx.x;
+    end = entries * p.hkv;
   }
-  const int ne = (int)entries;
-  const long long total = prefix[ne] * p.hkv;
-  long long per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < kMinTiles) per = kMinTiles;
-  long long at = blockIdx.x * per;
-  const long long end = min(at + per, total);
-  if (at >= end) return;
-  int lo = 0, hi = ne - 1;  // the entry that holds tile `at`: the last with hkv * prefix <= at
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] * p.hkv <= at) lo = mid;
-    else hi = mid - 1;
-  }
-  for (int e = lo; at < end; ++e) {
-    const long long cost = prefix[e + 1] - prefix[e];
-    if (cost == 0) continue;
-    for (int kvh = (int)((at - prefix[e] * p.hkv) / cost); kvh < p.hkv && at < end; ++kvh) {
-      const long long u0 = prefix[e] * p.hkv + kvh * cost, u1 = u0 + cost;
-      Segment sg;
-      sg.b = e / p.row_tiles;
-      sg.rt = e % p.row_tiles;
-      sg.kvh = kvh;
+  while (at < end) {
+    Segment sg;
+    long long u0 = 0, u1 = 0;  // the unit's tiles
+    if (p.balanced) {
+      const long long cost = prefix[e + 1] - prefix[e];
+      if (kvh == p.hkv || cost == 0) {
+        ++e;
+        kvh = 0;
+        continue;
+      }
+      u0 = prefix[e] * p.hkv + kvh * cost;
+      u1 = u0 + cost;
       sg.tile0 = (int)(at - u0);
       sg.tile1 = (int)(min(end, u1) - u0);
-      const bool whole = at == u0 && end >= u1;
-      const int slot = 2 * blockIdx.x + (at == blockIdx.x * per ? 0 : 1);
-      run_segment<HD, KIND, RW, WM>(p, sg, whole, slot, smem);
-      if (!whole) {
-        const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          last = atomicAdd(p.counter + c0, 1u) == (unsigned)(c1 - c0);
-          if (last) p.counter[c0] = 0u;  // ready for the next call
-        }
-        __syncthreads();
-        if (last) {
-          __threadfence();
-          join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (u0 == c0 * per ? 0 : 1));
-        }
-        __syncthreads();
-      }
-      at = min(end, u1);
+    } else {
+      e = at / p.hkv;
+      kvh = (int)(at % p.hkv);
     }
+    sg.b = (int)(e / p.row_tiles);
+    sg.rt = (int)(e % p.row_tiles);
+    sg.kvh = kvh;
+    if (!p.balanced) {
+      int news, len;
+      const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
+      at += gridDim.x;
+      if (n == 0) continue;
+      sg.tile0 = 0;
+      sg.tile1 = (n - 1) / kTile + 1;
+    }
+    const bool whole = !p.balanced || (at == u0 && end >= u1);
+    run_segment<HD, KIND, RW, WM>(p, sg, whole, 2 * blockIdx.x + (at == blockIdx.x * per ? 0 : 1), smem);
+    if (!p.balanced) continue;
+    if (!whole) {
+      const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        last = atomicAdd(p.counter + c0, 1u) == (unsigned)(c1 - c0);
+        if (last) p.counter[c0] = 0u;  // ready for the next call
+      }
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (u0 == c0 * per ? 0 : 1));
+      }
+      __syncthreads();
+    }
+    at = min(end, u1);
+    ++kvh;
   }
 }
 
@@ -640,13 +666,16 @@ int row_tile(int64_t T, int G) {
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
+// CTAs that fill the GPU once.
+int grid_of(int rows) { return sm_count() * (rows == 8 ? CTAS8 : 2); }
+
 size_t counter_bytes(int grid) { return ((size_t)grid * sizeof(unsigned) + 255) & ~(size_t)255; }
 
 template <int HD, int KIND, int RW, int WM>
 int launch(const AttnParams& p, int grid, cudaStream_t st) {
   auto kern = kv8_attention_kernel<HD, KIND, RW, WM>;
   constexpr int smem = Shape<HD, RW, WM>::kSmem;
-  static_assert(smem <= 110 * 1024, "two CTAs per SM");
+  static_assert((smem + 10 * 1024) * Shape<HD, RW, WM>::kCtas <= 227 * 1024, "resident CTAs");
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return WAL_ERR_CUDA;
   kern<<<grid, kThreads, smem, st>>>(p);
@@ -669,8 +698,8 @@ extern "C" {
 
 size_t wal_kv8_attention_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq) {
   if (!cache || cache->kv_heads <= 0 || B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads || T > 0x7fffffff) return 0;
-  const int grid = sm_count() * kCtasPerSm;
   const int64_t rows = row_tile(T, hq / cache->kv_heads);
+  const int grid = grid_of((int)rows);
   return counter_bytes(grid) + (size_t)grid * 2 * rows * (cache->head_dim * sizeof(float) + sizeof(float2));
 }
 
@@ -687,7 +716,6 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   if (ld_q < (int64_t)hq * hd || ld_out < (int64_t)hq * hd) return WAL_ERR_SHAPE;
   if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 255) || (ld_q % 8) || (ld_out % 8)) return WAL_ERR_ALIGNMENT;
   if (workspace_bytes < wal_kv8_attention_workspace(cache, B, T, hq)) return WAL_ERR_BUFFER_TOO_SMALL;
-  const int grid = sm_count() * kCtasPerSm;
   AttnParams p = {};
   p.q = q;
   p.ld_q = ld_q;
@@ -700,7 +728,7 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   p.P = cache->page_size;
   p.pages = (int)cache->num_pages;
   p.max_pages = (int)max_pages;
-  const int rows = row_tile(T, p.G);
+  const int rows = row_tile(T, p.G), grid = grid_of(rows);
   p.row_tiles = (int)((T * p.G + rows - 1) / rows);
   p.table = table;
   p.ld_table = ld_table;
