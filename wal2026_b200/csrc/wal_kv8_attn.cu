@@ -53,25 +53,6 @@ constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced c
 constexpr int kMinTiles = 4;       // least position tiles of a run: one per warp
 constexpr float kSlack = 8.f;      // weights may reach 2^8 before the running maximum moves
 
-struct AttnParams {
-  const uint16_t* q;
-  long long ld_q;
-  LayerView kv;
-  int B, T, hq, hkv, G, P, pages, max_pages;
-  int row_tiles;  // per (sequence, kv head)
-  const int* table;
-  long long ld_table;
-  const int* lens;
-  const int* new_lens;
-  float qscale;  // scale * log2(e)
-  uint16_t* out;
-  long long ld_out;
-  unsigned* counter;  // [grid] of the unit that starts in a CTA's run and goes on past it
-  float* part;        // [grid][2][rows][HD]
-  float2* stats;      // [grid][2][rows] (max, sum)
-  bool balanced;
-};
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -105,6 +86,13 @@ __device__ __forceinline__ void ldsm_t8_x2(uint32_t addr, uint32_t (&m)[4]) {
                : "r"(addr));
 }
 
+// The transpose of an 8 x 8 matrix of 16-bit values, two neighbours of a row per lane.
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t v;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
@@ -120,17 +108,28 @@ __host__ __device__ constexpr int k_at(int pair, int e) {
   return KIND == WAL_KV_INT8 ? split_at(pair, e) : 2 * pair + e;
 }
 
+// Bit patterns of the conversions, passed as a parameter: a three-input logic
+// instruction takes one immediate, and two known constants cost a move each time.
+struct Masks {
+  uint32_t low8 = 0x00ff00ffu, f16_128 = 0x64806480u;                       // 1024 + code + 128 as f16
+  uint32_t low7 = 0x007f007fu, bit7 = 0x00800080u, bf16_128 = 0x43004300u;  // 128 as bf16
+};
+
+template <int LUT>
+__device__ __forceinline__ uint32_t lop3(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, %4;" : "=r"(r) : "r"(a), "r"(b), "r"(c), "n"(LUT));
+  return r;
+}
+constexpr int kAndOr = 0xea, kAndXor = 0x6a;  // (a & b) | c, (a & b) ^ c
+
 // K codes as f16.
 template <int KIND>
-__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+__device__ __forceinline__ void to_f16(const Masks& k, uint32_t w, uint32_t& p0, uint32_t& p1) {
   if (KIND == WAL_KV_INT8) {
     // 0x6400 | u is 1024 + u; u = code + 128
-    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));  // 1152
-    const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    p0 = *reinterpret_cast<const uint32_t*>(&x);
-    p1 = *reinterpret_cast<const uint32_t*>(&y);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p0) : "r"(lop3<kAndXor>(w, k.low8, k.f16_128)), "r"(k.f16_128));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p1) : "r"(lop3<kAndXor>(w >> 8, k.low8, k.f16_128)), "r"(k.f16_128));
   } else {
     asm("{.reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n cvt.rn.f16x2.e4m3x2 %1, hi;\n}"
         : "=r"(p0), "=r"(p1)
@@ -144,16 +143,12 @@ __host__ __device__ constexpr float v_unit() {
   return KIND == WAL_KV_INT8 ? 1.f : 1.329227995784916e36f;  // 2^120
 }
 template <int KIND>
-__device__ __forceinline__ void to_bf16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+__device__ __forceinline__ void to_bf16(const Masks& k, uint32_t w, uint32_t& p0, uint32_t& p1) {
   if (KIND == WAL_KV_INT8) {
     // 0x4300 | low seven bits is 128 + them; 0x4300 | sign bit is 128 or 256
-    const uint32_t w1 = w >> 8;
-    const uint32_t a = (w & 0x007f007fu) | 0x43004300u, b = (w & 0x00800080u) | 0x43004300u;
-    const uint32_t c = (w1 & 0x007f007fu) | 0x43004300u, d = (w1 & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(&d));
-    p0 = *reinterpret_cast<const uint32_t*>(&x);
-    p1 = *reinterpret_cast<const uint32_t*>(&y);
+    const uint32_t v = w >> 8;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p0) : "r"(lop3<kAndOr>(w, k.low7, k.bf16_128)), "r"(lop3<kAndOr>(w, k.bit7, k.bf16_128)));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p1) : "r"(lop3<kAndOr>(v, k.low7, k.bf16_128)), "r"(lop3<kAndOr>(v, k.bit7, k.bf16_128)));
   } else {
     // exponent and fraction bits moved to bf16's: the value times 2^(7 - 127),
     // subnormals included, and finite for every byte
@@ -161,6 +156,26 @@ __device__ __forceinline__ void to_bf16(uint32_t w, uint32_t& p0, uint32_t& p1) 
     p1 = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);
   }
 }
+
+struct AttnParams {
+  const uint16_t* q;
+  long long ld_q;
+  LayerView kv;
+  int B, T, hq, hkv, G, P, pages, max_pages;
+  int row_tiles;  // per (sequence, kv head)
+  const int* table;
+  long long ld_table;
+  const int* lens;
+  const int* new_lens;
+  float qscale;  // scale * log2(e)
+  uint16_t* out;
+  long long ld_out;
+  unsigned* counter;  // [grid] of the unit that starts in a CTA's run and goes on past it
+  float* part;        // [grid][2][rows][HD]
+  float2* stats;      // [grid][2][rows] (max, sum)
+  bool balanced;
+  Masks masks;
+};
 
 // A tile's rows stand HD bytes apart; their 16-byte pieces are permuted within
 // 128-byte lines by xor with a key of the row, distinct among the eight rows
@@ -262,8 +277,8 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     if (gl == 4) sd[4] = __int_as_float((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
   };
   // what this lane addresses for the matrix loads of stage 0
-  const int krow = 4 * ((lane & 7) >> 1) + 2 * (lane & 1);
-  const uint32_t kld = ring + ((uint32_t)(krow * HD + (lane >> 3) * 16) ^ k_key(krow));
+  const int krow = 4 * ((lane & 7) >> 1) + split_at(lane >> 4, lane & 1);
+  const uint32_t kld = ring + ((uint32_t)(krow * HD + ((lane >> 3) & 1) * 16) ^ k_key(krow));
   const uint32_t vld = ring + kTile * HD + ((uint32_t)((lane & 15) * HD + (lane >> 4) * 16) ^ v_key<HD>(lane & 15));
 
   // fill the ring
@@ -281,16 +296,15 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   int npa = -1, npb = -1;  // pages of the next tile to load
   if (first + (S::kStages - 1) * S::NS < sg.tile1) pages_of(first + (S::kStages - 1) * S::NS, npa, npb);
 
-  // q: rows r and r + 8 of this warp's, scaled by powers of two into f16
-  const int row0 = sg.rt * RT + wm * RW + r;
-  uint32_t qa[KT][4];
-  float unscale[HH];
-  int lim[HH];  // positions each row attends to
+  // q rows 8hh + r as the B operand, scaled by powers of two into f16
+  const int row0 = sg.rt * RT + wm * RW;
+  uint32_t qb[KT][HH][2];
+  float unscale[HH][2], m[HH][2], l[HH][2], vref = 1e-30f;  // of rows 8hh + 2 * q4 + e, as the scores below
+  int lim[HH][2];                                           // positions those rows attend to
 #pragma unroll
   for (int hh = 0; hh < HH; ++hh) {
-    const int row = row0 + 8 * hh, t = row / p.G, g = row - t * p.G;
+    const int row = row0 + 8 * hh + r, t = row / p.G, g = row - t * p.G;
     const bool real = t < news;
-    lim[hh] = real ? (int)min((long long)len + t + 1, (long long)n) : n;  // rows that are not there compute something unread
     const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + g) * HD;
     uint2 w[KT];
     float mx = 0.f;
@@ -303,27 +317,31 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     // 2^e with mx * 2^e in [2^14, 2^15), kept within normal floats
     const int e = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-    unscale[hh] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23), un = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       const float x[4] = {bf16_lo(w[kt].x) * up, bf16_hi(w[kt].x) * up, bf16_lo(w[kt].y) * up, bf16_hi(w[kt].y) * up};
-      qa[kt][hh] = pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]);
-      qa[kt][2 + hh] = pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]);
-      if (HH == 1) qa[kt][1] = qa[kt][3] = 0u;
+      qb[kt][hh][0] = pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]);
+      qb[kt][hh][1] = pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      unscale[hh][x] = __shfl_sync(0xffffffffu, un, 8 * q4 + 4 * x);
+      const int tt = (row0 + 8 * hh + 2 * q4 + x) / p.G;
+      lim[hh][x] = tt < news ? (int)min((long long)len + tt + 1, (long long)n) : n;  // rows that are not there compute something unread
+      m[hh][x] = -INFINITY;
+      l[hh][x] = 0.f;
     }
   }
   const int lim_min = (int)min((long long)len + sg.rt * RT / p.G + 1, (long long)n);  // the unit's first row's
 
-  float m[HH], l[HH], vref = 1e-30f;
-#pragma unroll
-  for (int hh = 0; hh < HH; ++hh) m[hh] = -INFINITY, l[hh] = 0.f;
   float o[MT][HH][4];  // output, transposed: dims 16i + r (+ 8), rows 8hh + 2 * q4 (+ 1)
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int hh = 0; hh < HH; ++hh) o[i][hh][0] = o[i][hh][1] = o[i][hh][2] = o[i][hh][3] = 0.f;
 
+  const Masks mk = p.masks;
   int stage = 0;
   for (int tile = first; tile < sg.tile1; tile += S::NS) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(S::kStages - 2) : "memory");
@@ -339,85 +357,88 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     const int have = __float_as_int(side[stage * 8 + 4]);
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
-    // scores: n-tile 2j + s, column c is position 16j + 4 * (c / 2) + split_at(s, c % 2)
-    float s[4][4];
+    // scores, transposed: s[j][hh][2h + e] is position 16j + 4 * (r / 2) + split_at(h, r % 2), row 8hh + 2 * q4 + e
+    float s[2][HH][4];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-      // the next row of HD 64 is the other half of the line
-      const uint32_t at = (HD == 128 ? ks + (nt & 1) * HD : ks ^ ((nt & 1) * HD)) + (nt >> 1) * 16 * HD;
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int c = 0; c < C; c += 4) {
-        uint32_t w[4];
-        ldsm_x4(at ^ (uint32_t)(c << 4), w);
+      for (int hh = 0; hh < HH; ++hh) s[j][hh][0] = s[j][hh][1] = s[j][hh][2] = s[j][hh][3] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t b0, b1;
-          to_f16<KIND>(w[x], b0, b1);
-          mma_f16(s[nt], qa[c + x], b0, b1);
+      for (int c = 0; c < C; c += 2) {
+        uint32_t w[4];  // pieces c, c + 1 of rows h = 0, then of rows h = 1
+        ldsm_x4((ks ^ (uint32_t)(c << 4)) + j * 16 * HD, w);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a[4];
+          to_f16<KIND>(mk, w[x], a[0], a[2]);
+          to_f16<KIND>(mk, w[2 + x], a[1], a[3]);
+#pragma unroll
+          for (int hh = 0; hh < HH; ++hh) mma_f16(s[j][hh], a, qb[c + x][hh][0], qb[c + x][hh][1]);
         }
       }
     }
     const int t0 = tile * kTile;
-    const bool edge = have != 3 || t0 + kTile > lim_min;
+    bool grew = false;
 #pragma unroll
     for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s[nt][2 * hh + e] *= unscale[hh] * (nt < 2 ? sc.x : sc.y);
-    if (edge) {
+        for (int e = 0; e < 4; ++e) s[j][hh][e] *= unscale[hh][e & 1] * (j == 0 ? sc.x : sc.y);
+    if (have != 3 || t0 + kTile > lim_min) {
 #pragma unroll
       for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!((have >> (nt >> 1)) & 1) || t0 + (nt >> 1) * 16 + 4 * q4 + split_at(nt & 1, e) >= lim[hh])
-              s[nt][2 * hh + e] = -INFINITY;
+          for (int e = 0; e < 4; ++e)
+            if (!((have >> j) & 1) || t0 + 16 * j + 4 * (r >> 1) + split_at(e >> 1, r & 1) >= lim[hh][e & 1])
+              s[j][hh][e] = -INFINITY;
     }
-    float mn[HH];
-    bool grew = false;
+    float mn[HH][2];  // over this lane's positions
 #pragma unroll
-    for (int hh = 0; hh < HH; ++hh) {
-      mn[hh] = fmaxf(fmaxf(s[0][2 * hh], s[0][2 * hh + 1]), fmaxf(s[1][2 * hh], s[1][2 * hh + 1]));
-      mn[hh] = fmaxf(mn[hh], fmaxf(fmaxf(s[2][2 * hh], s[2][2 * hh + 1]), fmaxf(s[3][2 * hh], s[3][2 * hh + 1])));
-      mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 1));
-      mn[hh] = fmaxf(mn[hh], __shfl_xor_sync(0xffffffffu, mn[hh], 2));
-      grew |= mn[hh] > m[hh] + kSlack;
-    }
+    for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mn[hh][e] = fmaxf(fmaxf(s[0][hh][e], s[0][hh][2 + e]), fmaxf(s[1][hh][e], s[1][hh][2 + e]));
+        grew |= mn[hh][e] > m[hh][e] + kSlack;
+      }
     const float vmax = fmaxf(sc.z, sc.w);
     if (__any_sync(0xffffffffu, grew || vmax > vref)) {
       const float vr = vmax > vref ? vref / vmax : 1.f;
       vref = fmaxf(vref, vmax);
 #pragma unroll
       for (int hh = 0; hh < HH; ++hh) {
-        const float top = fmaxf(m[hh], mn[hh]), al = top == -INFINITY ? 0.f : ex2(m[hh] - top), av = al * vr;
-        m[hh] = top;
-        l[hh] *= al;
-        const float a0 = __shfl_sync(0xffffffffu, av, 8 * q4), a1 = __shfl_sync(0xffffffffu, av, 8 * q4 + 4);
+        float av[2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          o[i][hh][0] *= a0;
-          o[i][hh][1] *= a1;
-          o[i][hh][2] *= a0;
-          o[i][hh][3] *= a1;
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(m[hh][e], mn[hh][e]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float al = top == -INFINITY ? 0.f : ex2(m[hh][e] - top);
+          m[hh][e] = top;
+          l[hh][e] *= al;
+          av[e] = al * vr;
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][hh][e] *= av[e & 1];
       }
     }
     const float vinv = 1.f / vref, vf[2] = {sc.z * vinv * v_unit<KIND>(), sc.w * vinv * v_unit<KIND>()};
 #pragma unroll
-    for (int hh = 0; hh < HH; ++hh) {
-      const float base = m[hh] == -INFINITY ? 0.f : m[hh];
+    for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int e = 0; e < 4; ++e) {
+        const float base = m[hh][e & 1] == -INFINITY ? 0.f : m[hh][e & 1];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = ex2(s[nt][2 * hh + e] - base);
-          l[hh] += x;
-          s[nt][2 * hh + e] = x * vf[nt >> 1];
+        for (int j = 0; j < 2; ++j) {
+          const float x = ex2(s[j][hh][e] - base);
+          l[hh][e & 1] += x;
+          s[j][hh][e] = x * vf[j];
         }
-    }
+      }
     // V^T P^T, 16 positions at a time; each weight as a bf16 number and the rest of it
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -426,9 +447,10 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
       for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float u = s[2 * j + x][2 * hh], v = s[2 * j + x][2 * hh + 1];
-          hi[hh][x] = pack_bf16(u, v);
-          lo[hh][x] = pack_bf16(u - bf16_lo(hi[hh][x]), v - bf16_hi(hi[hh][x]));
+          const float u = s[j][hh][2 * x], v = s[j][hh][2 * x + 1];
+          const uint32_t w = pack_bf16(u, v);
+          hi[hh][x] = transpose(w);
+          lo[hh][x] = transpose(pack_bf16(u - bf16_lo(w), v - bf16_hi(w)));
         }
 #pragma unroll
       for (int c = 0; c < C; c += 2) {
@@ -437,8 +459,8 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           uint32_t a[4];
-          to_bf16<KIND>(w[2 * x], a[0], a[2]);
-          to_bf16<KIND>(w[2 * x + 1], a[1], a[3]);
+          to_bf16<KIND>(mk, w[2 * x], a[0], a[2]);
+          to_bf16<KIND>(mk, w[2 * x + 1], a[1], a[3]);
 #pragma unroll
           for (int hh = 0; hh < HH; ++hh) {
             mma_bf16(o[c + x][hh], a, hi[hh][0], hi[hh][1]);
@@ -450,10 +472,11 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 #pragma unroll
-  for (int hh = 0; hh < HH; ++hh) {
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-  }
+  for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[hh][e] += __shfl_xor_sync(0xffffffffu, l[hh][e], x);
 
   // join the warp groups: outputs and (max, sum) of every warp's rows
   __shared__ float2 wstat[kWarps][RW];
@@ -469,7 +492,10 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
       dst[16 * i + 8] = o[i][hh][2] * vref;
       dst[16 * i + 8 + LDO] = o[i][hh][3] * vref;
     }
-    if (q4 == 0) wstat[warp][r + 8 * hh] = make_float2(m[hh], l[hh]);
+    if (r == 0) {
+      wstat[warp][8 * hh + 2 * q4] = make_float2(m[hh][0], l[hh][0]);
+      wstat[warp][8 * hh + 2 * q4 + 1] = make_float2(m[hh][1], l[hh][1]);
+    }
   }
   __syncthreads();
   const int rows = min(RT, news * p.G - sg.rt * RT);
