@@ -42,15 +42,12 @@ namespace {
 
 using namespace wal_kv8;
 
-#ifndef CTAS8
-#define CTAS8 3
-#define STAGES8 2
-#endif
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 32;          // positions of a tile
 constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced call
 constexpr int kMinTiles = 4;       // least position tiles of a run: one per warp
+constexpr int kUnitCost = 8;      // what starting and ending a unit costs, in tiles
 constexpr float kSlack = 8.f;      // weights may reach 2^8 before the running maximum moves
 
 __device__ __forceinline__ float ex2(float x) {
@@ -188,25 +185,29 @@ __device__ __forceinline__ constexpr uint32_t v_key(int r) {
   return (uint32_t)(HD == 128 ? r & 7 : (r >> 1) & 3) << 4;
 }
 
-// RW rows per warp (8 or 16), WM warps per group.
+// RW rows per warp (8, 16 or 24), WM warps per group.
 template <int HD, int RW, int WM>
 struct Shape {
   static constexpr int kRows = RW * WM;         // query rows of a unit
   static constexpr int NS = kWarps / WM;        // warp groups
-  static constexpr int kCtas = RW == 8 ? CTAS8 : 2;  // per SM
-  static constexpr int kStages = WM == 4 ? 4 : RW == 8 ? STAGES8 : 3;
+  static constexpr int kCtas = RW == 8 ? 3 : 2;  // per SM
+  static constexpr int kStages = WM == 4 ? 4 : RW == 8 ? 2 : 3;
   static constexpr int kStageBytes = 2 * kTile * HD;  // K rows, then V rows
   static constexpr int kRing = NS * kStages * kStageBytes;
   static constexpr int LDO = HD + 4;            // padded row of the join buffer
   static constexpr int kJoin = kWarps * RW * LDO * 4;
   static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kSmem = kMain + NS * kStages * 32;  // then, per stage: 4 scales and the block mask
+  static constexpr int kSide = NS * kStages * 32;     // per stage: 4 scales and the block mask
+  static constexpr int kQ = kRows * HD * 2;           // q as B fragments: [row / 8][dim / 16][lane] 8 bytes
+  static constexpr int kSmem = kMain + kSide + kQ + kRows * 4;  // then what undoes each row's scaling
 };
 
 struct Segment {
   int b, rt, kvh;    // unit
   int tile0, tile1;  // position tiles
 };
+
+__device__ __forceinline__ int unit_cost(int n) { return n ? (n - 1) / kTile + 1 + kUnitCost : 0; }
 
 // Attended positions of sequence b by its last real token of row tile rt; 0 where the tile has none.
 template <int RT>
@@ -224,7 +225,7 @@ template <int HD, int KIND, int RW, int WM>
 __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& sg, bool whole, int slot, uint8_t* smem) {
   using S = Shape<HD, RW, WM>;
   constexpr int KT = HD / 16, MT = HD / 16, C = HD / 16, RT = S::kRows, LDO = S::LDO;
-  constexpr int HH = RW / 8;  // rows of a lane: r and, of 16, r + 8
+  constexpr int HH = RW / 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = warp / WM, wm = warp % WM, r = lane >> 2, q4 = lane & 3;
   int news, len;
@@ -296,14 +297,14 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   int npa = -1, npb = -1;  // pages of the next tile to load
   if (first + (S::kStages - 1) * S::NS < sg.tile1) pages_of(first + (S::kStages - 1) * S::NS, npa, npb);
 
-  // q rows 8hh + r as the B operand, scaled by powers of two into f16
-  const int row0 = sg.rt * RT + wm * RW;
-  uint32_t qb[KT][HH][2];
-  float unscale[HH][2], m[HH][2], l[HH][2], vref = 1e-30f;  // of rows 8hh + 2 * q4 + e, as the scores below
-  int lim[HH][2];                                           // positions those rows attend to
+  // q rows as the B operand, scaled by powers of two into f16; warps take 8 rows in turn
+  uint2* const qs = reinterpret_cast<uint2*>(smem + S::kMain + S::kSide);
+  float* const un = reinterpret_cast<float*>(smem + S::kMain + S::kSide + S::kQ);
 #pragma unroll
-  for (int hh = 0; hh < HH; ++hh) {
-    const int row = row0 + 8 * hh + r, t = row / p.G, g = row - t * p.G;
+  for (int i = 0; i < (RT / 8 + kWarps - 1) / kWarps; ++i) {
+    const int rg = i * kWarps + warp;
+    if (rg >= RT / 8) break;
+    const int row = sg.rt * RT + 8 * rg + r, t = row / p.G, g = row - t * p.G;
     const bool real = t < news;
     const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + g) * HD;
     uint2 w[KT];
@@ -317,22 +318,29 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     // 2^e with mx * 2^e in [2^14, 2^15), kept within normal floats
     const int e = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23), un = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    if (q4 == 0) un[8 * rg + r] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       const float x[4] = {bf16_lo(w[kt].x) * up, bf16_hi(w[kt].x) * up, bf16_lo(w[kt].y) * up, bf16_hi(w[kt].y) * up};
-      qb[kt][hh][0] = pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]);
-      qb[kt][hh][1] = pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]);
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      unscale[hh][x] = __shfl_sync(0xffffffffu, un, 8 * q4 + 4 * x);
-      const int tt = (row0 + 8 * hh + 2 * q4 + x) / p.G;
-      lim[hh][x] = tt < news ? (int)min((long long)len + tt + 1, (long long)n) : n;  // rows that are not there compute something unread
-      m[hh][x] = -INFINITY;
-      l[hh][x] = 0.f;
+      qs[(rg * KT + kt) * 32 + lane] = make_uint2(pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]),
+                                                  pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]));
     }
   }
+  __syncthreads();
+  const uint2* const qw = qs + wm * HH * KT * 32 + lane;
+  float unscale[HH][2], m[HH][2], l[HH][2], vref = 1e-30f;  // of rows 8hh + 2 * q4 + e, as the scores below
+  int lim[HH][2];                                           // positions those rows attend to
+#pragma unroll
+  for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = wm * RW + 8 * hh + 2 * q4 + e, t = (sg.rt * RT + row) / p.G;
+      unscale[hh][e] = un[row];
+      lim[hh][e] = t < news ? (int)min((long long)len + t + 1, (long long)n) : n;  // rows that are not there compute something unread
+      m[hh][e] = -INFINITY;
+      l[hh][e] = 0.f;
+    }
   const int lim_min = (int)min((long long)len + sg.rt * RT / p.G + 1, (long long)n);  // the unit's first row's
 
   float o[MT][HH][4];  // output, transposed: dims 16i + r (+ 8), rows 8hh + 2 * q4 (+ 1)
@@ -360,20 +368,26 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     // scores, transposed: s[j][hh][2h + e] is position 16j + 4 * (r / 2) + split_at(h, r % 2), row 8hh + 2 * q4 + e
     float s[2][HH][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int hh = 0; hh < HH; ++hh) s[j][hh][0] = s[j][hh][1] = s[j][hh][2] = s[j][hh][3] = 0.f;
 #pragma unroll
-      for (int c = 0; c < C; c += 2) {
-        uint32_t w[4];  // pieces c, c + 1 of rows h = 0, then of rows h = 1
-        ldsm_x4((ks ^ (uint32_t)(c << 4)) + j * 16 * HD, w);
+    for (int c = 0; c < C; c += 2) {
+      uint32_t w[2][4];  // pieces c, c + 1 of rows h = 0, then of rows h = 1
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+      for (int j = 0; j < 2; ++j) ldsm_x4((ks ^ (uint32_t)(c << 4)) + j * 16 * HD, w[j]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint2 qf[HH];
+#pragma unroll
+        for (int hh = 0; hh < HH; ++hh) qf[hh] = qw[(hh * KT + c + x) * 32];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
           uint32_t a[4];
-          to_f16<KIND>(mk, w[x], a[0], a[2]);
-          to_f16<KIND>(mk, w[2 + x], a[1], a[3]);
+          to_f16<KIND>(mk, w[j][x], a[0], a[2]);
+          to_f16<KIND>(mk, w[j][2 + x], a[1], a[3]);
 #pragma unroll
-          for (int hh = 0; hh < HH; ++hh) mma_f16(s[j][hh], a, qb[c + x][hh][0], qb[c + x][hh][1]);
+          for (int hh = 0; hh < HH; ++hh) mma_f16(s[j][hh], a, qf[hh].x, qf[hh].y);
         }
       }
     }
@@ -542,19 +556,28 @@ __device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg
     const int row = i / (HD / 4), c = i % (HD / 4);
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = c0; k <= c1; ++k) {
-      const long long slot = k == c0 ? slot0 : 2 * k;
-      const float2 st = __ldcg(p.stats + slot * RT + row);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part) + (slot * RT + row) * (HD / 4) + c);
-      if (st.y == 0.f) continue;  // no position seen
-      const float mn = fmaxf(M, st.x), a = ex2(M - mn), f = ex2(st.x - mn);
-      M = mn;
-      L = fmaf(L, a, f * st.y);
-      acc.x = fmaf(acc.x, a, f * v.x);
-      acc.y = fmaf(acc.y, a, f * v.y);
-      acc.z = fmaf(acc.z, a, f * v.z);
-      acc.w = fmaf(acc.w, a, f * v.w);
+    constexpr int N = 8;  // runs whose loads are in flight together
+    for (int k0 = c0; k0 <= c1; k0 += N) {
+      float2 st[N];
+      float4 v[N];
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int k = min(k0 + x, c1);
+        const long long slot = k == c0 ? slot0 : 2 * k;
+        st[x] = __ldcg(p.stats + slot * RT + row);
+        v[x] = __ldcg(reinterpret_cast<const float4*>(p.part) + (slot * RT + row) * (HD / 4) + c);
+      }
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        if (k0 + x > c1 || st[x].y == 0.f) continue;  // no position seen
+        const float mn = fmaxf(M, st[x].x), a = ex2(M - mn), f = ex2(st[x].x - mn);
+        M = mn;
+        L = fmaf(L, a, f * st[x].y);
+        acc.x = fmaf(acc.x, a, f * v[x].x);
+        acc.y = fmaf(acc.y, a, f * v[x].y);
+        acc.z = fmaf(acc.z, a, f * v[x].z);
+        acc.w = fmaf(acc.w, a, f * v[x].w);
+      }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int grow = sg.rt * RT + row, t = grow / p.G, g = grow - t * p.G;
@@ -568,19 +591,13 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
   using S = Shape<HD, RW, WM>;
   constexpr int RT = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long prefix[kMaxEntries + 1];  // position tiles of one kv head before each entry
+  __shared__ unsigned prefix[kMaxEntries + 1];  // cost of one kv head before each entry
   __shared__ long long wsum[kWarps];
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  // rows without a position are zeros: each CTA takes its share of the batch's rows
-  for (long long m = blockIdx.x; m < (long long)p.B * p.T; m += gridDim.x) {
-    const int b = (int)(m / p.T), t = (int)(m - (long long)b * p.T);
-    const int nn = p.new_lens ? p.new_lens[b] : p.T;
-    if (t >= nn)
-      for (int i = tid; i < p.hq * HD / 8; i += kThreads)
-        *reinterpret_cast<uint4*>(p.out + m * p.ld_out + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
-  }
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const long long entries = (long long)p.B * p.row_tiles;
   const int ne = (int)min(entries, (long long)kMaxEntries);
   long long per = 0, at = 0, end = 0;  // this CTA's run of position tiles, or of whole units
@@ -592,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
     long long mine = 0;
     for (int i = e0; i < e1; ++i) {
       int news, len;
-      mine += (positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+      mine += unit_cost(positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len));
     }
     long long inc = mine;
 #pragma unroll
@@ -606,31 +623,31 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
     for (int w = 0; w < warp; ++w) sum += wsum[w];
     for (int i = e0; i < e1; ++i) {
       int news, len;
-      prefix[i] = sum;
-      sum += (positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len) + kTile - 1) / kTile;
+      prefix[i] = (unsigned)sum;
+      sum += unit_cost(positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len));
     }
-    if (e1 == ne && e0 < e1) prefix[ne] = sum;
+    if (e1 == ne && e0 < e1) prefix[ne] = (unsigned)sum;
     __syncthreads();
-    const long long total = prefix[ne] * p.hkv;
+    const long long total = (long long)prefix[ne] * p.hkv;
     per = max((total + gridDim.x - 1) / gridDim.x, (long long)kMinTiles);
     at = blockIdx.x * per;
     end = min(at + per, total);
-    if (at >= end) return;
     int lo = 0, hi = ne - 1;  // the entry that holds tile `at`: the last with hkv * prefix <= at
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] * p.hkv <= at) lo = mid;
+      if ((long long)prefix[mid] * p.hkv <= at) lo = mid;
       else hi = mid - 1;
     }
     e = lo;
-    kvh = (int)((at - prefix[e] * p.hkv) / (prefix[e + 1] - prefix[e]));
+    if (at < end) kvh = (int)((at - (long long)prefix[e] * p.hkv) / (prefix[e + 1] - prefix[e]));
   } else {
     at = blockIdx.x;
     end = entries * p.hkv;
   }
   while (at < end) {
     Segment sg;
-    long long u0 = 0, u1 = 0;  // the unit's tiles
+    long long r0 = 0, u1 = 0, stop = 0;  // the unit's first tile and end, this CTA's end in it
+    bool whole = true, leads = false;
     if (p.balanced) {
       const long long cost = prefix[e + 1] - prefix[e];
       if (kvh == p.hkv || cost == 0) {
@@ -638,45 +655,52 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
         kvh = 0;
         continue;
       }
-      u0 = prefix[e] * p.hkv + kvh * cost;
-      u1 = u0 + cost;
-      sg.tile0 = (int)(at - u0);
-      sg.tile1 = (int)(min(end, u1) - u0);
+      r0 = (long long)prefix[e] * p.hkv + kvh * cost + kUnitCost;
+      u1 = r0 + cost - kUnitCost;
+      stop = min(end, u1);
+      const long long s0 = max(at, r0);
+      at = stop;
+      sg.kvh = kvh++;
+      if (s0 >= stop) continue;
+      sg.tile0 = (int)(s0 - r0);
+      sg.tile1 = (int)(stop - r0);
+      whole = s0 == r0 && stop == u1;
+      leads = s0 == blockIdx.x * per;
     } else {
       e = at / p.hkv;
-      kvh = (int)(at % p.hkv);
+      sg.kvh = (int)(at % p.hkv);
+      at += gridDim.x;
     }
     sg.b = (int)(e / p.row_tiles);
     sg.rt = (int)(e % p.row_tiles);
-    sg.kvh = kvh;
     if (!p.balanced) {
       int news, len;
       const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
-      at += gridDim.x;
       if (n == 0) continue;
       sg.tile0 = 0;
       sg.tile1 = (n - 1) / kTile + 1;
     }
-    const bool whole = !p.balanced || (at == u0 && end >= u1);
-    run_segment<HD, KIND, RW, WM>(p, sg, whole, 2 * blockIdx.x + (at == blockIdx.x * per ? 0 : 1), smem);
-    if (!p.balanced) continue;
+    run_segment<HD, KIND, RW, WM>(p, sg, whole, 2 * blockIdx.x + (leads ? 0 : 1), smem);
     if (!whole) {
-      const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
+      const int c0 = (int)(r0 / per), c1 = (int)((u1 - 1) / per);
+      if (tid == 0) {  // the other threads' stores came before the barrier that ended run_segment
+        __threadfence();
         last = atomicAdd(p.counter + c0, 1u) == (unsigned)(c1 - c0);
         if (last) p.counter[c0] = 0u;  // ready for the next call
+        __threadfence();
       }
       __syncthreads();
-      if (last) {
-        __threadfence();
-        join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (u0 == c0 * per ? 0 : 1));
-      }
+      if (last) join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (r0 == c0 * per ? 0 : 1));
       __syncthreads();
     }
-    at = min(end, u1);
-    ++kvh;
+  }
+  // rows without a position are zeros: each CTA takes its share of the batch's rows
+  for (long long m = blockIdx.x; m < (long long)p.B * p.T; m += gridDim.x) {
+    const int b = (int)(m / p.T), t = (int)(m - (long long)b * p.T);
+    const int nn = p.new_lens ? p.new_lens[b] : p.T;
+    if (t >= nn)
+      for (int i = tid; i < p.hq * HD / 8; i += kThreads)
+        *reinterpret_cast<uint4*>(p.out + m * p.ld_out + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -686,14 +710,17 @@ int sm_count() {
   return sms > 0 ? sms : 148;
 }
 
-// Row tile of a call: the smallest of 8, 16, 32, 64 that holds the rows of a kv head, else 64.
+// Row tile of a call: the smallest of 8, 16, 24, 32, 48, 64 that holds the rows
+// of a kv head; beyond, 64 or 96, whichever pads them less.
 int row_tile(int64_t T, int G) {
   const int64_t rows = T * G;
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  for (int t : {8, 16, 24, 32, 48, 64})
+    if (rows <= t) return t;
+  return (rows + 95) / 96 * 96 <= (rows + 63) / 64 * 64 ? 96 : 64;
 }
 
 // CTAs that fill the GPU once.
-int grid_of(int rows) { return sm_count() * (rows == 8 ? CTAS8 : 2); }
+int grid_of(int rows) { return sm_count() * (rows == 8 ? 3 : 2); }
 
 size_t counter_bytes(int grid) { return ((size_t)grid * sizeof(unsigned) + 255) & ~(size_t)255; }
 
@@ -701,10 +728,20 @@ template <int HD, int KIND, int RW, int WM>
 int launch(const AttnParams& p, int grid, cudaStream_t st) {
   auto kern = kv8_attention_kernel<HD, KIND, RW, WM>;
   constexpr int smem = Shape<HD, RW, WM>::kSmem;
-  static_assert((smem + 10 * 1024) * Shape<HD, RW, WM>::kCtas <= 227 * 1024, "resident CTAs");
+  static_assert((smem + 6 * 1024) * Shape<HD, RW, WM>::kCtas <= 227 * 1024, "resident CTAs");
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return WAL_ERR_CUDA;
-  kern<<<grid, kThreads, smem, st>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return WAL_ERR_CUDA;
   return launch_status();
 }
 
@@ -713,8 +750,11 @@ int launch_rows(const AttnParams& p, int rows, int grid, cudaStream_t st) {
   switch (rows) {
     case 8: return launch<HD, KIND, 8, 1>(p, grid, st);
     case 16: return launch<HD, KIND, 16, 1>(p, grid, st);
+    case 24: return launch<HD, KIND, 24, 1>(p, grid, st);
     case 32: return launch<HD, KIND, 16, 2>(p, grid, st);
-    default: return launch<HD, KIND, 16, 4>(p, grid, st);
+    case 48: return launch<HD, KIND, 24, 2>(p, grid, st);
+    case 64: return launch<HD, KIND, 16, 4>(p, grid, st);
+    default: return launch<HD, KIND, 24, 4>(p, grid, st);
   }
 }
 
@@ -763,7 +803,8 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   p.qscale = scale * 1.4426950408889634f;  // log2(e)
   p.out = out;
   p.ld_out = ld_out;
-  p.balanced = B * p.row_tiles <= kMaxEntries;
+  // the sums of costs fit 32 bits, whatever the lengths
+  p.balanced = B * p.row_tiles <= kMaxEntries && B * p.row_tiles * (max_pages * p.P / kTile + 1 + kUnitCost) < (1LL << 32);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counter = reinterpret_cast<unsigned*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes(grid));
