@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace wal_kv8 {
 
 // One layer's half (K or V) of the cache: codes [pages][hkv][P][hd], scales [pages][hkv].
@@ -82,7 +84,47 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return v;
 }
 
-// The device a pointer's kernel must run on is the caller's current device.
-inline int launch_status() { return cudaGetLastError() == cudaSuccess ? WAL_OK : WAL_ERR_CUDA; }
+// Programmatic dependent launch: a kernel waits for the grids before it in the
+// stream before it touches memory, and lets the next one start launching.
+__device__ __forceinline__ void chain() {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
+constexpr int kMaxDevices = 64;
+
+// SM count of the current device, looked up once per device.
+inline int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Launches kern(p) in the chain.
+template <typename Kern, typename Params>
+int launch_chain(Kern kern, dim3 grid, int threads, int smem, cudaStream_t stream, const Params& p, int cluster = 0) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)(cluster > 0 ? cluster : 1);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return WAL_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? WAL_OK : WAL_ERR_CUDA;
+}
 
 }  // namespace wal_kv8

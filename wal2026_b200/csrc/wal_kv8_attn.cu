@@ -596,8 +596,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  chain();
   const long long entries = (long long)p.B * p.row_tiles;
   const int ne = (int)min(entries, (long long)kMaxEntries);
   long long per = 0, at = 0, end = 0;  // this CTA's run of position tiles, or of whole units
@@ -704,12 +703,6 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 148;
-}
-
 // Row tile of a call: the smallest of 8, 16, 24, 32, 48, 64 that holds the rows
 // of a kv head; beyond, 64 or 96, whichever pads them less.
 int row_tile(int64_t T, int G) {
@@ -726,23 +719,17 @@ size_t counter_bytes(int grid) { return ((size_t)grid * sizeof(unsigned) + 255) 
 
 template <int HD, int KIND, int RW, int WM>
 int launch(const AttnParams& p, int grid, cudaStream_t st) {
-  auto kern = kv8_attention_kernel<HD, KIND, RW, WM>;
   constexpr int smem = Shape<HD, RW, WM>::kSmem;
   static_assert((smem + 6 * 1024) * Shape<HD, RW, WM>::kCtas <= 227 * 1024, "resident CTAs");
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return WAL_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return WAL_ERR_CUDA;
-  return launch_status();
+  auto kern = kv8_attention_kernel<HD, KIND, RW, WM>;
+  static std::atomic<uint64_t> allowed{0};  // devices where the kernel may use its shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WAL_ERR_CUDA;
+  if (!(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return WAL_ERR_CUDA;
+    allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  return launch_chain(kern, dim3((unsigned)grid), kThreads, smem, st, p);
 }
 
 template <int HD, int KIND>

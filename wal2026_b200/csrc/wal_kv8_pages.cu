@@ -1,26 +1,33 @@
 // Pages of the 8-bit KV cache: the tables of the next step (kept, forked,
 // freed and new pages), compaction, and the copies both ask for.
 //
-//   kv_pages_assign_kernel   one CTA.  Counts the references that the kept
-//                            prefixes make to each page, decides which partly
-//                            filled last pages need a copy before they are
-//                            written, and hands out free pages in rising order
-//                            to the rows in rising order.  All counts are
-//                            integers, so the result does not depend on the
-//                            order of the atomics.
-//   kv_pages_compact_kernel  one CTA.  Used pages beyond the live count move to
-//                            the free pages below it, both in rising order.
+//   kv_pages_assign_kernel   Counts the references that the kept prefixes make
+//                            to each page, decides which partly filled last
+//                            pages need a copy before they are written, and
+//                            hands out free pages in rising order to the rows
+//                            in rising order.  All counts are integers, so the
+//                            result does not depend on the order of the atomics.
+//   kv_pages_compact_kernel  Used pages beyond the live count move to the free
+//                            pages below it, both in rising order.
 //   kv_pages_copy_kernel     page src[i] -> dst[i] in every layer, K, V, scales.
+//
+// The first two are one cluster each, of one CTA for small pools and of eight
+// for large ones: what they do is a few dependent passes over a few hundred
+// kilobytes, bound by the latency of the passes and of the barriers between.
 #include "wal_kv8.cuh"
+
+#include <cooperative_groups.h>
 
 namespace {
 
+namespace cg = cooperative_groups;
 using namespace wal_kv8;
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
+constexpr int kCluster = 8;
 
-// Exclusive prefix sum over the CTA; *total gets the sum.  sm: kWarps + 1 ints.
+// Exclusive prefix sum over the CTA; *total gets the sum.  sm: kWarps ints.
 __device__ __forceinline__ int block_scan(int v, int* sm, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
@@ -45,6 +52,25 @@ __device__ __forceinline__ int block_scan(int v, int* sm, int* total) {
   *total = sm[kWarps - 1];
   return x - v + (warp ? sm[warp - 1] : 0);
 }
+
+// The same over the cluster, by rank; `box` (kCluster ints) is not used again by the kernel.  Ends with a cluster barrier.
+__device__ __forceinline__ int cluster_scan(cg::cluster_group& cl, int v, int* sm, int* box, int* total) {
+  const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
+  int mine;
+  int at = block_scan(v, sm, &mine);
+  if (threadIdx.x < ncta) cl.map_shared_rank(box, threadIdx.x)[rank] = mine;
+  cl.sync();
+  int sum = 0;
+  for (int i = 0; i < ncta; ++i) {
+    if (i < rank) at += box[i];
+    sum += box[i];
+  }
+  *total = sum;
+  return at;
+}
+
+// Chunks of kChunk entries of the rows of a table, one per warp at a time.
+constexpr int kChunk = 128;
 
 struct AssignParams {
   const int* table;
@@ -89,31 +115,43 @@ __device__ __forceinline__ Row load_row(const AssignParams& p, int b) {
 }
 
 __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_constant__ AssignParams p) {
-  extern __shared__ int begin[];  // [rows + 1] first wanted page of each row
-  __shared__ int scan[kWarps];
+  extern __shared__ int begin[];  // [rows + 1] first wanted page of each row, then a bit per row that copies
+  __shared__ int scan[kWarps], box[2][kCluster];
   __shared__ int lost;
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gtid = rank * kThreads + tid, gthreads = ncta * kThreads, gwarp = rank * kWarps + warp, gwarps = ncta * kWarps;
+  unsigned* const copies = reinterpret_cast<unsigned*>(begin + p.rows + 1);
+  chain();
   if (tid == 0) lost = 0;
-  for (int i = tid; i < p.pages; i += kThreads) p.ref[i] = 0u;
-  __syncthreads();
+  for (int i = gtid; i < p.pages; i += gthreads) p.ref[i] = 0u;
+  for (int i = tid; i < (p.rows + 31) / 32; i += kThreads) copies[i] = 0u;
+  cl.sync();
   // kept entries and their references
-  for (int b = warp; b < p.rows; b += kWarps) {
+  const int per_row = (p.width + kChunk - 1) / kChunk;
+  for (long long u = gwarp; u < (long long)p.rows * per_row; u += gwarps) {
+    const int b = (int)(u / per_row), j0 = (int)(u % per_row) * kChunk + lane;
     const Row r = load_row(p, b);
-    for (int j = lane; j < p.width; j += 32) {
-      int e = -1;
-      if (j < r.have) {
-        e = valid_page(p.table[(long long)r.parent * p.ld_table + j], p.pages);
-        if (e >= 0) atomicAdd(p.ref + e, r.writes && j == r.have - 1 ? 0x10001u : 1u);
-      }
-      p.out[(long long)b * p.ld_out + j] = e;
+    int e[kChunk / 32];
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i) {
+      const int j = j0 + 32 * i;
+      e[i] = j < r.have ? valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + j), p.pages) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i) {
+      const int j = j0 + 32 * i;
+      if (e[i] >= 0) atomicAdd(p.ref + e[i], r.writes && j == r.have - 1 ? 0x10001u : 1u);
+      if (j < p.width) p.out[(long long)b * p.ld_out + j] = e[i];
     }
   }
-  __syncthreads();
-  // rows that write: sole owner, one of writers only, or beside readers
-  for (int b = tid; b < p.rows; b += kThreads) {
+  cl.sync();
+  // rows that write: sole owner, one of writers only (2), or beside readers (1)
+  for (int b = gtid; b < p.rows; b += gthreads) {
     const Row r = load_row(p, b);
-    const int e = r.writes ? p.out[(long long)b * p.ld_out + r.have - 1] : -1;
-    int kind = 0;  // 1: copies, 2: copies unless it is the lowest writer
+    const int e = r.writes ? valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + r.have - 1), p.pages) : -1;
+    int kind = 0;
     if (e >= 0) {
       const unsigned w = __ldcg(p.ref + e), total = w & 0xffffu, writers = w >> 16;
       if (total > 1) kind = total == writers ? 2 : 1;
@@ -121,88 +159,84 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
     p.src[b] = e;
     p.dst[b] = kind;
   }
-  __syncthreads();
-  for (int b = tid; b < p.rows; b += kThreads)
+  cl.sync();
+  for (int b = gtid; b < p.rows; b += gthreads)
     if (p.dst[b] == 2) atomicMax(p.ref + p.src[b], kFlag | (kRowMask - (unsigned)b));
-  __syncthreads();
-  // wanted pages of each row: its copy, then the new ones
+  cl.sync();
+  // wanted pages of each row: its copy, then the new ones (every CTA for itself)
   int base = 0;
   for (int b0 = 0; b0 < p.rows; b0 += kThreads) {
     const int b = b0 + tid;
     int n = 0, total;
     if (b < p.rows) {
       const Row r = load_row(p, b);
-      bool cow = p.dst[b] == 1;
-      if (p.dst[b] == 2) cow = (kRowMask - (__ldcg(p.ref + p.src[b]) & kRowMask)) != (unsigned)b;
+      const int kind = __ldcg(p.dst + b);
+      bool cow = kind == 1;
+      if (kind == 2) cow = (kRowMask - (__ldcg(p.ref + __ldcg(p.src + b)) & kRowMask)) != (unsigned)b;
       n = (cow ? 1 : 0) + r.want - r.have;
-      if (!cow) p.src[b] = -1;
-      p.dst[b] = -1;
+      if (cow) atomicOr(copies + (b >> 5), 1u << (b & 31));
       const long long over = ((long long)r.keep + r.add + p.P - 1) / p.P - r.want;
       if (r.add && over > 0) atomicAdd(&lost, (int)min(over, 0x3fffffffLL));
     }
     const int at = block_scan(n, scan, &total);
     if (b < p.rows) begin[b] = base + at;
     base += total;
-    __syncthreads();
   }
   if (tid == 0) begin[p.rows] = base;
   __syncthreads();
-  // free pages in rising order to wanted ones in rising order; final counts
-  int given = 0, left = 0;
-  for (int i0 = 0; i0 < p.pages; i0 += kThreads) {
-    const int i = i0 + tid;
-    unsigned w = 1u;
-    if (i < p.pages) w = __ldcg(p.ref + i);
-    int total;
-    const int k = given + block_scan(w == 0u, scan, &total);
-    if (i < p.pages) {
-      int count;
-      if (w == 0u) {
-        count = k < base;
-        left += !count;
-        if (count) {
-          int lo = 0, hi = p.rows - 1;  // the last row whose first wanted page is <= k
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (begin[mid] <= k) lo = mid;
-            else hi = mid - 1;
-          }
-          const Row r = load_row(p, lo);
-          int s = k - begin[lo];
-          const bool cow = p.src[lo] >= 0;
-          if (cow && s == 0) p.dst[lo] = i;
-          const int j = cow ? r.have - 1 + s : r.have + s;
-          p.out[(long long)lo * p.ld_out + j] = i;
-        }
-      } else if (w & kFlag) {
-        count = 1;
-      } else {
-        const int t = w & 0xffffu, writers = w >> 16;
-        count = t == writers ? 1 : t - writers;
-      }
-      p.ref[i] = (unsigned)count;
+  // free pages in rising order to wanted ones in rising order; final counts.  Each thread has a run of pages.
+  const int each = (p.pages + gthreads - 1) / gthreads, i0 = (int)min((long long)gtid * each, (long long)p.pages), i1 = min(i0 + each, p.pages);
+  int mine = 0, found, unused;
+  for (int i = i0; i < i1; ++i) mine += __ldcg(p.ref + i) == 0u;
+  int k = cluster_scan(cl, mine, scan, box[0], &found);  // from here on no CTA reads src or dst
+  if (rank == 0)
+    for (int b = tid; b < p.rows; b += kThreads) {
+      const bool cow = copies[b >> 5] >> (b & 31) & 1u;
+      if (!cow || begin[b] >= found) p.src[b] = -1;
+      if (!cow || begin[b] >= found) p.dst[b] = -1;
     }
-    given += total;
-    __syncthreads();
+  for (int i = i0; i < i1; ++i) {
+    const unsigned w = __ldcg(p.ref + i);
+    int count;
+    if (w == 0u) {
+      count = k < base;
+      if (count) {
+        int lo = 0, hi = p.rows - 1;  // the last row whose first wanted page is <= k
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (begin[mid] <= k) lo = mid;
+          else hi = mid - 1;
+        }
+        const Row r = load_row(p, lo);
+        const int s = k - begin[lo];
+        const bool cow = copies[lo >> 5] >> (lo & 31) & 1u;
+        if (cow && s == 0) p.dst[lo] = i;
+        p.out[(long long)lo * p.ld_out + (cow ? r.have - 1 + s : r.have + s)] = i;
+      }
+      ++k;
+    } else if (w & kFlag) {
+      count = 1;
+    } else {
+      const int t = w & 0xffffu, writers = w >> 16;
+      count = t == writers ? 1 : t - writers;
+    }
+    p.ref[i] = (unsigned)count;
   }
   // what found no page
-  if (given < base) {
-    for (int b = tid; b < p.rows; b += kThreads)
-      if (begin[b + 1] > given) {
+  if (found < base)
+    for (int b = gtid; b < p.rows; b += gthreads)
+      if (begin[b + 1] > found) {
         const Row r = load_row(p, b);
-        const bool cow = p.src[b] >= 0;
-        for (int k = max(begin[b], given); k < begin[b + 1]; ++k) {
-          const int s = k - begin[b];
+        const bool cow = copies[b >> 5] >> (b & 31) & 1u;
+        for (int x = max(begin[b], found); x < begin[b + 1]; ++x) {
+          const int s = x - begin[b];
           p.out[(long long)b * p.ld_out + (cow ? r.have - 1 + s : r.have + s)] = -1;
-          if (cow && s == 0) p.src[b] = -1;
         }
       }
-  }
-  int total;
-  block_scan(left, scan, &total);
-  if (tid == 0) {
-    p.info[0] = total;
-    p.info[1] = lost + (given < base ? base - given : 0);
+  if (rank == 0 && tid == 0) {
+    unused = max(found - base, 0);
+    p.info[0] = unused;
+    p.info[1] = lost + max(base - found, 0);
   }
 }
 
@@ -220,51 +254,66 @@ struct CompactParams {
 };
 
 __global__ void __launch_bounds__(kThreads) kv_pages_compact_kernel(const __grid_constant__ CompactParams p) {
-  __shared__ int scan[kWarps];
+  __shared__ int scan[kWarps], box[3][kCluster];
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < p.pages; i += kThreads) {
+  const int gtid = rank * kThreads + tid, gthreads = ncta * kThreads, gwarp = rank * kWarps + warp, gwarps = ncta * kWarps;
+  chain();
+  for (int i = gtid; i < p.pages; i += gthreads) {
     p.remap[i] = -1;
     p.src[i] = -1;
     p.dst[i] = -1;
   }
-  __syncthreads();
-  for (int b = warp; b < p.rows; b += kWarps) {
+  cl.sync();
+  const int per_row = (p.width + kChunk - 1) / kChunk;
+  for (long long u = gwarp; u < (long long)p.rows * per_row; u += gwarps) {
+    const int b = (int)(u / per_row), j0 = (int)(u % per_row) * kChunk + lane;
     const int have = (min(max(p.lens[b], 0), p.width * p.P) + p.P - 1) / p.P;
-    for (int j = lane; j < have; j += 32) {
-      const int e = valid_page(p.table[(long long)b * p.ld_table + j], p.pages);
-      if (e >= 0) p.remap[e] = 0;
-    }
+    int e[kChunk / 32];
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i)
+      e[i] = j0 + 32 * i < have ? valid_page(p.table[(long long)b * p.ld_table + j0 + 32 * i], p.pages) : -1;
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i)
+      if (e[i] >= 0) p.remap[e[i]] = 0;
   }
-  __syncthreads();
-  int mine = 0, live;
-  for (int i = tid; i < p.pages; i += kThreads) mine += __ldcg(p.remap + i) >= 0;
-  block_scan(mine, scan, &live);
-  int movers = 0, holes = 0;
-  for (int i0 = 0; i0 < p.pages; i0 += kThreads) {
-    const int i = i0 + tid;
-    const bool used = i < p.pages && __ldcg(p.remap + i) >= 0;
-    const bool mover = used && i >= live, hole = i < p.pages && !used && i < live;
-    int total;
-    const int km = movers + block_scan(mover, scan, &total);
-    movers += total;
-    __syncthreads();
-    const int kh = holes + block_scan(hole, scan, &total);
-    holes += total;
-    if (mover) p.src[km] = i;
-    if (hole) p.dst[kh] = i;
+  cl.sync();
+  // each thread has a run of pages
+  const int each = (p.pages + gthreads - 1) / gthreads, i0 = (int)min((long long)gtid * each, (long long)p.pages), i1 = min(i0 + each, p.pages);
+  int mine = 0, live, movers, holes;
+  for (int i = i0; i < i1; ++i) mine += __ldcg(p.remap + i) >= 0;
+  const int used_before = cluster_scan(cl, mine, scan, box[0], &live);
+  // holes below `live` and movers from there on follow from the used pages before a page
+  int u = used_before, beyond = 0;
+  for (int i = i0; i < i1; ++i) beyond += i >= live && __ldcg(p.remap + i) >= 0;
+  int km = cluster_scan(cl, beyond, scan, box[1], &movers);
+  for (int i = i0; i < i1; ++i) {
+    const bool used = __ldcg(p.remap + i) >= 0;
+    if (used && i >= live) p.src[km++] = i;
+    if (!used && i < live) p.dst[i - u] = i;
     if (used) p.remap[i] = i;
-    __syncthreads();
+    u += used;
   }
-  for (int k = tid; k < movers; k += kThreads) p.remap[p.src[k]] = p.dst[k];
-  __syncthreads();
-  for (int b = warp; b < p.rows; b += kWarps) {
+  holes = movers;  // as many as there are movers
+  cl.sync();
+  for (int k = gtid; k < holes; k += gthreads) p.remap[__ldcg(p.src + k)] = __ldcg(p.dst + k);
+  cl.sync();
+  for (long long x = gwarp; x < (long long)p.rows * per_row; x += gwarps) {
+    const int b = (int)(x / per_row), j0 = (int)(x % per_row) * kChunk + lane;
     const int have = (min(max(p.lens[b], 0), p.width * p.P) + p.P - 1) / p.P;
-    for (int j = lane; j < p.width; j += 32) {
-      const int e = j < have ? valid_page(p.table[(long long)b * p.ld_table + j], p.pages) : -1;
-      p.out[(long long)b * p.ld_out + j] = e >= 0 ? __ldcg(p.remap + e) : -1;
-    }
+    int e[kChunk / 32];
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i)
+      e[i] = j0 + 32 * i < have ? valid_page(p.table[(long long)b * p.ld_table + j0 + 32 * i], p.pages) : -1;
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i)
+      if (e[i] >= 0) e[i] = __ldcg(p.remap + e[i]);
+#pragma unroll
+    for (int i = 0; i < kChunk / 32; ++i)
+      if (j0 + 32 * i < p.width) p.out[(long long)b * p.ld_out + j0 + 32 * i] = e[i];
   }
-  if (tid == 0) {
+  if (rank == 0 && tid == 0) {
     p.info[0] = live;
     p.info[1] = movers;
   }
@@ -282,32 +331,65 @@ struct CopyParams {
 
 constexpr int kCopyThreads = 256;
 constexpr int kSegBytes = kCopyThreads * 16;  // bytes that one CTA copies of one page and plane
+constexpr int kCopyBatch = 8;                 // pairs whose loads are in flight together
+constexpr int kRun = 4 * kCopyThreads;        // pairs that a CTA looks through at a time
 
-// grid.x: segments of a plane's page x planes (layer, K or V); grid.y: runs of 32 pairs.
+// grid.x: segments of a plane's page x planes (layer, K or V); grid.y: runs of
+// pairs; grid.z: shares of a run's pairs.
 __global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const __grid_constant__ CopyParams p) {
-  const int seg = blockIdx.x % p.segs, plane = blockIdx.x / p.segs, lane = threadIdx.x & 31;
-  for (int i0 = blockIdx.y * 32; i0 < p.n; i0 += gridDim.y * 32) {
-    int s = -1, d = -1;
-    if (i0 + lane < p.n) {
-      s = valid_page(p.src[i0 + lane], p.pages);
-      d = valid_page(p.dst[i0 + lane], p.pages);
+  __shared__ int2 list[kRun];
+  __shared__ int counts[kRun / 32];
+  const int seg = blockIdx.x % p.segs, plane = blockIdx.x / p.segs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* const base = p.codes + plane * p.half_bytes + (long long)seg * kSegBytes + tid * 16;
+  float* const sc = p.scales + plane * p.half_scales;
+  const bool mine = (long long)seg * kSegBytes + tid * 16 < p.page_bytes;
+  chain();
+  for (int i0 = blockIdx.y * kRun; i0 < p.n; i0 += gridDim.y * kRun) {
+    int s[4], d[4];
+    unsigned todo[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = i0 + x * kCopyThreads + tid;
+      s[x] = i < p.n ? valid_page(p.src[i], p.pages) : -1;
+      d[x] = i < p.n ? valid_page(p.dst[i], p.pages) : -1;
     }
-    unsigned todo = __ballot_sync(0xffffffffu, s >= 0 && d >= 0);
-    while (todo) {
-      const int l = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const long long sp = __shfl_sync(0xffffffffu, s, l), dp = __shfl_sync(0xffffffffu, d, l);
-      uint8_t* base = p.codes + plane * p.half_bytes;
-      const long long off = (long long)seg * kSegBytes + threadIdx.x * 16;
-      if (off < p.page_bytes)
-        *reinterpret_cast<uint4*>(base + dp * p.page_bytes + off) = *reinterpret_cast<const uint4*>(base + sp * p.page_bytes + off);
-      if (seg == 0) {
-        float* sc = p.scales + plane * p.half_scales;
-        for (int h = threadIdx.x; h < p.hkv; h += kCopyThreads) sc[dp * p.hkv + h] = sc[sp * p.hkv + h];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      todo[x] = __ballot_sync(0xffffffffu, s[x] >= 0 && d[x] >= 0);
+      if (lane == 0) counts[x * (kCopyThreads / 32) + warp] = __popc(todo[x]);
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int w = 0; w < kCopyThreads / 32; ++w) {
+        if (w == warp && (todo[x] >> lane & 1u)) list[total + __popc(todo[x] & ((1u << lane) - 1u))] = make_int2(s[x], d[x]);
+        total += counts[x * (kCopyThreads / 32) + w];
       }
+    __syncthreads();
+    for (int k = blockIdx.z; k < total; k += kCopyBatch * gridDim.z) {
+      uint4 v[kCopyBatch];
+#pragma unroll
+      for (int i = 0; i < kCopyBatch; ++i)
+        if (mine && k + i * (int)gridDim.z < total)
+          v[i] = __ldcs(reinterpret_cast<const uint4*>(base + list[k + i * gridDim.z].x * p.page_bytes));
+#pragma unroll
+      for (int i = 0; i < kCopyBatch; ++i)
+        if (mine && k + i * (int)gridDim.z < total)
+          __stcs(reinterpret_cast<uint4*>(base + list[k + i * gridDim.z].y * p.page_bytes), v[i]);
+      if (seg == 0)
+        for (int i = 0; i < kCopyBatch && k + i * (int)gridDim.z < total; ++i) {
+          const long long sp = list[k + i * gridDim.z].x, dp = list[k + i * gridDim.z].y;
+          for (int h = tid; h < p.hkv; h += kCopyThreads) sc[dp * p.hkv + h] = sc[sp * p.hkv + h];
+        }
     }
+    __syncthreads();
   }
 }
+
+// CTAs of the table kernels' cluster.
+int table_cluster(int64_t entries, int64_t pages) { return entries + pages > 4 * kThreads ? kCluster : 1; }
 
 }  // namespace
 
@@ -325,11 +407,11 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   AssignParams p = {table, ld_table, (int)rows_in, parent, keep, add, (int)rows, (int)width, (int)num_pages, page_size,
                     table_out, ld_out, reinterpret_cast<unsigned*>(ref_out), copy_src, copy_dst, info};
-  const int smem = ((int)rows + 1) * (int)sizeof(int);
+  const int smem = ((int)rows + 1 + ((int)rows + 31) / 32) * (int)sizeof(int);
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kv_pages_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return WAL_ERR_CUDA;
-  kv_pages_assign_kernel<<<1, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status();
+  const int cluster = table_cluster(rows * width, num_pages);
+  return launch_chain(kv_pages_assign_kernel, dim3((unsigned)cluster), kThreads, smem, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
 int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* lens, int64_t rows, int64_t width,
@@ -341,8 +423,8 @@ int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* 
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   CompactParams p = {table, ld_table, lens, (int)rows, (int)width, (int)num_pages, page_size, table_out, ld_out, remap,
                      move_src, move_dst, info};
-  kv_pages_compact_kernel<<<1, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status();
+  const int cluster = table_cluster(rows * width, num_pages);
+  return launch_chain(kv_pages_compact_kernel, dim3((unsigned)cluster), kThreads, 0, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
 int wal_kv_pages_copy(const wal_kv8_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
@@ -365,10 +447,14 @@ int wal_kv_pages_copy(const wal_kv8_cache* cache, const int32_t* src, const int3
   p.n = (int)n;
   const long long gx = (long long)p.planes * p.segs;
   if (gx > 0x7fffffff) return WAL_ERR_SHAPE;
-  const long long runs = (n + 31) / 32;
-  const dim3 grid((unsigned)gx, (unsigned)(runs < 1024 ? runs : 1024));
-  kv_pages_copy_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status();
+  // about sixteen CTAs per SM: up to eight runs side by side, then shares of a run
+  const long long want = 16LL * sm_count(), runs = (n + kRun - 1) / kRun;
+  const long long gy = runs < 8 ? runs : 8;
+  long long gz = want / (gx * gy);
+  gz = gz < 1 ? 1 : gz > 64 ? 64 : gz;
+  if (gz > n) gz = n;
+  const dim3 grid((unsigned)gx, (unsigned)gy, (unsigned)gz);
+  return launch_chain(kv_pages_copy_kernel, grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 }  // extern "C"

@@ -50,20 +50,30 @@ __device__ __forceinline__ Pair load_pair(const uint16_t* src, int c) {
   return p;
 }
 
+// Cosines and sines of the angles of dims [8c, 8c + 8) at a position.
+struct Angles {
+  float c[8], s[8];
+};
+
 template <int HD>
-__device__ __forceinline__ void rotate(Pair& p, const float* cos, const float* sin, int pos, int c) {
+__device__ __forceinline__ Angles load_angles(const float* cos, const float* sin, int pos, int c) {
+  Angles g;
   const float4* cp = reinterpret_cast<const float4*>(cos + (long long)pos * (HD / 2) + 8 * c);
   const float4* sp = reinterpret_cast<const float4*>(sin + (long long)pos * (HD / 2) + 8 * c);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const float4 cv = __ldg(cp + h), sv = __ldg(sp + h);
-    const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, ss[4] = {sv.x, sv.y, sv.z, sv.w};
+    *reinterpret_cast<float4*>(g.c + 4 * h) = __ldg(cp + h);
+    *reinterpret_cast<float4*>(g.s + 4 * h) = __ldg(sp + h);
+  }
+  return g;
+}
+
+__device__ __forceinline__ void rotate(Pair& p, const Angles& g) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = p.a[4 * h + i], y = p.b[4 * h + i];
-      p.a[4 * h + i] = __fadd_rn(__fmul_rn(x, cc[i]), __fmul_rn(-y, ss[i]));
-      p.b[4 * h + i] = __fadd_rn(__fmul_rn(y, cc[i]), __fmul_rn(x, ss[i]));
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float x = p.a[i], y = p.b[i];
+    p.a[i] = __fadd_rn(__fmul_rn(x, g.c[i]), __fmul_rn(-y, g.s[i]));
+    p.b[i] = __fadd_rn(__fmul_rn(y, g.c[i]), __fmul_rn(x, g.s[i]));
   }
 }
 
@@ -84,31 +94,48 @@ __device__ __forceinline__ float finite_abs(float x) {
 
 constexpr int kThreads = 128;
 
+// Query heads that a warp rotates.
+template <int HD>
+__host__ __device__ constexpr int kHeads() {
+  return 4 * 32 / (HD / 16);
+}
+
 template <int HD, int P, int KIND>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int C = HD / 16;                              // 16-value pieces per token and head
   constexpr int IT = (P * C + kThreads - 1) / kThreads;   // pieces per thread of a whole page
   const int tid = threadIdx.x;
-  if (blockIdx.x >= p.kv_ctas) {  // q rows
-    const long long i = (long long)(blockIdx.x - p.kv_ctas) * kThreads + tid;
-    const int c = (int)(i % C);
-    const long long mh = i / C;
-    const int h = (int)(mh % p.hq);
-    const long long m = mh / p.hq;
-    if (m >= (long long)p.B * p.T) return;
-    const int b = (int)(m / p.T), t = (int)(m - (long long)b * p.T);
+  chain();
+  if (blockIdx.x >= p.kv_ctas) {  // q rows: a warp rotates up to kHeads heads of one token by one load of its angles
+    constexpr int H = 32 / C, kIter = kHeads<HD>() / H;
+    const int lane = tid & 31, c = lane % C, groups = (p.hq + kHeads<HD>() - 1) / kHeads<HD>();
+    const unsigned w = (blockIdx.x - p.kv_ctas) * (kThreads / 32) + (tid >> 5);
+    const unsigned m = w / groups, h0 = (w - m * groups) * kHeads<HD>() + lane / C;
+    if (m >= (unsigned)(p.B * p.T)) return;
+    const int b = (int)m / p.T, t = (int)m - b * p.T;
     const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
     const long long pos = (long long)max(p.lens[b], 0) + t;
-    uint16_t* dst = p.q_out + m * p.ld_q + (long long)h * HD + 8 * c;
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (t < nn && (!p.cos || pos < p.max_pos)) {
-      Pair x = load_pair<HD>(p.qkv + m * p.ld + (long long)h * HD, c);
-      if (p.cos) rotate<HD>(x, p.cos, p.sin, (int)pos, c);
-      lo = make_uint4(pack_bf16(x.a[0], x.a[1]), pack_bf16(x.a[2], x.a[3]), pack_bf16(x.a[4], x.a[5]), pack_bf16(x.a[6], x.a[7]));
-      hi = make_uint4(pack_bf16(x.b[0], x.b[1]), pack_bf16(x.b[2], x.b[3]), pack_bf16(x.b[4], x.b[5]), pack_bf16(x.b[6], x.b[7]));
+    const bool real = t < nn && (!p.cos || pos < p.max_pos);
+    const uint16_t* src = p.qkv + (long long)m * p.ld + h0 * HD;
+    uint16_t* dst = p.q_out + (long long)m * p.ld_q + h0 * HD + 8 * c;
+    Pair x[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (real && h0 + i * H < (unsigned)p.hq) x[i] = load_pair<HD>(src + i * H * HD, c);
+    Angles g;
+    if (real && p.cos) g = load_angles<HD>(p.cos, p.sin, (int)pos, c);
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      if (h0 + i * H >= (unsigned)p.hq) break;
+      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+      if (real) {
+        if (p.cos) rotate(x[i], g);
+        lo = make_uint4(pack_bf16(x[i].a[0], x[i].a[1]), pack_bf16(x[i].a[2], x[i].a[3]), pack_bf16(x[i].a[4], x[i].a[5]), pack_bf16(x[i].a[6], x[i].a[7]));
+        hi = make_uint4(pack_bf16(x[i].b[0], x[i].b[1]), pack_bf16(x[i].b[2], x[i].b[3]), pack_bf16(x[i].b[4], x[i].b[5]), pack_bf16(x[i].b[6], x[i].b[7]));
+      }
+      *reinterpret_cast<uint4*>(dst + i * H * HD) = lo;
+      *reinterpret_cast<uint4*>(dst + i * H * HD + HD / 2) = hi;
     }
-    *reinterpret_cast<uint4*>(dst) = lo;
-    *reinterpret_cast<uint4*>(dst + HD / 2) = hi;
     return;
   }
   const int kv = blockIdx.x & 1;
@@ -137,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     const int i = it * kThreads + tid, t = i / C, c = i % C;
     if (t < cnt) {
       x[it] = load_pair<HD>(src + (long long)t * p.ld, c);
-      if (kv == 0 && p.cos) rotate<HD>(x[it], p.cos, p.sin, (int)(len + t0) + t, c);
+      if (kv == 0 && p.cos) rotate(x[it], load_angles<HD>(p.cos, p.sin, (int)(len + t0) + t, c));
 #pragma unroll
       for (int e = 0; e < 8; ++e) a = fmaxf(a, fmaxf(finite_abs(x[it].a[e]), finite_abs(x[it].b[e])));
     }
@@ -180,6 +207,7 @@ struct ReadParams {
   LayerView kv;
   int B, hkv, pages, max_pages;
   long long L;
+  unsigned chunks;  // CTAs per (sequence, kv head) of K or V
   const int* table;
   long long ld_table;
   const int* first;
@@ -188,51 +216,67 @@ struct ReadParams {
   void* v_out;
 };
 
+// A CTA reads kReadRows positions of one (sequence, kv head) of K or V, 16 codes per thread at a time.
+constexpr int kReadRows = 64;
+
 template <int HD, int P, int KIND, bool F32>
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int C = HD / 8;  // 8-value pieces per row
-  const long long total = (long long)p.B * p.hkv * p.L * C;
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < 2 * total; i += (long long)gridDim.x * kThreads) {
-    const int kv = i >= total;
-    long long r = kv ? i - total : i;
-    const int c = (int)(r % C);
-    r /= C;  // (b, h, position)
-    const long long l = r % p.L, bh = r / p.L;
-    const int h = (int)(bh % p.hkv), b = (int)(bh / p.hkv);
-    const long long pos = (long long)max(p.first[b], 0) + l;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (l < p.count[b] && pos / P < p.max_pages) {
+  constexpr int C = HD / 16, STEP = kThreads / C;
+  chain();
+  const unsigned u = blockIdx.x / p.chunks, chunk = blockIdx.x - u * p.chunks, kv = u & 1, bh = u >> 1;
+  const int b = (int)(bh / p.hkv), h = (int)(bh - b * p.hkv), c = threadIdx.x % C;
+  const int count = p.count[b];
+  const long long first = max(p.first[b], 0);
+  const uint8_t* codes = (kv ? p.kv.v : p.kv.k) + (long long)h * (P * HD) + 16 * c;
+  const float* scales = (kv ? p.kv.vs : p.kv.ks) + h;
+  uint4 w[kReadRows / STEP];
+  float s[kReadRows / STEP];
+#pragma unroll
+  for (int i = 0; i < kReadRows / STEP; ++i) {
+    const int l = (int)chunk * kReadRows + i * STEP + threadIdx.x / C;
+    const long long pos = first + l;
+    w[i] = make_uint4(0u, 0u, 0u, 0u);
+    s[i] = 0.f;
+    if (l < count && l < p.L && pos / P < p.max_pages) {
       const int page = valid_page(p.table[(long long)b * p.ld_table + pos / P], p.pages);
       if (page >= 0) {
-        const long long blk = (long long)page * p.hkv + h;
-        const float s = (kv ? p.kv.vs : p.kv.ks)[blk];
-        const uint2 w = *reinterpret_cast<const uint2*>((kv ? p.kv.v : p.kv.k) + (blk * P + pos % P) * HD + 8 * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(decode<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu), s);
+        s[i] = scales[(long long)page * p.hkv];
+        w[i] = *reinterpret_cast<const uint4*>(codes + (long long)page * p.hkv * (P * HD) + (int)(pos % P) * HD);
       }
     }
+  }
+#pragma unroll
+  for (int i = 0; i < kReadRows / STEP; ++i) {
+    const int l = (int)chunk * kReadRows + i * STEP + threadIdx.x / C;
+    if (l >= p.L) break;
+    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+    float f[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] = __fmul_rn(decode<KIND>((x[e >> 2] >> (8 * (e & 3))) & 0xffu), s[i]);
+    const long long at = ((long long)bh * p.L + l) * HD + 16 * c;
     if (F32) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(kv ? p.v_out : p.k_out) + r * HD + 8 * c);
-      dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-      dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(kv ? p.v_out : p.k_out) + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
     } else {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(kv ? p.v_out : p.k_out) + r * HD + 8 * c);
-      *dst = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(kv ? p.v_out : p.k_out) + at);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        dst[e] = make_uint4(pack_bf16(f[8 * e], f[8 * e + 1]), pack_bf16(f[8 * e + 2], f[8 * e + 3]),
+                            pack_bf16(f[8 * e + 4], f[8 * e + 5]), pack_bf16(f[8 * e + 6], f[8 * e + 7]));
     }
   }
 }
 
 template <int HD, int P, int KIND>
 int launch_append(const AppendParams& p, unsigned grid, cudaStream_t st) {
-  kv8_append_kernel<HD, P, KIND><<<grid, kThreads, 0, st>>>(p);
-  return launch_status();
+  return launch_chain(kv8_append_kernel<HD, P, KIND>, dim3(grid), kThreads, 0, st, p);
 }
 
 template <int HD, int P, int KIND>
 int launch_read(const ReadParams& p, bool f32, unsigned grid, cudaStream_t st) {
-  if (f32) kv8_read_kernel<HD, P, KIND, true><<<grid, kThreads, 0, st>>>(p);
-  else kv8_read_kernel<HD, P, KIND, false><<<grid, kThreads, 0, st>>>(p);
-  return launch_status();
+  if (f32) return launch_chain(kv8_read_kernel<HD, P, KIND, true>, dim3(grid), kThreads, 0, st, p);
+  return launch_chain(kv8_read_kernel<HD, P, KIND, false>, dim3(grid), kThreads, 0, st, p);
 }
 
 // Calls F<HD, P, KIND>(args...) for the cache's shape (check_cache has passed).
@@ -296,7 +340,9 @@ int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qk
   p.ld_q = ld_q;
   p.kv = layer_view(*cache, layer);
   const long long kv_ctas = 2LL * B * p.touched * p.hkv;
-  const long long q_ctas = (B * T * hq * (hd / 16) + kThreads - 1) / kThreads;
+  const int heads = hd == 128 ? kHeads<128>() : kHeads<64>();
+  if (B * T > 0x3fffffff / ((hq + heads - 1) / heads)) return WAL_ERR_SHAPE;
+  const long long q_ctas = (B * T * ((hq + heads - 1) / heads) + kThreads / 32 - 1) / (kThreads / 32);
   if (kv_ctas + q_ctas > 0x7fffffff) return WAL_ERR_SHAPE;
   p.kv_ctas = (unsigned)kv_ctas;
   const unsigned grid = (unsigned)(kv_ctas + q_ctas);
@@ -326,8 +372,10 @@ int wal_kv8_read(const wal_kv8_cache* cache, int32_t layer, int64_t B, const int
   p.count = count;
   p.k_out = k_out;
   p.v_out = v_out;
-  const long long ctas = (2LL * B * p.hkv * L * (cache->head_dim / 8) + kThreads - 1) / kThreads;
-  const unsigned grid = (unsigned)(ctas < 148 * 16 ? ctas : 148 * 16);
+  p.chunks = (unsigned)((L + kReadRows - 1) / kReadRows);
+  const long long units = 2LL * B * p.hkv;
+  if (units > 0x7fffffff / p.chunks) return WAL_ERR_SHAPE;
+  const unsigned grid = (unsigned)(units * p.chunks);
   WAL_KV8_DISPATCH(cache, launch_read, p, out_dtype == WAL_F32, grid, static_cast<cudaStream_t>(stream));
 }
 

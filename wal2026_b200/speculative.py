@@ -7,12 +7,31 @@ import torch
 from torch import Tensor
 
 from . import _abi
-from .kv8 import _call, _cuda, _i32, _on
+from .kv8 import _call, _cuda, _i32, _is_i32, _on
 
 
 def _row_stride(t: Tensor) -> int:
     """Elements between the rows of one sequence (the stride of a single row says nothing)."""
-    return t.stride(1) if t.shape[1] > 1 else t.shape[2]
+    return t.stride()[1] if t.shape[1] > 1 else t.shape[2]
+
+
+def _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens) -> tuple[int, int, int]:
+    dev = target.device
+    if target.dtype != torch.float32 or target.dim() != 3 or target.stride(2) != 1 or target.shape[1] < 1:
+        raise ValueError("target must be fp32 [B, T + 1, V] with contiguous rows")
+    B, T, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    if draft is not None and (draft.dtype != torch.float32 or tuple(draft.shape) != (B, T, V) or draft.stride(2) != 1):
+        raise ValueError("draft must be fp32 [B, T, V] with contiguous rows")
+    _i32("drafts", drafts, B, T)
+    _i32("accepted", accepted, B)
+    _i32("tokens", tokens, B, T + 1)
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, T + 1) or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be fp32 [B, T + 1] contiguous")
+    if draft_lens is not None:
+        _i32("draft_lens", draft_lens, B)
+    _cuda(dev)
+    _on(dev, draft=draft, drafts=drafts, uniforms=uniforms, accepted=accepted, tokens=tokens, draft_lens=draft_lens)
+    return B, T, V
 
 
 def verify_drafts(target: Tensor, draft: Optional[Tensor], drafts: Tensor, uniforms: Tensor, accepted: Tensor,
@@ -30,24 +49,20 @@ def verify_drafts(target: Tensor, draft: Optional[Tensor], drafts: Tensor, unifo
     in whole numbers of 2^-38, so the outcome is the same in any order of
     summation.  A row whose probabilities are all zero gives token -1.
     """
-    dev = target.device
-    if target.dtype != torch.float32 or target.dim() != 3 or target.stride(2) != 1 or target.shape[1] < 1:
-        raise ValueError("target must be fp32 [B, T + 1, V] with contiguous rows")
-    B, T, V = target.shape[0], target.shape[1] - 1, target.shape[2]
-    if draft is not None and (draft.dtype != torch.float32 or tuple(draft.shape) != (B, T, V) or draft.stride(2) != 1):
-        raise ValueError("draft must be fp32 [B, T, V] with contiguous rows")
-    _i32("drafts", drafts, B, T)
-    _i32("accepted", accepted, B)
-    _i32("tokens", tokens, B, T + 1)
-    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, T + 1) or not uniforms.is_contiguous():
-        raise ValueError("uniforms must be fp32 [B, T + 1] contiguous")
-    if draft_lens is not None:
-        _i32("draft_lens", draft_lens, B)
-    _cuda(dev)
-    _on(dev, draft=draft, drafts=drafts, uniforms=uniforms, accepted=accepted, tokens=tokens, draft_lens=draft_lens)
+    index, s, s1 = target.get_device(), target.shape, target.stride()
+    fit = index >= 0 and len(s) == 3 and s[1] >= 1 and target.dtype is torch.float32 and s1[2] == 1
+    if fit:
+        B, T, V = s[0], s[1] - 1, s[2]
+        fit = ((draft is None or (draft.shape == (B, T, V) and draft.dtype is torch.float32 and draft.stride()[2] == 1
+                                  and draft.get_device() == index))
+               and _is_i32(drafts, (B, T), index) and _is_i32(accepted, (B,), index) and _is_i32(tokens, (B, T + 1), index)
+               and uniforms.shape == (B, T + 1) and uniforms.dtype is torch.float32 and uniforms.is_contiguous()
+               and uniforms.get_device() == index and (draft_lens is None or _is_i32(draft_lens, (B,), index)))
+    if not fit:
+        B, T, V = _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens)
     if T == 0:
         draft = None
-    d0, d1 = (0, V) if draft is None else (draft.stride(0), _row_stride(draft))
-    _call(dev, "wal_verify_drafts", target.data_ptr(), target.stride(0), _row_stride(target), _abi.ptr(draft), d0, d1,
-          drafts.data_ptr() if T else None, T, _abi.ptr(draft_lens), uniforms.data_ptr(), T + 1, B, T, V,
-          accepted.data_ptr(), tokens.data_ptr(), T + 1)
+    d0, d1 = (0, V) if draft is None else (draft.stride()[0], _row_stride(draft))
+    _call(index, "wal_verify_drafts", target.data_ptr(), s1[0], _row_stride(target), None if draft is None else draft.data_ptr(),
+          d0, d1, drafts.data_ptr() if T else None, T, None if draft_lens is None else draft_lens.data_ptr(),
+          uniforms.data_ptr(), T + 1, B, T, V, accepted.data_ptr(), tokens.data_ptr(), T + 1)
