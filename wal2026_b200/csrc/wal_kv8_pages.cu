@@ -70,7 +70,7 @@ __device__ __forceinline__ int cluster_scan(cg::cluster_group& cl, int v, int* s
 }
 
 // Chunks of kChunk entries of the rows of a table, one per warp at a time.
-constexpr int kChunk = 128;
+constexpr int kChunk = 512;
 
 struct AssignParams {
   const int* table;
@@ -115,15 +115,30 @@ __device__ __forceinline__ Row load_row(const AssignParams& p, int b) {
 }
 
 __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_constant__ AssignParams p) {
-  extern __shared__ int begin[];  // [rows + 1] first wanted page of each row, then a bit per row that copies
-  __shared__ int scan[kWarps], box[2][kCluster];
+  extern __shared__ int begin[];  // [rows + 1] first wanted page of each row, [rows] kept pages, [rows] parents, bits of rows that copy
+  __shared__ int scan[kWarps], box[kCluster];
   __shared__ int lost;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gtid = rank * kThreads + tid, gthreads = ncta * kThreads, gwarp = rank * kWarps + warp, gwarps = ncta * kWarps;
-  unsigned* const copies = reinterpret_cast<unsigned*>(begin + p.rows + 1);
+  int* const have = begin + p.rows + 1;
+  int* const parent = have + p.rows;  // minus one less the parent where the row writes into its last page
+  unsigned* const copies = reinterpret_cast<unsigned*>(parent + p.rows);
   chain();
+  // every CTA knows every row; a thread keeps its first row in registers
+  Row first = {};
+  int last_page = -1;  // that it will write
+  for (int b = tid; b < p.rows; b += kThreads) {
+    const Row r = load_row(p, b);
+    have[b] = r.have;
+    begin[b] = r.want;
+    parent[b] = r.writes ? -1 - r.parent : r.parent;
+    if (b == tid) first = r;
+  }
+  if (tid < p.rows) {
+    if (first.writes) last_page = valid_page(__ldg(p.table + (long long)first.parent * p.ld_table + first.have - 1), p.pages);
+  }
   if (tid == 0) lost = 0;
   for (int i = gtid; i < p.pages; i += gthreads) p.ref[i] = 0u;
   for (int i = tid; i < (p.rows + 31) / 32; i += kThreads) copies[i] = 0u;
@@ -132,49 +147,67 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
   const int per_row = (p.width + kChunk - 1) / kChunk;
   for (long long u = gwarp; u < (long long)p.rows * per_row; u += gwarps) {
     const int b = (int)(u / per_row), j0 = (int)(u % per_row) * kChunk + lane;
-    const Row r = load_row(p, b);
+    const int kept = have[b], want = begin[b], last = parent[b] < 0 ? kept - 1 : -1;
+    const int* row = p.table + (long long)(parent[b] < 0 ? -1 - parent[b] : parent[b]) * p.ld_table;
     int e[kChunk / 32];
 #pragma unroll
     for (int i = 0; i < kChunk / 32; ++i) {
       const int j = j0 + 32 * i;
-      e[i] = j < r.have ? valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + j), p.pages) : -1;
+      e[i] = j < kept ? valid_page(__ldg(row + j), p.pages) : -1;
     }
 #pragma unroll
     for (int i = 0; i < kChunk / 32; ++i) {
       const int j = j0 + 32 * i;
-      if (e[i] >= 0) atomicAdd(p.ref + e[i], r.writes && j == r.have - 1 ? 0x10001u : 1u);
-      if (j < p.width) p.out[(long long)b * p.ld_out + j] = e[i];
+      if (e[i] >= 0) atomicAdd(p.ref + e[i], j == last ? 0x10001u : 1u);
+      if (j < p.width && (j < kept || j >= want)) p.out[(long long)b * p.ld_out + j] = e[i];
     }
   }
   cl.sync();
-  // rows that write: sole owner, one of writers only (2), or beside readers (1)
-  for (int b = gtid; b < p.rows; b += gthreads) {
-    const Row r = load_row(p, b);
-    const int e = r.writes ? valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + r.have - 1), p.pages) : -1;
-    int kind = 0;
+  // rows that write: sole owner, beside readers (a copy), or one of writers only (a copy unless it is the lowest)
+  bool among = false;
+  for (int b = tid; b < p.rows; b += kThreads) {
+    Row r = first;
+    int e = last_page;
+    if (b >= kThreads) {
+      r = load_row(p, b);
+      e = r.writes ? valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + r.have - 1), p.pages) : -1;
+    }
     if (e >= 0) {
       const unsigned w = __ldcg(p.ref + e), total = w & 0xffffu, writers = w >> 16;
-      if (total > 1) kind = total == writers ? 2 : 1;
+      if (total > 1) {
+        atomicOr(copies + (b >> 5), 1u << (b & 31));
+        among |= total == writers;
+      }
     }
-    p.src[b] = e;
-    p.dst[b] = kind;
   }
-  cl.sync();
-  for (int b = gtid; b < p.rows; b += gthreads)
-    if (p.dst[b] == 2) atomicMax(p.ref + p.src[b], kFlag | (kRowMask - (unsigned)b));
-  cl.sync();
-  // wanted pages of each row: its copy, then the new ones (every CTA for itself)
+  if (__syncthreads_or(among)) {  // the same in every CTA
+    cl.sync();                    // nobody reads the counts any more
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int b = tid; b < p.rows; b += kThreads) {
+        if (!(copies[b >> 5] >> (b & 31) & 1u)) continue;
+        int e = last_page;
+        if (b >= kThreads) {
+          const Row r = load_row(p, b);
+          e = valid_page(__ldg(p.table + (long long)r.parent * p.ld_table + r.have - 1), p.pages);
+        }
+        const unsigned w = __ldcg(p.ref + e);
+        if (pass == 0) {
+          if ((w & kFlag) || (w & 0xffffu) == w >> 16) atomicMax(p.ref + e, kFlag | (kRowMask - (unsigned)b));
+        } else if ((w & kFlag) && (w & kRowMask) == kRowMask - (unsigned)b) {
+          atomicAnd(copies + (b >> 5), ~(1u << (b & 31)));
+        }
+      }
+      cl.sync();
+    }
+  }
+  // wanted pages of each row: its copy, then the new ones
   int base = 0;
   for (int b0 = 0; b0 < p.rows; b0 += kThreads) {
     const int b = b0 + tid;
     int n = 0, total;
     if (b < p.rows) {
-      const Row r = load_row(p, b);
-      const int kind = __ldcg(p.dst + b);
-      bool cow = kind == 1;
-      if (kind == 2) cow = (kRowMask - (__ldcg(p.ref + __ldcg(p.src + b)) & kRowMask)) != (unsigned)b;
-      n = (cow ? 1 : 0) + r.want - r.have;
-      if (cow) atomicOr(copies + (b >> 5), 1u << (b & 31));
+      const Row r = b0 == 0 ? first : load_row(p, b);
+      n = (int)(copies[b >> 5] >> (b & 31) & 1u) + r.want - r.have;
       const long long over = ((long long)r.keep + r.add + p.P - 1) / p.P - r.want;
       if (r.add && over > 0) atomicAdd(&lost, (int)min(over, 0x3fffffffLL));
     }
@@ -183,20 +216,26 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
     base += total;
   }
   if (tid == 0) begin[p.rows] = base;
-  __syncthreads();
   // free pages in rising order to wanted ones in rising order; final counts.  Each thread has a run of pages.
   const int each = (p.pages + gthreads - 1) / gthreads, i0 = (int)min((long long)gtid * each, (long long)p.pages), i1 = min(i0 + each, p.pages);
-  int mine = 0, found, unused;
-  for (int i = i0; i < i1; ++i) mine += __ldcg(p.ref + i) == 0u;
-  int k = cluster_scan(cl, mine, scan, box[0], &found);  // from here on no CTA reads src or dst
-  if (rank == 0)
-    for (int b = tid; b < p.rows; b += kThreads) {
-      const bool cow = copies[b >> 5] >> (b & 31) & 1u;
-      if (!cow || begin[b] >= found) p.src[b] = -1;
-      if (!cow || begin[b] >= found) p.dst[b] = -1;
-    }
-  for (int i = i0; i < i1; ++i) {
-    const unsigned w = __ldcg(p.ref + i);
+  int mine = 0, found;
+  for (int i = i0; i < i1; i += 8) {
+    unsigned w[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) w[x] = i + x < i1 ? __ldcg(p.ref + i + x) : 1u;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) mine += w[x] == 0u;
+  }
+  int k = cluster_scan(cl, mine, scan, box, &found);
+  for (int i8 = i0; i8 < i1; i8 += 8) {
+    unsigned words[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) words[x] = i8 + x < i1 ? __ldcg(p.ref + i8 + x) : 1u;
+#pragma unroll
+   for (int x = 0; x < 8; ++x) {
+    const int i = i8 + x;
+    const unsigned w = words[x];
+    if (i >= i1) break;
     int count;
     if (w == 0u) {
       count = k < base;
@@ -207,11 +246,10 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
           if (begin[mid] <= k) lo = mid;
           else hi = mid - 1;
         }
-        const Row r = load_row(p, lo);
         const int s = k - begin[lo];
         const bool cow = copies[lo >> 5] >> (lo & 31) & 1u;
         if (cow && s == 0) p.dst[lo] = i;
-        p.out[(long long)lo * p.ld_out + (cow ? r.have - 1 + s : r.have + s)] = i;
+        p.out[(long long)lo * p.ld_out + have[lo] + s - cow] = i;
       }
       ++k;
     } else if (w & kFlag) {
@@ -221,21 +259,22 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
       count = t == writers ? 1 : t - writers;
     }
     p.ref[i] = (unsigned)count;
+   }
   }
-  // what found no page
-  if (found < base)
-    for (int b = gtid; b < p.rows; b += gthreads)
-      if (begin[b + 1] > found) {
-        const Row r = load_row(p, b);
-        const bool cow = copies[b >> 5] >> (b & 31) & 1u;
-        for (int x = max(begin[b], found); x < begin[b + 1]; ++x) {
-          const int s = x - begin[b];
-          p.out[(long long)b * p.ld_out + (cow ? r.have - 1 + s : r.have + s)] = -1;
-        }
-      }
+  // copies' sources, and what found no page
+  for (int b = gtid; b < p.rows; b += gthreads) {
+    const bool cow = copies[b >> 5] >> (b & 31) & 1u;
+    int s = -1;
+    if (cow && begin[b] < found) {
+      s = p.table[(long long)(-1 - parent[b]) * p.ld_table + have[b] - 1];
+    } else {
+      p.dst[b] = -1;
+    }
+    p.src[b] = s;
+    for (int x = max(begin[b], found); x < begin[b + 1]; ++x) p.out[(long long)b * p.ld_out + have[b] + x - begin[b] - cow] = -1;
+  }
   if (rank == 0 && tid == 0) {
-    unused = max(found - base, 0);
-    p.info[0] = unused;
+    p.info[0] = max(found - base, 0);
     p.info[1] = lost + max(base - found, 0);
   }
 }
@@ -282,18 +321,30 @@ __global__ void __launch_bounds__(kThreads) kv_pages_compact_kernel(const __grid
   // each thread has a run of pages
   const int each = (p.pages + gthreads - 1) / gthreads, i0 = (int)min((long long)gtid * each, (long long)p.pages), i1 = min(i0 + each, p.pages);
   int mine = 0, live, movers, holes;
-  for (int i = i0; i < i1; ++i) mine += __ldcg(p.remap + i) >= 0;
+  for (int i = i0; i < i1; i += 8)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) mine += i + x < i1 && __ldcg(p.remap + i + x) >= 0;
   const int used_before = cluster_scan(cl, mine, scan, box[0], &live);
   // holes below `live` and movers from there on follow from the used pages before a page
   int u = used_before, beyond = 0;
-  for (int i = i0; i < i1; ++i) beyond += i >= live && __ldcg(p.remap + i) >= 0;
+  if (i1 > live)
+    for (int i = i0; i < i1; i += 8)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) beyond += i + x >= live && i + x < i1 && __ldcg(p.remap + i + x) >= 0;
   int km = cluster_scan(cl, beyond, scan, box[1], &movers);
-  for (int i = i0; i < i1; ++i) {
-    const bool used = __ldcg(p.remap + i) >= 0;
-    if (used && i >= live) p.src[km++] = i;
-    if (!used && i < live) p.dst[i - u] = i;
-    if (used) p.remap[i] = i;
-    u += used;
+  for (int i8 = i0; i8 < i1; i8 += 8) {
+    bool used[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) used[x] = i8 + x < i1 && __ldcg(p.remap + i8 + x) >= 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int i = i8 + x;
+      if (i >= i1) break;
+      if (used[x] && i >= live) p.src[km++] = i;
+      if (!used[x] && i < live) p.dst[i - u] = i;
+      if (used[x]) p.remap[i] = i;
+      u += used[x];
+    }
   }
   holes = movers;  // as many as there are movers
   cl.sync();
@@ -329,62 +380,51 @@ struct CopyParams {
   int n;
 };
 
-constexpr int kCopyThreads = 256;
-constexpr int kSegBytes = kCopyThreads * 16;  // bytes that one CTA copies of one page and plane
-constexpr int kCopyBatch = 8;                 // pairs whose loads are in flight together
-constexpr int kRun = 4 * kCopyThreads;        // pairs that a CTA looks through at a time
+// An item is 4 KB of one page and plane (layer, K or V) of one pair.  Warps take
+// items a grid apart, so that those of a moved page go to as many warps and a
+// list with few pairs in it (most of a compaction's is empty) still spreads;
+// 32 items are looked up together, one per lane, and no warp waits for another.
+constexpr int kCopyThreads = 128;
+constexpr int kCopyCtasPerSm = 8;
+constexpr int kItemVecs = 8;  // 16-byte pieces per lane
+constexpr int kItemBytes = kItemVecs * 32 * 16;
 
-// grid.x: segments of a plane's page x planes (layer, K or V); grid.y: runs of
-// pairs; grid.z: shares of a run's pairs.
-__global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const __grid_constant__ CopyParams p) {
-  __shared__ int2 list[kRun];
-  __shared__ int counts[kRun / 32];
-  const int seg = blockIdx.x % p.segs, plane = blockIdx.x / p.segs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint8_t* const base = p.codes + plane * p.half_bytes + (long long)seg * kSegBytes + tid * 16;
-  float* const sc = p.scales + plane * p.half_scales;
-  const bool mine = (long long)seg * kSegBytes + tid * 16 < p.page_bytes;
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) kv_pages_copy_kernel(const __grid_constant__ CopyParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long warps = (long long)gridDim.x * (kCopyThreads / 32), items = (long long)p.n * p.planes * p.segs;
   chain();
-  for (int i0 = blockIdx.y * kRun; i0 < p.n; i0 += gridDim.y * kRun) {
-    int s[4], d[4];
-    unsigned todo[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = i0 + x * kCopyThreads + tid;
-      s[x] = i < p.n ? valid_page(p.src[i], p.pages) : -1;
-      d[x] = i < p.n ? valid_page(p.dst[i], p.pages) : -1;
+  for (long long it = (long long)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); it < items; it += 32 * warps) {
+    const long long item = it + lane * warps;
+    int s = -1, d = -1, plane = 0, seg = 0;
+    if (item < items) {
+      const long long i = item / (p.planes * p.segs);
+      const int rest = (int)(item - i * (p.planes * p.segs));
+      plane = rest / p.segs;
+      seg = rest - plane * p.segs;
+      s = valid_page(__ldg(p.src + i), p.pages);
+      d = valid_page(__ldg(p.dst + i), p.pages);
     }
+    unsigned todo = __ballot_sync(0xffffffffu, s >= 0 && d >= 0);
+    while (todo) {
+      const int l = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const long long sp = __shfl_sync(0xffffffffu, s, l), dp = __shfl_sync(0xffffffffu, d, l);
+      const int pl = __shfl_sync(0xffffffffu, plane, l), sg = __shfl_sync(0xffffffffu, seg, l);
+      const long long off = (long long)sg * kItemBytes + lane * 16;
+      uint8_t* const base = p.codes + pl * p.half_bytes + off;
+      const int left = (int)min(p.page_bytes - off, (long long)kItemBytes);  // bytes from this lane's first piece on
+      uint4 v[kItemVecs];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      todo[x] = __ballot_sync(0xffffffffu, s[x] >= 0 && d[x] >= 0);
-      if (lane == 0) counts[x * (kCopyThreads / 32) + warp] = __popc(todo[x]);
-    }
-    __syncthreads();
-    int total = 0;
+      for (int i = 0; i < kItemVecs; ++i)
+        if (i * 512 < left) v[i] = __ldcs(reinterpret_cast<const uint4*>(base + sp * p.page_bytes + i * 512));
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int w = 0; w < kCopyThreads / 32; ++w) {
-        if (w == warp && (todo[x] >> lane & 1u)) list[total + __popc(todo[x] & ((1u << lane) - 1u))] = make_int2(s[x], d[x]);
-        total += counts[x * (kCopyThreads / 32) + w];
+      for (int i = 0; i < kItemVecs; ++i)
+        if (i * 512 < left) __stcs(reinterpret_cast<uint4*>(base + dp * p.page_bytes + i * 512), v[i]);
+      if (sg == 0) {
+        float* const sc = p.scales + pl * p.half_scales;
+        for (int h = lane; h < p.hkv; h += 32) sc[dp * p.hkv + h] = sc[sp * p.hkv + h];
       }
-    __syncthreads();
-    for (int k = blockIdx.z; k < total; k += kCopyBatch * gridDim.z) {
-      uint4 v[kCopyBatch];
-#pragma unroll
-      for (int i = 0; i < kCopyBatch; ++i)
-        if (mine && k + i * (int)gridDim.z < total)
-          v[i] = __ldcs(reinterpret_cast<const uint4*>(base + list[k + i * gridDim.z].x * p.page_bytes));
-#pragma unroll
-      for (int i = 0; i < kCopyBatch; ++i)
-        if (mine && k + i * (int)gridDim.z < total)
-          __stcs(reinterpret_cast<uint4*>(base + list[k + i * gridDim.z].y * p.page_bytes), v[i]);
-      if (seg == 0)
-        for (int i = 0; i < kCopyBatch && k + i * (int)gridDim.z < total; ++i) {
-          const long long sp = list[k + i * gridDim.z].x, dp = list[k + i * gridDim.z].y;
-          for (int h = tid; h < p.hkv; h += kCopyThreads) sc[dp * p.hkv + h] = sc[sp * p.hkv + h];
-        }
     }
-    __syncthreads();
   }
 }
 
@@ -407,7 +447,7 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   AssignParams p = {table, ld_table, (int)rows_in, parent, keep, add, (int)rows, (int)width, (int)num_pages, page_size,
                     table_out, ld_out, reinterpret_cast<unsigned*>(ref_out), copy_src, copy_dst, info};
-  const int smem = ((int)rows + 1 + ((int)rows + 31) / 32) * (int)sizeof(int);
+  const int smem = (3 * (int)rows + 1 + ((int)rows + 31) / 32) * (int)sizeof(int);
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kv_pages_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return WAL_ERR_CUDA;
   const int cluster = table_cluster(rows * width, num_pages);
@@ -441,19 +481,14 @@ int wal_kv_pages_copy(const wal_kv8_cache* cache, const int32_t* src, const int3
   p.hkv = cache->kv_heads;
   p.pages = (int)cache->num_pages;
   p.planes = 2 * cache->layers;
-  p.segs = (int)((p.page_bytes + kSegBytes - 1) / kSegBytes);
+  if (2LL * cache->layers * ((p.page_bytes + kItemBytes - 1) / kItemBytes) > 0x7fffffff) return WAL_ERR_SHAPE;
+  p.segs = (int)((p.page_bytes + kItemBytes - 1) / kItemBytes);
   p.src = src;
   p.dst = dst;
   p.n = (int)n;
-  const long long gx = (long long)p.planes * p.segs;
-  if (gx > 0x7fffffff) return WAL_ERR_SHAPE;
-  // about sixteen CTAs per SM: up to eight runs side by side, then shares of a run
-  const long long want = 16LL * sm_count(), runs = (n + kRun - 1) / kRun;
-  const long long gy = runs < 8 ? runs : 8;
-  long long gz = want / (gx * gy);
-  gz = gz < 1 ? 1 : gz > 64 ? 64 : gz;
-  if (gz > n) gz = n;
-  const dim3 grid((unsigned)gx, (unsigned)gy, (unsigned)gz);
+  const long long items = (long long)n * p.planes * p.segs, ctas = (items + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
+  const long long most = (long long)kCopyCtasPerSm * sm_count();
+  const dim3 grid((unsigned)(ctas < most ? ctas : most));
   return launch_chain(kv_pages_copy_kernel, grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream), p);
 }
 

@@ -42,11 +42,19 @@ __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
   f[4] = bf16_lo(v.z); f[5] = bf16_hi(v.z); f[6] = bf16_lo(v.w); f[7] = bf16_hi(v.w);
 }
 
+struct Raw {
+  uint4 a, b;
+};
+
 template <int HD>
-__device__ __forceinline__ Pair load_pair(const uint16_t* src, int c) {
+__device__ __forceinline__ Raw load_raw(const uint16_t* src, int c) {
+  return {__ldg(reinterpret_cast<const uint4*>(src + 8 * c)), __ldg(reinterpret_cast<const uint4*>(src + HD / 2 + 8 * c))};
+}
+
+__device__ __forceinline__ Pair widen(const Raw& r) {
   Pair p;
-  unpack(__ldg(reinterpret_cast<const uint4*>(src + 8 * c)), p.a);
-  unpack(__ldg(reinterpret_cast<const uint4*>(src + HD / 2 + 8 * c)), p.b);
+  unpack(r.a, p.a);
+  unpack(r.b, p.b);
   return p;
 }
 
@@ -112,16 +120,16 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     const unsigned w = (blockIdx.x - p.kv_ctas) * (kThreads / 32) + (tid >> 5);
     const unsigned m = w / groups, h0 = (w - m * groups) * kHeads<HD>() + lane / C;
     if (m >= (unsigned)(p.B * p.T)) return;
+    const uint16_t* src = p.qkv + (long long)m * p.ld + h0 * HD;
+    uint16_t* dst = p.q_out + (long long)m * p.ld_q + h0 * HD + 8 * c;
+    Raw raw[kIter];  // asked for before the lengths are known
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (h0 + i * H < (unsigned)p.hq) raw[i] = load_raw<HD>(src + i * H * HD, c);
     const int b = (int)m / p.T, t = (int)m - b * p.T;
     const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
     const long long pos = (long long)max(p.lens[b], 0) + t;
     const bool real = t < nn && (!p.cos || pos < p.max_pos);
-    const uint16_t* src = p.qkv + (long long)m * p.ld + h0 * HD;
-    uint16_t* dst = p.q_out + (long long)m * p.ld_q + h0 * HD + 8 * c;
-    Pair x[kIter];
-#pragma unroll
-    for (int i = 0; i < kIter; ++i)
-      if (real && h0 + i * H < (unsigned)p.hq) x[i] = load_pair<HD>(src + i * H * HD, c);
     Angles g;
     if (real && p.cos) g = load_angles<HD>(p.cos, p.sin, (int)pos, c);
 #pragma unroll
@@ -129,9 +137,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
       if (h0 + i * H >= (unsigned)p.hq) break;
       uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
       if (real) {
-        if (p.cos) rotate(x[i], g);
-        lo = make_uint4(pack_bf16(x[i].a[0], x[i].a[1]), pack_bf16(x[i].a[2], x[i].a[3]), pack_bf16(x[i].a[4], x[i].a[5]), pack_bf16(x[i].a[6], x[i].a[7]));
-        hi = make_uint4(pack_bf16(x[i].b[0], x[i].b[1]), pack_bf16(x[i].b[2], x[i].b[3]), pack_bf16(x[i].b[4], x[i].b[5]), pack_bf16(x[i].b[6], x[i].b[7]));
+        Pair x = widen(raw[i]);
+        if (p.cos) rotate(x, g);
+        lo = make_uint4(pack_bf16(x.a[0], x.a[1]), pack_bf16(x.a[2], x.a[3]), pack_bf16(x.a[4], x.a[5]), pack_bf16(x.a[6], x.a[7]));
+        hi = make_uint4(pack_bf16(x.b[0], x.b[1]), pack_bf16(x.b[2], x.b[3]), pack_bf16(x.b[4], x.b[5]), pack_bf16(x.b[6], x.b[7]));
       }
       *reinterpret_cast<uint4*>(dst + i * H * HD) = lo;
       *reinterpret_cast<uint4*>(dst + i * H * HD + HD / 2) = hi;
@@ -157,13 +166,19 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
   if (page < 0) return;
   const int slot0 = (int)(len + t0 - start), cnt = (int)(t1 - t0);  // slots [slot0, slot0 + cnt)
   const uint16_t* src = p.qkv + ((long long)b * p.T + t0) * p.ld + (long long)(p.hq + kv * p.hkv + h) * HD;
+  Raw raw[IT];
   Pair x[IT];
   float a = 0.f;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int i = it * kThreads + tid, t = i / C, c = i % C;
+    if (t < cnt) raw[it] = load_raw<HD>(src + (long long)t * p.ld, c);
+  }
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * kThreads + tid, t = i / C, c = i % C;
     if (t < cnt) {
-      x[it] = load_pair<HD>(src + (long long)t * p.ld, c);
+      x[it] = widen(raw[it]);
       if (kv == 0 && p.cos) rotate(x[it], load_angles<HD>(p.cos, p.sin, (int)(len + t0) + t, c));
 #pragma unroll
       for (int e = 0; e < 8; ++e) a = fmaxf(a, fmaxf(finite_abs(x[it].a[e]), finite_abs(x[it].b[e])));

@@ -25,7 +25,6 @@ using namespace wal_kv8;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr unsigned long long kOne = 1ull << 38;
 
 struct VerifyParams {
   const float* p;  // [B][T + 1][V]
@@ -43,10 +42,29 @@ struct VerifyParams {
   long long ld_tokens;
 };
 
-__device__ __forceinline__ unsigned long long units(float x) {
-  x = fminf(fmaxf(x, 0.f), 1.f);  // a NaN becomes 0
-  return (unsigned long long)__float2ll_rn(x * (float)kOne);
+// round(2^38 x) of x clamped to [0, 1] (NaN as 0), as hi * 2^23 + lo: adding 2^23
+// to 2^15 x rounds it to a whole number, and what is left is exact and takes 23
+// bits more in the same way.  The bit patterns of the two sums count from
+// kHiBits and kLoBits.  (A conversion to 64-bit integers does the same at a
+// fraction of the rate.)
+struct Fixed {
+  uint32_t hi, lo;
+};
+constexpr uint32_t kHiBits = 0x4b000000u, kLoBits = 0x4b400000u;  // 2^23, 1.5 * 2^23
+
+__device__ __forceinline__ Fixed fixed(float x) {
+  x = __saturatef(x);
+  const float t = __fmaf_rn(x, 32768.f, 8388608.f);
+  const float rest = __fmaf_rn(x, 32768.f, -__fadd_rn(t, -8388608.f));
+  return {__float_as_uint(t), __float_as_uint(__fmaf_rn(rest, 8388608.f, 12582912.f))};
 }
+
+__device__ __forceinline__ long long difference(const Fixed& a, uint32_t hi, uint32_t lo) {
+  return (long long)(int)(a.hi - hi) * 8388608ll + (int)(a.lo - lo);
+}
+
+__device__ __forceinline__ unsigned long long units(float x) { return (unsigned long long)difference(fixed(x), kHiBits, kLoBits); }
+
 __device__ __forceinline__ unsigned long long uniform24(float u) {
   u = fminf(fmaxf(u, 0.f), 0.99999994f);
   return (unsigned long long)(u * 16777216.f);
@@ -58,14 +76,25 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
   return x;
 }
 
-// Weight of token v: the positive part of p - q, of p less the refused draft `out`, or p.
-__device__ __forceinline__ unsigned long long weight(float p, float q, bool has_q, bool refused) {
-  const unsigned long long pv = units(p), qv = has_q ? units(q) : refused ? kOne : 0ull;
-  return pv > qv ? pv - qv : 0ull;
+// Weight of a token: the positive part of p - q (q = 0 where there is none), nothing for the refused draft.
+__device__ __forceinline__ unsigned long long weight(float p, float q, bool refused) {
+  const Fixed f = fixed(q);
+  const long long w = difference(fixed(p), f.hi, f.lo);
+  return w > 0 && !refused ? (unsigned long long)w : 0ull;
 }
 
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
-  constexpr int U = 8;  // loads in flight per lane and row
+// Entries v .. v + 3 of a row, zeros from `end` on.  VEC: the rows are 16-byte aligned, v and end multiples of 4.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* row, int v, int end) {
+  if (VEC) return v < end ? __ldg(reinterpret_cast<const float4*>(row + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(v < end ? __ldg(row + v) : 0.f, v + 1 < end ? __ldg(row + v + 1) : 0.f,
+                     v + 2 < end ? __ldg(row + v + 2) : 0.f, v + 3 < end ? __ldg(row + v + 3) : 0.f);
+}
+
+// CTAS: per SM
+template <bool VEC, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) verify_kernel(const __grid_constant__ VerifyParams p) {
+  constexpr int U = 4;  // groups of four entries in flight per lane and row
   __shared__ int s_a;
   __shared__ unsigned long long warps[kWarps];
   __shared__ unsigned long long ctas[2][kMaxCluster];
@@ -78,14 +107,14 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   const unsigned long long place = uniform24(p.u[b * p.ld_u + p.T]);
   if (tid == 0) s_a = len;
   __syncthreads();
-  for (int t = tid; t < len; t += kThreads) {
+  for (int t = tid; t < p.T; t += kThreads) {
     const int xt = x[t];
     bool ok = (unsigned)xt < (unsigned)p.V;
-    if (ok) {
+    if (ok && t < len) {
       const float pv = p.p[b * p.p_seq + t * p.p_row + xt], qv = p.q ? p.q[b * p.q_seq + t * p.q_row + xt] : 1.f;
       ok = uniform24(p.u[b * p.ld_u + t]) * units(qv) < units(pv) << 24;
     }
-    if (!ok) atomicMin(&s_a, t);
+    if (!ok && t < len) atomicMin(&s_a, t);
   }
   __syncthreads();
   const int a = s_a;
@@ -96,26 +125,29 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     for (int t = tid; t <= p.T; t += kThreads)
       if (t != a) p.tokens[b * p.ld_tokens + t] = t < a ? x[t] : -1;
   if (rank == 0 && tid == 0) p.accepted[b] = a;
-  const int per = (p.V + ncta * kWarps - 1) / (ncta * kWarps), w = rank * kWarps + warp;
-  const int v0 = min(w * per, p.V), v1 = min(v0 + per, p.V);
+  const int per = ((p.V + ncta * kWarps - 1) / (ncta * kWarps) + 3) & ~3, w = rank * kWarps + warp;
+  const int v0 = (int)min((long long)w * per, (long long)p.V), v1 = min(v0 + per, p.V);
   for (int pass = 0; pass < 2; ++pass) {  // the second one draws from p itself where the residual is empty
     unsigned long long sum = 0;
-    for (int v = v0 + lane; v < v1; v += 32 * U) {
-      float pv[U], qv[U];
+    for (int v = v0 + 4 * lane; v < v1; v += 128 * U) {
+      float4 pv[U], qv[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const bool in = v + 32 * i < v1;
-        pv[i] = in ? __ldg(pr + v + 32 * i) : 0.f;
-        qv[i] = in && qr ? __ldg(qr + v + 32 * i) : 0.f;
+        pv[i] = load4<VEC>(pr, v + 128 * i, v1);
+        qv[i] = qr ? load4<VEC>(qr, v + 128 * i, v1) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int i = 0; i < U; ++i) sum += weight(pv[i], qv[i], qr, v + 32 * i == out);
+      for (int i = 0; i < U; ++i) {
+        const int o = out - (v + 128 * i);
+        sum += weight(pv[i].x, qv[i].x, o == 0) + weight(pv[i].y, qv[i].y, o == 1) + weight(pv[i].z, qv[i].z, o == 2) +
+               weight(pv[i].w, qv[i].w, o == 3);
+      }
     }
     sum = warp_sum(sum);
     if (lane == 0) warps[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-      const unsigned long long mine = warp_sum(warps[lane]);
+      const unsigned long long mine = warp_sum(lane < kWarps ? warps[lane] : 0ull);
       if (lane < ncta) cl.map_shared_rank(&ctas[pass][0], lane)[rank] = mine;
     }
     cl.sync();
@@ -133,18 +165,24 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     }
     const unsigned long long r = (((total >> 32) * place) << 8) + (((total & 0xffffffffull) * place) >> 24);
     for (int i = 0; i < warp; ++i) before += warps[i];
-    if (before <= r && r < before + sum) {
-      for (int v = v0; v < v1; v += 32) {
-        unsigned long long inc = 0;
-        if (v + lane < v1) inc = weight(__ldg(pr + v + lane), qr ? __ldg(qr + v + lane) : 0.f, qr, v + lane == out);
+    if (before <= r && r < before + sum) {  // this warp's share holds the place: its weights once more, in order
+      for (int v = v0; v < v1; v += 128) {
+        const int at = v + 4 * lane, o = out - at;
+        const float4 pv = load4<VEC>(pr, at, v1), qv = qr ? load4<VEC>(qr, at, v1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const unsigned long long w0 = weight(pv.x, qv.x, o == 0), w1 = w0 + weight(pv.y, qv.y, o == 1),
+                                 w2 = w1 + weight(pv.z, qv.z, o == 2), w3 = w2 + weight(pv.w, qv.w, o == 3);
+        unsigned long long inc = w3;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += y;
+        for (int x = 1; x < 32; x <<= 1) {
+          const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, x);
+          if (lane >= x) inc += y;
         }
         const unsigned over = __ballot_sync(0xffffffffu, before + inc > r);
         if (over) {
-          if (lane == 0) p.tokens[b * p.ld_tokens + a] = v + __ffs(over) - 1;
+          if (lane == __ffs(over) - 1) {
+            const unsigned long long c = before + inc - w3;
+            p.tokens[b * p.ld_tokens + a] = at + (c + w0 > r ? 0 : c + w1 > r ? 1 : c + w2 > r ? 2 : 3);
+          }
           break;
         }
         before += __shfl_sync(0xffffffffu, inc, 31);
@@ -153,11 +191,6 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     break;
   }
 }
-
-// CTAs of a cluster: many for few sequences, which leave SMs idle; a batch that
-// fills the GPU pays for each CTA's start and barriers.  V = 128256 on B200: 64
-// sequences 40.8 us with 8, 33.7 with 4, 40.5 with 2.
-int cluster_of(int64_t B) { return B * kMaxCluster <= 2 * sm_count() ? kMaxCluster : 4; }
 
 }  // namespace
 
@@ -172,6 +205,14 @@ extern "C" int wal_verify_drafts(const float* target, int64_t target_seq, int64_
   if (ld_drafts < T || ld_uniforms < T + 1 || ld_tokens < T + 1) return WAL_ERR_SHAPE;
   VerifyParams p = {target, target_seq, target_row, draft, draft_seq, draft_row, drafts, ld_drafts, draft_lens, uniforms,
                     ld_uniforms, (int)T, (int)V, accepted, tokens, ld_tokens};
-  const int cluster = cluster_of(B);
-  return launch_chain(verify_kernel, dim3((unsigned)(B * cluster)), kThreads, 0, static_cast<cudaStream_t>(stream), p, cluster);
+  const bool vec = V % 4 == 0 && target_seq % 4 == 0 && target_row % 4 == 0 && ((uintptr_t)target & 15) == 0 &&
+                   (!draft || (draft_seq % 4 == 0 && draft_row % 4 == 0 && ((uintptr_t)draft & 15) == 0));
+  // Few sequences leave SMs idle: eight CTAs each, one per SM.  A batch pays for
+  // each CTA's start and barriers: four each, two per SM.  V = 128256 on B200:
+  // one sequence 7.1 us with eight CTAs one per SM, 7.8 two per SM; 64 sequences
+  // 26.1 us with four CTAs one per SM, 22.9 two per SM, 24.8 with eight of half the threads.
+  const bool few = B * kMaxCluster <= sm_count();
+  const int cluster = few ? kMaxCluster : 4;
+  auto kern = few ? (vec ? verify_kernel<true, 1> : verify_kernel<false, 1>) : (vec ? verify_kernel<true, 2> : verify_kernel<false, 2>);
+  return launch_chain(kern, dim3((unsigned)(B * cluster)), kThreads, 0, static_cast<cudaStream_t>(stream), p, cluster);
 }
