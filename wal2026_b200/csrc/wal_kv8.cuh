@@ -57,11 +57,23 @@ __device__ __forceinline__ float qmax() {
   return KIND == WAL_KV_INT8 ? 127.f : 448.f;
 }
 
+// The four codes of a word as fp32.
 template <int KIND>
-__device__ __forceinline__ float decode(uint32_t code) {
-  if (KIND == WAL_KV_INT8) return (float)(int8_t)(uint8_t)code;
-  __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3);
-  return __half2float(__half(h));
+__device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
+  if (KIND == WAL_KV_INT8) {
+    // byte u = code + 128 in the fraction of 2^23: a logic instruction and an exact subtraction (a conversion runs at a quarter of the rate)
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + i)) - 8388736.f;
+  } else {
+    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
+    f[0] = a.x;
+    f[1] = a.y;
+    f[2] = b.x;
+    f[3] = b.y;
+  }
 }
 
 // round(clamp(x)) as a code; x is already divided by the scale.  NaN -> 0.

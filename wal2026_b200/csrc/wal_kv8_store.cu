@@ -30,6 +30,7 @@ struct AppendParams {
   long long ld_q;
   LayerView kv;
   unsigned kv_ctas;  // CTAs of the K/V part, before those of q
+  unsigned q_items;  // (token, group of heads) pairs
 };
 
 // 16 values of one token and head: dims [8c, 8c + 8) and their rotation partners hd/2 later.
@@ -100,7 +101,8 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;
 }
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;       // append
+constexpr int kReadThreads = 128;
 
 // Query heads that a warp rotates.
 template <int HD>
@@ -109,41 +111,42 @@ __host__ __device__ constexpr int kHeads() {
 }
 
 template <int HD, int P, int KIND>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 3) kv8_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int C = HD / 16;                              // 16-value pieces per token and head
   constexpr int IT = (P * C + kThreads - 1) / kThreads;   // pieces per thread of a whole page
   const int tid = threadIdx.x;
   chain();
   if (blockIdx.x >= p.kv_ctas) {  // q rows: a warp rotates up to kHeads heads of one token by one load of its angles
     constexpr int H = 32 / C, kIter = kHeads<HD>() / H;
-    const int lane = tid & 31, c = lane % C, groups = (p.hq + kHeads<HD>() - 1) / kHeads<HD>();
-    const unsigned w = (blockIdx.x - p.kv_ctas) * (kThreads / 32) + (tid >> 5);
-    const unsigned m = w / groups, h0 = (w - m * groups) * kHeads<HD>() + lane / C;
-    if (m >= (unsigned)(p.B * p.T)) return;
-    const uint16_t* src = p.qkv + (long long)m * p.ld + h0 * HD;
-    uint16_t* dst = p.q_out + (long long)m * p.ld_q + h0 * HD + 8 * c;
-    Raw raw[kIter];  // asked for before the lengths are known
+    const int lane = tid & 31, c = lane % C;
+    const unsigned groups = (unsigned)(p.hq + kHeads<HD>() - 1) / kHeads<HD>(), warps = (gridDim.x - p.kv_ctas) * (kThreads / 32);
+    for (unsigned w = (blockIdx.x - p.kv_ctas) * (kThreads / 32) + (tid >> 5); w < p.q_items; w += warps) {
+      const unsigned m = w / groups, h0 = (w - m * groups) * kHeads<HD>() + lane / C;
+      const int b = (int)m / p.T, t = (int)m - b * p.T;
+      const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
+      const long long pos = (long long)max(p.lens[b], 0) + t;
+      const bool real = t < nn && (!p.cos || pos < p.max_pos);
+      const uint16_t* src = p.qkv + (long long)m * p.ld + h0 * HD;
+      uint16_t* dst = p.q_out + (long long)m * p.ld_q + h0 * HD + 8 * c;
+      Raw raw[kIter];
 #pragma unroll
-    for (int i = 0; i < kIter; ++i)
-      if (h0 + i * H < (unsigned)p.hq) raw[i] = load_raw<HD>(src + i * H * HD, c);
-    const int b = (int)m / p.T, t = (int)m - b * p.T;
-    const int nn = p.new_lens ? min(p.new_lens[b], p.T) : p.T;
-    const long long pos = (long long)max(p.lens[b], 0) + t;
-    const bool real = t < nn && (!p.cos || pos < p.max_pos);
-    Angles g;
-    if (real && p.cos) g = load_angles<HD>(p.cos, p.sin, (int)pos, c);
+      for (int i = 0; i < kIter; ++i)
+        if (real && h0 + i * H < (unsigned)p.hq) raw[i] = load_raw<HD>(src + i * H * HD, c);
+      Angles g;
+      if (real && p.cos) g = load_angles<HD>(p.cos, p.sin, (int)pos, c);
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      if (h0 + i * H >= (unsigned)p.hq) break;
-      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-      if (real) {
-        Pair x = widen(raw[i]);
-        if (p.cos) rotate(x, g);
-        lo = make_uint4(pack_bf16(x.a[0], x.a[1]), pack_bf16(x.a[2], x.a[3]), pack_bf16(x.a[4], x.a[5]), pack_bf16(x.a[6], x.a[7]));
-        hi = make_uint4(pack_bf16(x.b[0], x.b[1]), pack_bf16(x.b[2], x.b[3]), pack_bf16(x.b[4], x.b[5]), pack_bf16(x.b[6], x.b[7]));
+      for (int i = 0; i < kIter; ++i) {
+        if (h0 + i * H >= (unsigned)p.hq) break;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (real) {
+          Pair x = widen(raw[i]);
+          if (p.cos) rotate(x, g);
+          lo = make_uint4(pack_bf16(x.a[0], x.a[1]), pack_bf16(x.a[2], x.a[3]), pack_bf16(x.a[4], x.a[5]), pack_bf16(x.a[6], x.a[7]));
+          hi = make_uint4(pack_bf16(x.b[0], x.b[1]), pack_bf16(x.b[2], x.b[3]), pack_bf16(x.b[4], x.b[5]), pack_bf16(x.b[6], x.b[7]));
+        }
+        *reinterpret_cast<uint4*>(dst + i * H * HD) = lo;
+        *reinterpret_cast<uint4*>(dst + i * H * HD + HD / 2) = hi;
       }
-      *reinterpret_cast<uint4*>(dst + i * H * HD) = lo;
-      *reinterpret_cast<uint4*>(dst + i * H * HD + HD / 2) = hi;
     }
     return;
   }
@@ -200,9 +203,11 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     for (int i = tid; i < slot0 * (HD / 4); i += kThreads) {
       uint32_t* w = reinterpret_cast<uint32_t*>(blk) + i;
       const uint32_t v = *w;
+      float f[4];
+      decode4<KIND>(v, f);
       uint32_t n = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) n |= encode<KIND>(__fmul_rn(decode<KIND>((v >> (8 * e)) & 0xffu), r)) << (8 * e);
+      for (int e = 0; e < 4; ++e) n |= encode<KIND>(__fmul_rn(f[e], r)) << (8 * e);
       *w = n;
     }
   }
@@ -235,8 +240,8 @@ struct ReadParams {
 constexpr int kReadRows = 64;
 
 template <int HD, int P, int KIND, bool F32>
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int C = HD / 16, STEP = kThreads / C;
+__global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const __grid_constant__ ReadParams p) {
+  constexpr int C = HD / 16, STEP = kReadThreads / C;
   chain();
   const unsigned u = blockIdx.x / p.chunks, chunk = blockIdx.x - u * p.chunks, kv = u & 1, bh = u >> 1;
   const int b = (int)(bh / p.hkv), h = (int)(bh - b * p.hkv), c = threadIdx.x % C;
@@ -267,7 +272,12 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constan
     const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
     float f[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = __fmul_rn(decode<KIND>((x[e >> 2] >> (8 * (e & 3))) & 0xffu), s[i]);
+    for (int e = 0; e < 4; ++e) {
+      float g[4];
+      decode4<KIND>(x[e], g);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) f[4 * e + y] = __fmul_rn(g[y], s[i]);
+    }
     const long long at = ((long long)bh * p.L + l) * HD + 16 * c;
     if (F32) {
       float4* dst = reinterpret_cast<float4*>(static_cast<float*>(kv ? p.v_out : p.k_out) + at);
@@ -290,8 +300,8 @@ int launch_append(const AppendParams& p, unsigned grid, cudaStream_t st) {
 
 template <int HD, int P, int KIND>
 int launch_read(const ReadParams& p, bool f32, unsigned grid, cudaStream_t st) {
-  if (f32) return launch_chain(kv8_read_kernel<HD, P, KIND, true>, dim3(grid), kThreads, 0, st, p);
-  return launch_chain(kv8_read_kernel<HD, P, KIND, false>, dim3(grid), kThreads, 0, st, p);
+  if (f32) return launch_chain(kv8_read_kernel<HD, P, KIND, true>, dim3(grid), kReadThreads, 0, st, p);
+  return launch_chain(kv8_read_kernel<HD, P, KIND, false>, dim3(grid), kReadThreads, 0, st, p);
 }
 
 // Calls F<HD, P, KIND>(args...) for the cache's shape (check_cache has passed).
@@ -357,7 +367,8 @@ int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qk
   const long long kv_ctas = 2LL * B * p.touched * p.hkv;
   const int heads = hd == 128 ? kHeads<128>() : kHeads<64>();
   if (B * T > 0x3fffffff / ((hq + heads - 1) / heads)) return WAL_ERR_SHAPE;
-  const long long q_ctas = (B * T * ((hq + heads - 1) / heads) + kThreads / 32 - 1) / (kThreads / 32);
+  p.q_items = (unsigned)(B * T * ((hq + heads - 1) / heads));
+  const long long q_most = (p.q_items + kThreads / 32 - 1) / (kThreads / 32), q_ctas = q_most < 16LL * sm_count() ? q_most : 16LL * sm_count();
   if (kv_ctas + q_ctas > 0x7fffffff) return WAL_ERR_SHAPE;
   p.kv_ctas = (unsigned)kv_ctas;
   const unsigned grid = (unsigned)(kv_ctas + q_ctas);

@@ -76,6 +76,14 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
   return x;
 }
 
+// hi * 2^23 + lo += P - min(P, Q); parts of 16 weights fit.
+__device__ __forceinline__ void add_weight(float p, float q, uint32_t& hi, uint32_t& lo) {
+  p = __saturatef(p);
+  const Fixed f = fixed(p), g = fixed(fminf(p, __saturatef(q)));
+  hi += f.hi - g.hi;
+  lo += f.lo - g.lo;
+}
+
 // Weight of a token: the positive part of p - q (q = 0 where there is none), nothing for the refused draft.
 __device__ __forceinline__ unsigned long long weight(float p, float q, bool refused) {
   const Fixed f = fixed(q);
@@ -136,12 +144,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) verify_kernel(const __grid_con
         pv[i] = load4<VEC>(pr, v + 128 * i, v1);
         qv[i] = qr ? load4<VEC>(qr, v + 128 * i, v1) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      // the sum of P - min(P, Q), part by part: the smaller of the two in fp32 has the smaller whole number
+      uint32_t hi = 0, lo = 0;
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int o = out - (v + 128 * i);
-        sum += weight(pv[i].x, qv[i].x, o == 0) + weight(pv[i].y, qv[i].y, o == 1) + weight(pv[i].z, qv[i].z, o == 2) +
-               weight(pv[i].w, qv[i].w, o == 3);
+        add_weight(pv[i].x, o == 0 ? pv[i].x : qv[i].x, hi, lo);
+        add_weight(pv[i].y, o == 1 ? pv[i].y : qv[i].y, hi, lo);
+        add_weight(pv[i].z, o == 2 ? pv[i].z : qv[i].z, hi, lo);
+        add_weight(pv[i].w, o == 3 ? pv[i].w : qv[i].w, hi, lo);
       }
+      sum += (unsigned long long)((long long)(int)hi * 8388608ll + (int)lo);
     }
     sum = warp_sum(sum);
     if (lane == 0) warps[warp] = sum;
