@@ -48,6 +48,7 @@ constexpr int kTile = 32;          // positions of a tile
 constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced call
 constexpr int kMinTiles = 4;       // least position tiles of a run: one per warp
 constexpr int kUnitCost = 8;      // what starting and ending a unit costs, in tiles
+constexpr unsigned kWholeCost = 28;  // units of at most this cost are not split
 constexpr float kSlack = 8.f;      // weights may reach 2^8 before the running maximum moves
 
 __device__ __forceinline__ float ex2(float x) {
@@ -170,6 +171,7 @@ struct AttnParams {
   unsigned* counter;  // [grid] of the unit that starts in a CTA's run and goes on past it
   float* part;        // [grid][2][rows][HD]
   float2* stats;      // [grid][2][rows] (max, sum)
+  unsigned units;  // (sequence, row tile, kv head)
   bool balanced;
   Masks masks;
 };
@@ -282,6 +284,37 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   const uint32_t kld = ring + ((uint32_t)(krow * HD + ((lane >> 3) & 1) * 16) ^ k_key(krow));
   const uint32_t vld = ring + kTile * HD + ((uint32_t)((lane & 15) * HD + (lane >> 4) * 16) ^ v_key<HD>(lane & 15));
 
+  // q rows as the B operand, scaled by powers of two into f16; warps take 8 rows in turn
+  uint2* const qs = reinterpret_cast<uint2*>(smem + S::kMain + S::kSide);
+  float* const un = reinterpret_cast<float*>(smem + S::kMain + S::kSide + S::kQ);
+  auto load_q = [&](int rg, uint2 (&w)[KT]) {
+    const int row = sg.rt * RT + 8 * rg + r, t = row / p.G, g = row - t * p.G;
+    const bool real = rg < RT / 8 && t < news;
+    const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + (real ? g : 0)) * HD;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) w[kt] = real ? __ldg(reinterpret_cast<const uint2*>(src + kt * 16 + 4 * q4)) : make_uint2(0u, 0u);
+  };
+  auto store_q = [&](int rg, const uint2 (&w)[KT]) {
+    float mx = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+      mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(w[kt].x)), fabsf(bf16_hi(w[kt].x))), fmaxf(fabsf(bf16_lo(w[kt].y)), fabsf(bf16_hi(w[kt].y)))));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // 2^e with mx * 2^e in [2^14, 2^15), kept within normal floats
+    const int e = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    if (q4 == 0) un[8 * rg + r] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const float x[4] = {bf16_lo(w[kt].x) * up, bf16_hi(w[kt].x) * up, bf16_lo(w[kt].y) * up, bf16_hi(w[kt].y) * up};
+      qs[(rg * KT + kt) * 32 + lane] = make_uint2(pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]),
+                                                  pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]));
+    }
+  };
+  uint2 qw0[KT];  // this warp's first rows, asked for before the pages are looked up
+  load_q(warp, qw0);
+
   // fill the ring
   const int first = sg.tile0 + grp;
 #pragma unroll
@@ -297,36 +330,14 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
   int npa = -1, npb = -1;  // pages of the next tile to load
   if (first + (S::kStages - 1) * S::NS < sg.tile1) pages_of(first + (S::kStages - 1) * S::NS, npa, npb);
 
-  // q rows as the B operand, scaled by powers of two into f16; warps take 8 rows in turn
-  uint2* const qs = reinterpret_cast<uint2*>(smem + S::kMain + S::kSide);
-  float* const un = reinterpret_cast<float*>(smem + S::kMain + S::kSide + S::kQ);
+  if (warp < RT / 8) store_q(warp, qw0);
 #pragma unroll
-  for (int i = 0; i < (RT / 8 + kWarps - 1) / kWarps; ++i) {
-    const int rg = i * kWarps + warp;
-    if (rg >= RT / 8) break;
-    const int row = sg.rt * RT + 8 * rg + r, t = row / p.G, g = row - t * p.G;
-    const bool real = t < news;
-    const uint16_t* src = p.q + ((long long)sg.b * p.T + (real ? t : 0)) * p.ld_q + (long long)(sg.kvh * p.G + g) * HD;
-    uint2 w[KT];
-    float mx = 0.f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      w[kt] = real ? __ldg(reinterpret_cast<const uint2*>(src + kt * 16 + 4 * q4)) : make_uint2(0u, 0u);
-      mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(w[kt].x)), fabsf(bf16_hi(w[kt].x))), fmaxf(fabsf(bf16_lo(w[kt].y)), fabsf(bf16_hi(w[kt].y)))));
+  for (int i = 1; i < (RT / 8 + kWarps - 1) / kWarps; ++i)
+    if (i * kWarps + warp < RT / 8) {
+      uint2 w[KT];
+      load_q(i * kWarps + warp, w);
+      store_q(i * kWarps + warp, w);
     }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // 2^e with mx * 2^e in [2^14, 2^15), kept within normal floats
-    const int e = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-    if (q4 == 0) un[8 * rg + r] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const float x[4] = {bf16_lo(w[kt].x) * up, bf16_hi(w[kt].x) * up, bf16_lo(w[kt].y) * up, bf16_hi(w[kt].y) * up};
-      qs[(rg * KT + kt) * 32 + lane] = make_uint2(pack_f16(x[k_at<KIND>(0, 0)], x[k_at<KIND>(0, 1)]),
-                                                  pack_f16(x[k_at<KIND>(1, 0)], x[k_at<KIND>(1, 1)]));
-    }
-  }
   __syncthreads();
   const uint2* const qw = qs + wm * HH * KT * 32 + lane;
   float unscale[HH][2], m[HH][2], l[HH][2], vref = 1e-30f;  // of rows 8hh + 2 * q4 + e, as the scores below
@@ -562,14 +573,16 @@ __device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg
       float4 v[N];
 #pragma unroll
       for (int x = 0; x < N; ++x) {
-        const int k = min(k0 + x, c1);
-        const long long slot = k == c0 ? slot0 : 2 * k;
-        st[x] = __ldcg(p.stats + slot * RT + row);
-        v[x] = __ldcg(reinterpret_cast<const float4*>(p.part) + (slot * RT + row) * (HD / 4) + c);
+        st[x] = make_float2(0.f, 0.f);
+        if (k0 + x <= c1) {
+          const long long at = (long long)(k0 + x == c0 ? slot0 : 2 * (k0 + x)) * RT + row;
+          st[x] = __ldcg(p.stats + at);
+          v[x] = __ldcg(reinterpret_cast<const float4*>(p.part) + at * (HD / 4) + c);
+        }
       }
 #pragma unroll
       for (int x = 0; x < N; ++x) {
-        if (k0 + x > c1 || st[x].y == 0.f) continue;  // no position seen
+        if (st[x].y == 0.f) continue;  // no position seen
         const float mn = fmaxf(M, st[x].x), a = ex2(M - mn), f = ex2(st[x].x - mn);
         M = mn;
         L = fmaf(L, a, f * st[x].y);
@@ -592,86 +605,95 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
   constexpr int RT = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned prefix[kMaxEntries + 1];  // cost of one kv head before each entry
-  __shared__ long long wsum[kWarps];
+  __shared__ unsigned wsum[kWarps];
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   chain();
-  const long long entries = (long long)p.B * p.row_tiles;
-  const int ne = (int)min(entries, (long long)kMaxEntries);
-  long long per = 0, at = 0, end = 0;  // this CTA's run of position tiles, or of whole units
-  long long e = 0;
-  int kvh = 0;
+  // a run of position tiles (with kUnitCost more before each unit's), or every gridDim-th unit
+  unsigned per = 0, at = blockIdx.x, end = p.units;
+  int e = 0, kvh = 0;
   if (p.balanced) {
-    // tiles of each entry and their running sum
-    const int each = (ne + kThreads - 1) / kThreads, e0 = min(tid * each, ne), e1 = min(e0 + each, ne);
-    long long mine = 0;
+    // cost of each entry and their running sum
+    const int ne = p.B * p.row_tiles, each = (ne + kThreads - 1) / kThreads, e0 = min(tid * each, ne), e1 = min(e0 + each, ne);
+    unsigned mine = 0;
     for (int i = e0; i < e1; ++i) {
       int news, len;
       mine += unit_cost(positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len));
     }
-    long long inc = mine;
+    unsigned inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    long long sum = inc - mine;
+    unsigned sum = inc - mine;
     for (int w = 0; w < warp; ++w) sum += wsum[w];
     for (int i = e0; i < e1; ++i) {
       int news, len;
-      prefix[i] = (unsigned)sum;
+      prefix[i] = sum;
       sum += unit_cost(positions<RT>(p, i / p.row_tiles, i % p.row_tiles, &news, &len));
     }
-    if (e1 == ne && e0 < e1) prefix[ne] = (unsigned)sum;
+    if (e1 == ne && e0 < e1) prefix[ne] = sum;
     __syncthreads();
-    const long long total = (long long)prefix[ne] * p.hkv;
-    per = max((total + gridDim.x - 1) / gridDim.x, (long long)kMinTiles);
-    at = blockIdx.x * per;
-    end = min(at + per, total);
-    int lo = 0, hi = ne - 1;  // the entry that holds tile `at`: the last with hkv * prefix <= at
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((long long)prefix[mid] * p.hkv <= at) lo = mid;
-      else hi = mid - 1;
+    const unsigned total = prefix[ne] * p.hkv;
+    per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kMinTiles);
+    // the entry that holds x < total: the last with hkv * prefix <= x
+    auto entry_of = [&](unsigned x) {
+      int lo = 0, hi = ne - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (prefix[mid] * p.hkv <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      return lo;
+    };
+    // run boundaries inside a short unit move to its nearer end
+    auto boundary = [&](unsigned i) {
+      const unsigned x = i * per;
+      if (x >= total) return total;
+      const int b = entry_of(x);
+      const unsigned cost = prefix[b + 1] - prefix[b], into = (x - prefix[b] * p.hkv) % cost;
+      return cost > kWholeCost ? x : 2 * into < cost ? x - into : x - into + cost;
+    };
+    at = boundary(blockIdx.x);
+    end = boundary(blockIdx.x + 1);
+    if (at < end) {
+      e = entry_of(at);
+      kvh = (int)((at - prefix[e] * p.hkv) / (prefix[e + 1] - prefix[e]));
     }
-    e = lo;
-    if (at < end) kvh = (int)((at - (long long)prefix[e] * p.hkv) / (prefix[e + 1] - prefix[e]));
-  } else {
-    at = blockIdx.x;
-    end = entries * p.hkv;
   }
+  const unsigned begin = at;
   while (at < end) {
     Segment sg;
-    long long r0 = 0, u1 = 0, stop = 0;  // the unit's first tile and end, this CTA's end in it
+    unsigned r0 = 0, u1 = 0;  // the unit's first tile and its end
     bool whole = true, leads = false;
     if (p.balanced) {
-      const long long cost = prefix[e + 1] - prefix[e];
+      const unsigned cost = prefix[e + 1] - prefix[e];
       if (kvh == p.hkv || cost == 0) {
         ++e;
         kvh = 0;
         continue;
       }
-      r0 = (long long)prefix[e] * p.hkv + kvh * cost + kUnitCost;
+      r0 = prefix[e] * p.hkv + kvh * cost + kUnitCost;
       u1 = r0 + cost - kUnitCost;
-      stop = min(end, u1);
-      const long long s0 = max(at, r0);
+      const unsigned stop = min(end, u1), s0 = max(at, r0);
       at = stop;
       sg.kvh = kvh++;
       if (s0 >= stop) continue;
       sg.tile0 = (int)(s0 - r0);
       sg.tile1 = (int)(stop - r0);
       whole = s0 == r0 && stop == u1;
-      leads = s0 == blockIdx.x * per;
+      leads = s0 == begin;
     } else {
-      e = at / p.hkv;
+      e = (int)(at / p.hkv);
       sg.kvh = (int)(at % p.hkv);
-      at += gridDim.x;
+      at = at + gridDim.x < at ? end : at + gridDim.x;
     }
-    sg.b = (int)(e / p.row_tiles);
-    sg.rt = (int)(e % p.row_tiles);
+    sg.b = e / p.row_tiles;
+    sg.rt = e % p.row_tiles;
     if (!p.balanced) {
       int news, len;
       const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
@@ -791,7 +813,10 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   p.out = out;
   p.ld_out = ld_out;
   // the sums of costs fit 32 bits, whatever the lengths
-  p.balanced = B * p.row_tiles <= kMaxEntries && B * p.row_tiles * (max_pages * p.P / kTile + 1 + kUnitCost) < (1LL << 32);
+  if (B * p.row_tiles > 0xffffffffLL / p.hkv) return WAL_ERR_SHAPE;
+  p.units = (unsigned)(B * p.row_tiles * p.hkv);
+  p.balanced = B * p.row_tiles <= kMaxEntries &&
+               (long long)p.units * (max_pages * p.P / kTile + 1 + kUnitCost) + (long long)grid * kMinTiles * 2 < (1LL << 31);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counter = reinterpret_cast<unsigned*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes(grid));
