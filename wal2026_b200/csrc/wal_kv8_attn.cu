@@ -87,7 +87,7 @@ __device__ __forceinline__ void ldsm_t8_x2(uint32_t addr, uint32_t (&m)[4]) {
 // The transpose of an 8 x 8 matrix of 16-bit values, two neighbours of a row per lane.
 __device__ __forceinline__ uint32_t transpose(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -480,18 +480,21 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
 #pragma unroll
       for (int c = 0; c < C; c += 2) {
         uint32_t w[4];
+        uint32_t a[2][4];
         ldsm_t8_x2((vs ^ (uint32_t)(c << 4)) + j * 16 * HD, w);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          uint32_t a[4];
-          to_bf16<KIND>(mk, w[2 * x], a[0], a[2]);
-          to_bf16<KIND>(mk, w[2 * x + 1], a[1], a[3]);
-#pragma unroll
-          for (int hh = 0; hh < HH; ++hh) {
-            mma_bf16(o[c + x][hh], a, hi[hh][0], hi[hh][1]);
-            mma_bf16(o[c + x][hh], a, lo[hh][0], lo[hh][1]);
-          }
+          to_bf16<KIND>(mk, w[2 * x], a[x][0], a[x][2]);
+          to_bf16<KIND>(mk, w[2 * x + 1], a[x][1], a[x][3]);
         }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int hh = 0; hh < HH; ++hh) mma_bf16(o[c + x][hh], a[x], hi[hh][0], hi[hh][1]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int hh = 0; hh < HH; ++hh) mma_bf16(o[c + x][hh], a[x], lo[hh][0], lo[hh][1]);
       }
     }
   }
