@@ -180,6 +180,70 @@ def test_attention_extreme_scores_and_scales():
     _check_attention(cache, q, table, [n - 1], scale=-0.3)
 
 
+def test_attention_of_more_sequences_than_the_balance_sums():
+    # 1100 sequences take the path that gives each CTA whole units; some are empty tables, some idle
+    P, hd, hq, hkv, B = 16, 64, 4, 2, 1100
+    lens = [(i * 7) % 40 for i in range(B)]
+    ends = [n + 1 for n in lens]
+    pages = sum(-(-n // P) for n in ends)
+    cache = _filled(1, pages, hkv, P, hd, E4M3, 51)
+    table = _tables(ends, P, pages, 9)
+    news = [0 if i % 13 == 5 else 1 for i in range(B)]
+    q = torch.randn(B, hq * hd, device=DEV, generator=_gen(52)).to(torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    kv8_attention(cache, 0, q, table, _i32(lens), out, kv8_attention_workspace(cache, B, hq), new_lens=_i32(news))
+    for a in range(0, B, 550):  # the same rows in calls that are balanced: the order of sums differs, a rounding at most
+        part = torch.empty_like(q[a:a + 550])
+        kv8_attention(cache, 0, q[a:a + 550], table[a:a + 550], _i32(lens[a:a + 550]), part,
+                      kv8_attention_workspace(cache, 550, hq), new_lens=_i32(news[a:a + 550]))
+        diff = (part.float() - out[a:a + 550].float()).abs()
+        assert bool((diff <= 2.0 ** -7 * part.float().abs() + 1e-6).all())
+    pick = [0, 1, 5, 18, 700, 1099]
+    want, mag = _attention64(cache, 0, q[pick], table[pick], [lens[i] for i in pick], [news[i] for i in pick], hd ** -0.5)
+    assert bool(((out[pick].double() - want).abs() <= 2 * (2.0 ** -8 * want.abs() + 2.0 ** -11 * mag) + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("hq,T", [(4, 1), (8, 2), (8, 3), (16, 4)])
+def test_attention_every_code_counts(dtype, hq, T):
+    # each code as a V value at one position that has nearly all the weight, e4m3's subnormals included, and as a K value
+    P, hd, n = 64, 64, 256
+    codes = torch.arange(256, device=DEV).to(torch.uint8)
+    if dtype == INT8:
+        codes[128] = 0  # -128 is not a code
+    else:
+        codes[0x7F], codes[0xFF] = 0, 0  # NaN is none either
+    cache = _filled(1, 4, 1, P, hd, dtype, 61)
+    cache.scales[:] = 1.0
+    cache.codes.view(torch.uint8)[0, 1, :, 0] = codes.view(4, P, 1).expand(4, P, hd)  # V: position j holds code j in every dim
+    for shift in (0, 100):
+        k = torch.zeros(n, hd, dtype=torch.uint8, device=DEV)
+        for d in range(hd):
+            k[:, d] = codes.roll(shift + 3 * d)
+        cache.codes.view(torch.uint8)[0, 0, :, 0] = k.view(4, P, hd)
+        q = (torch.randn(T, hq * hd, device=DEV, generator=_gen(62 + shift)) * 0.02).to(torch.bfloat16)
+        _check_attention(cache, q, _i32([[0, 1, 2, 3]]), [n - T])
+
+
+@pytest.mark.parametrize("hq,T", [(4, 1), (8, 2), (16, 4)])
+def test_attention_keeps_a_bad_row_to_itself(hq, T):
+    P, hd = 32, 128
+    cache = _filled(1, 20, 1, P, hd, INT8, 71)
+    table = _tables([500], P, 20, 3)
+    q = torch.randn(T, hq * hd, device=DEV, generator=_gen(72)).to(torch.bfloat16)
+    ws = kv8_attention_workspace(cache, 1, hq, T)
+    good, bad = torch.empty_like(q), torch.empty_like(q)
+    kv8_attention(cache, 0, q, table, _i32([500 - T]), good, ws)
+    for value in (float("nan"), float("inf")):
+        worse = q.clone()
+        worse[T - 1, hd + 5] = value  # head 1 of the last token
+        kv8_attention(cache, 0, worse, table, _i32([500 - T]), bad, ws)
+        assert bool(bad[T - 1, hd:2 * hd].isnan().all())
+        rest = torch.ones_like(q, dtype=torch.bool)
+        rest[T - 1, hd:2 * hd] = False
+        assert torch.equal(bad[rest], good[rest])
+
+
 def test_attention_strided_rows_one_workspace_and_another_stream():
     P, hd, hq, hkv = 64, 128, 8, 2
     cache = _filled(1, 80, hkv, P, hd, E4M3, 31)
