@@ -4,11 +4,23 @@
 //                      sequence into their pages.  A CTA owns one (sequence,
 //                      touched page, kv head) of K or of V: it reads its new
 //                      values, takes their largest magnitude a, sets the block's
-//                      scale to max(old, a * (1 / Q)), re-rounds the earlier codes of
-//                      the block where the scale grew, and stores the codes.
-//                      Further CTAs rotate q.  Rotation rounds each product and
-//                      sum in fp32; K is rounded once, from fp32 to its code.
+//                      scale to max(old, a * (1 / Q)), re-rounds the earlier codes
+//                      of the block where the scale grew, and stores the codes.
+//                      No other CTA touches the block, so the result has one
+//                      order; a page's values stay in registers between the
+//                      maximum and the codes.  Further CTAs rotate q, a warp per
+//                      token and group of heads that share one load of angles.
+//                      Rotation rounds each product and sum in fp32; K is rounded
+//                      once, from fp32 to its code.
 //   kv8_read_kernel    values code * scale of a range of positions.
+//
+// Bounds, on B200: four prompts of 1270 tokens on average (64 query and 8 kv heads of 128; 8192 rows
+// with padding): append 55 us for 277 MB, 5.0 TB/s or 77% of a copy's rate, of which
+// 265 MB are q and qkv; read-back 13 us for 48 MB.  A decode step of three
+// sequences takes 4.6 us for both kernels, all of it launch and two dependent
+// loads.  Threads per CTA and CTAs per SM: 256 and 3 against 128 and 5 made no
+// difference to the whole (68 us); fewer looping query warps lose (72 us with 3
+// CTAs per SM, 68 with 16).
 #include "wal_kv8.cuh"
 
 namespace {

@@ -13,6 +13,10 @@
 // order of tokens is the order of warps) and sends the sum to the others; the
 // warp whose share holds the drawn place reads it once more.  One row of p and,
 // after a rejection, one of q is all that is read.
+//
+// On B200, 128256 tokens: one sequence 6.6 us (1 MB: three dependent loads, the
+// sums, a cluster barrier and the second reading of one share), 64 sequences 20.5 us for 66
+// MB, 3.2 TB/s: half the time is the same chain before and after the rows stream.
 #include "wal_kv8.cuh"
 
 #include <cooperative_groups.h>

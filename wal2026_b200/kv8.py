@@ -122,9 +122,14 @@ def _batch(rows: int, table: Tensor, lens: Tensor, new_lens: Optional[Tensor]) -
         _i32("new_lens", new_lens, B)
 
 
+_entry: dict = {}
+
+
 def _call(index: int, name: str, *args) -> None:
     """One entry point on the current stream of device ``index``."""
-    fn = getattr(_abi.load(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_abi.load(), name)
     if _abi._raw_stream is not None and index == _current_device():
         st = fn(*args, _abi._raw_stream(index))
     else:
@@ -134,15 +139,18 @@ def _call(index: int, name: str, *args) -> None:
         _abi.check(st, name)
 
 
-def _is_step(cache: PagedKV8Cache, x: Tensor, width: int, y: Tensor, hq: int, table: Tensor, lens: Tensor,
-             new_lens: Optional[Tensor]) -> bool:
-    """Token rows x [B * T, width] and y [B * T, hq * head_dim], a table and lengths, all fit to launch."""
+def _step(cache: PagedKV8Cache, x: Tensor, width: int, y: Tensor, hq: int, table: Tensor, lens: Tensor,
+          new_lens: Optional[Tensor]) -> Optional[tuple]:
+    """(sequences, tokens each, pages, strides of x, y, table) where token rows x [B * T, width] and y [B * T, hq *
+    head_dim], a table and lengths all fit to launch."""
     i, ts, xs, x1, y1, t1 = cache.index, table.shape, x.shape, x.stride(), y.stride(), table.stride()
-    return (i >= 0 and len(ts) == 2 and len(xs) == 2 and ts[0] > 0 and xs[0] > 0 and xs[0] % ts[0] == 0 and xs[1] == width
+    if (i >= 0 and len(ts) == 2 and len(xs) == 2 and ts[0] > 0 and xs[0] > 0 and xs[0] % ts[0] == 0 and xs[1] == width
             and y.shape == (xs[0], hq * cache.head_dim) and x1[1] == 1 and y1[1] == 1 and t1[1] == 1 and t1[0] >= ts[1]
             and x.dtype is _BF16 and y.dtype is _BF16 and table.dtype is _I32 and x.get_device() == i
             and y.get_device() == i and table.get_device() == i and _is_i32(lens, ts[:1], i)
-            and (new_lens is None or _is_i32(new_lens, ts[:1], i)))
+            and (new_lens is None or _is_i32(new_lens, ts[:1], i))):
+        return ts[0], xs[0] // ts[0], ts[1], x1[0], y1[0], t1[0]
+    return None
 
 
 def _why_not_append(cache, qkv, hq, table, lens, q_out, cos, sin, new_lens) -> None:
@@ -159,6 +167,7 @@ def _why_not_append(cache, qkv, hq, table, lens, q_out, cos, sin, new_lens) -> N
             if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd // 2 or not t.is_contiguous() or t.shape != cos.shape:
                 raise ValueError(f"{name} must be fp32 [max_pos, head_dim / 2] contiguous")
     _on(cache.device, qkv=qkv, q_out=q_out, table=table, lens=lens, new_lens=new_lens, cos=cos, sin=sin)
+    raise ValueError("kv8_append: arguments do not fit together")
 
 
 def kv8_append(cache: PagedKV8Cache, layer: int, qkv: Tensor, hq: int, table: Tensor, lens: Tensor, q_out: Tensor, *,
@@ -172,18 +181,19 @@ def kv8_append(cache: PagedKV8Cache, layer: int, qkv: Tensor, hq: int, table: Te
     codes are re-rounded when it does.
     """
     hd, max_pos = cache.head_dim, 0
-    fit = _is_step(cache, qkv, (hq + 2 * cache.kv_heads) * hd, q_out, hq, table, lens, new_lens) and (cos is None) == (sin is None)
+    step = _step(cache, qkv, (hq + 2 * cache.kv_heads) * hd, q_out, hq, table, lens, new_lens)
+    fit = step is not None and (cos is None) == (sin is None)
     if fit and cos is not None:
-        max_pos = cos.shape[0] if cos.dim() == 2 else 0
-        fit = (cos.shape == (max_pos, hd // 2) and sin.shape == cos.shape and cos.dtype is _F32 and sin.dtype is _F32
+        cs = cos.shape
+        max_pos = cs[0] if len(cs) == 2 else 0
+        fit = (cs == (max_pos, hd // 2) and sin.shape == cs and cos.dtype is _F32 and sin.dtype is _F32
                and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == cache.index)
     if not fit:
         _why_not_append(cache, qkv, hq, table, lens, q_out, cos, sin, new_lens)
-    B, width = table.shape
-    _call(cache.index, "wal_kv8_append", cache._ref, layer, qkv.data_ptr(), qkv.stride()[0], B, qkv.shape[0] // B, hq,
-          table.data_ptr(), table.stride()[0], width, lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
-          None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), max_pos, q_out.data_ptr(),
-          q_out.stride()[0])
+    B, T, pages, ld_x, ld_q, ld_t = step
+    _call(cache.index, "wal_kv8_append", cache._ref, layer, qkv.data_ptr(), ld_x, B, T, hq, table.data_ptr(), ld_t, pages,
+          lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), None if cos is None else cos.data_ptr(),
+          None if sin is None else sin.data_ptr(), max_pos, q_out.data_ptr(), ld_q)
 
 
 def _why_not_read(cache, table, first, count, k_out, v_out) -> None:
@@ -236,6 +246,7 @@ def _why_not_attention(cache, q, table, lens, out, workspace, new_lens) -> None:
     _on(cache.device, q=q, out=out, table=table, lens=lens, new_lens=new_lens, workspace=workspace)
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
+    raise ValueError("kv8_attention: arguments do not fit together")
 
 
 def kv8_attention(cache: PagedKV8Cache, layer: int, q: Tensor, table: Tensor, lens: Tensor, out: Tensor,
@@ -250,13 +261,14 @@ def kv8_attention(cache: PagedKV8Cache, layer: int, q: Tensor, table: Tensor, le
     hd = cache.head_dim
     width = q.shape[-1] if q.dim() else 0
     hq = width // hd
-    if not (_is_step(cache, q, width, out, hq, table, lens, new_lens) and width > 0 and width % (hd * cache.kv_heads) == 0
+    step = _step(cache, q, width, out, hq, table, lens, new_lens)
+    if not (step is not None and width > 0 and width % (hd * cache.kv_heads) == 0
             and workspace.get_device() == cache.index and workspace.is_contiguous()):
         _why_not_attention(cache, q, table, lens, out, workspace, new_lens)
-    B, pages = table.shape
-    _call(cache.index, "wal_kv8_attention", cache._ref, layer, q.data_ptr(), q.stride()[0], B, q.shape[0] // B, hq,
-          table.data_ptr(), table.stride()[0], pages, lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
-          hd ** -0.5 if scale is None else scale, out.data_ptr(), out.stride()[0], workspace.data_ptr(), workspace.nbytes)
+    B, T, pages, ld_q, ld_o, ld_t = step
+    _call(cache.index, "wal_kv8_attention", cache._ref, layer, q.data_ptr(), ld_q, B, T, hq, table.data_ptr(), ld_t, pages,
+          lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), hd ** -0.5 if scale is None else scale,
+          out.data_ptr(), ld_o, workspace.data_ptr(), workspace.nbytes)
 
 
 def _why_not_assign(table, parent, keep, add, table_out, ref_out, copy_src, copy_dst, info) -> None:
