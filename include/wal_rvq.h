@@ -529,8 +529,8 @@ typedef struct wal_kv8_cache {
  * times the fp32 number next to 1 / Q) and a new code is round-to-nearest-even of x / s clamped to [-Q, Q] (an
  * infinity saturates, a NaN and every value of a block with s = 0 becomes 0);
  * where s > s0 the earlier codes c become the codes of c * (s0 / s).  Tokens
- * whose position has no page, or is max_pos or more, are not stored.  Pages
- * written here must belong to one sequence alone (wal_kv_pages_assign).
+ * whose position has no page, or is max_pos or more, are not stored (past
+ * max_pos q_out is zeros too).  Pages written here must belong to one sequence alone (wal_kv_pages_assign).
  * qkv, q_out, cos, sin 16-byte aligned; ld_qkv, ld_q multiples of 8.
  */
 WAL_API int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qkv, int64_t ld_qkv, int64_t B,
@@ -554,10 +554,10 @@ WAL_API int wal_kv8_read(const wal_kv8_cache* cache, int32_t layer, int64_t B, c
  * a kv head.  Rows with t >= new_lens[b], and rows without a position that has
  * a page, are zeros.  q, out: bf16 rows ld_q / ld_out apart, heads contiguous,
  * 16-byte aligned, ld multiples of 8; any hq that is a multiple of kv_heads.
- * workspace: at least wal_kv8_attention_workspace bytes (0 = invalid shape),
- * 256-byte aligned and zero-filled before its first use; calls leave it ready
- * for the next one, whatever its lengths, and calls that share one must not
- * overlap in time.
+ * workspace: at least wal_kv8_attention_workspace bytes (0 = invalid shape; it
+ * never shrinks with more tokens T), 256-byte aligned and zero-filled before its
+ * first use; calls leave it ready for the next one, whatever its lengths and
+ * tokens, and calls that share one must not overlap in time.
  */
 WAL_API size_t wal_kv8_attention_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq);
 WAL_API int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t* q, int64_t ld_q, int64_t B,

@@ -265,6 +265,18 @@ def test_attention_strided_rows_one_workspace_and_another_stream():
     assert torch.equal(a, b)
 
 
+def test_attention_workspace_shared_by_steps_of_different_sizes():
+    # one workspace for steps of 1 to 30 tokens in turn: each must find its counters at zero
+    P, hd, hq, hkv, B = 64, 64, 8, 1, 2
+    lens = [3000, 1700]
+    cache = _filled(1, 80, hkv, P, hd, INT8, 81)
+    table = _tables([n + 30 for n in lens], P, 80, 4)
+    ws = kv8_attention_workspace(cache, B, hq, 30)
+    for T in (1, 12, 1, 16, 2, 30, 1, 3, 5, 1, 8, 6, 1):
+        q = torch.randn(B * T, hq * hd, device=DEV, generator=_gen(T)).to(torch.bfloat16)
+        _check_attention(cache, q, table, lens, ws=ws)
+
+
 def test_attention_offsets_past_32_bits():
     # 2.4e9 code bytes in one pool half: the last page starts past 2^31
     P, hd, hkv, pages = 64, 128, 8, 36700
@@ -535,6 +547,13 @@ def test_assign_many_rows_and_pages():
     table = _tables(lens, P, need + rows, 2)
     _check_assign(table, [i if i % 5 else i // 2 for i in range(rows)], [n if i % 5 else lens[i // 2] for i, n in enumerate(lens)],
                   [i % 3 for i in range(rows)], P, need + rows)
+
+
+def test_assign_as_many_rows_as_it_takes():
+    P, rows = 16, 16383
+    table = _i32([[0, 1]])
+    # every row continues one sequence: page 0 is shared, page 1 copied by all but the first, and a page runs short
+    _check_assign(table, [0] * rows, [20] * rows, [1] * rows, P, rows)
 
 
 @pytest.mark.parametrize("P,pages,rows,hi", [(16, 50, 4, 100), (64, 3000, 40, 2000), (32, 8, 1, 0), (16, 2049, 300, 90)])

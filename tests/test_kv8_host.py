@@ -86,6 +86,12 @@ def test_attention_workspace_of_invalid_shapes_is_zero():
         assert lib.wal_kv8_attention_workspace(None if c is None else ctypes.byref(c), B, T, hq) == 0
 
 
+def test_attention_workspace_never_shrinks_with_more_tokens():
+    lib, c = _abi.load(), _c()
+    sizes = [lib.wal_kv8_attention_workspace(ctypes.byref(c), 3, T, 4) for T in range(1, 200)]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
 ASSIGN = dict(table=P256, ld_table=6, rows_in=3, parent=P256, keep=P256, add=P256, rows=4, width=6, num_pages=9, page_size=16,
               out=P256, ld_out=6, ref=P256, src=P256, dst=P256, info=P256, stream=None)
 COMPACT = dict(table=P256, ld_table=6, lens=P256, rows=4, width=6, num_pages=9, page_size=16, out=P256, ld_out=6, remap=P256,

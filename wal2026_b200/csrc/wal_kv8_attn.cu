@@ -760,7 +760,9 @@ int row_tile(int64_t T, int G) {
 // CTAs that fill the GPU once.
 int grid_of(int rows) { return sm_count() * (rows == 8 ? 3 : 2); }
 
-size_t counter_bytes(int grid) { return ((size_t)grid * sizeof(unsigned) + 255) & ~(size_t)255; }
+// The counters have one place whatever the row tile, so that calls of different
+// tokens per sequence find them at zero where the others left them.
+size_t counter_bytes() { return ((size_t)3 * sm_count() * sizeof(unsigned) + 255) & ~(size_t)255; }
 
 template <int HD, int KIND, int RW, int WM>
 int launch(const AttnParams& p, int grid, cudaStream_t st) {
@@ -796,9 +798,10 @@ extern "C" {
 
 size_t wal_kv8_attention_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq) {
   if (!cache || cache->kv_heads <= 0 || B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads || T > 0x7fffffff) return 0;
-  const int64_t rows = row_tile(T, hq / cache->kv_heads);
+  int64_t rows = row_tile(T, hq / cache->kv_heads);
+  if (rows == 64 && T * (hq / cache->kv_heads) > 64) rows = 96;  // never less for more tokens
   const int grid = grid_of((int)rows);
-  return counter_bytes(grid) + (size_t)grid * 2 * rows * (cache->head_dim * sizeof(float) + sizeof(float2));
+  return counter_bytes() + (size_t)grid * 2 * rows * (cache->head_dim * sizeof(float) + sizeof(float2));
 }
 
 int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t* q, int64_t ld_q, int64_t B, int64_t T,
@@ -842,7 +845,7 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
                (long long)p.units * (max_pages * p.P / kTile + 1 + kUnitCost) + (long long)grid * kMinTiles * 2 < (1LL << 31);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counter = reinterpret_cast<unsigned*>(ws);
-  p.part = reinterpret_cast<float*>(ws + counter_bytes(grid));
+  p.part = reinterpret_cast<float*>(ws + counter_bytes());
   p.stats = reinterpret_cast<float2*>(p.part + (size_t)grid * 2 * rows * hd);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (hd == 128)

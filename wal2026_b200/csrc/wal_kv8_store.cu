@@ -376,9 +376,9 @@ int wal_kv8_append(const wal_kv8_cache* cache, int32_t layer, const uint16_t* qk
   p.q_out = q_out;
   p.ld_q = ld_q;
   p.kv = layer_view(*cache, layer);
-  const long long kv_ctas = 2LL * B * p.touched * p.hkv;
   const int heads = hd == 128 ? kHeads<128>() : kHeads<64>();
   if (B * T > 0x3fffffff / ((hq + heads - 1) / heads)) return WAL_ERR_SHAPE;
+  const long long kv_ctas = 2LL * B * p.touched * p.hkv;
   p.q_items = (unsigned)(B * T * ((hq + heads - 1) / heads));
   const long long q_most = (p.q_items + kThreads / 32 - 1) / (kThreads / 32), q_ctas = q_most < 16LL * sm_count() ? q_most : 16LL * sm_count();
   if (kv_ctas + q_ctas > 0x7fffffff) return WAL_ERR_SHAPE;
