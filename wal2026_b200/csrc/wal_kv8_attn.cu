@@ -728,10 +728,10 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
     if (!whole) {
       const int c0 = (int)(r0 / per), c1 = (int)((u1 - 1) / per);
       if (tid == 0) {  // the other threads' stores came before the barrier that ended run_segment
-        __threadfence();
-        last = atomicAdd(p.counter + c0, 1u) == (unsigned)(c1 - c0);
+        unsigned before;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counter + c0) : "memory");
+        last = before == (unsigned)(c1 - c0);
         if (last) p.counter[c0] = 0u;  // ready for the next call
-        __threadfence();
       }
       __syncthreads();
       if (last) join_runs<HD, RW, WM>(p, sg, c0, c1, 2 * c0 + (r0 == c0 * per ? 0 : 1));
