@@ -11,11 +11,11 @@
 //                            pages below it, both in rising order.
 //   kv_pages_copy_kernel     page src[i] -> dst[i] in every layer, K, V, scales.
 //
-// The first two are one cluster each, of one CTA for small pools and of eight
-// for large ones: what they do is a few dependent passes over a few hundred
+// The first two are one cluster each, of one CTA for small pools and of eight or
+// sixteen for large ones: what they do is a few dependent passes over a few hundred
 // kilobytes, bound by the latency of the passes and of the barriers between, so
 // rows are kept in shared memory and pages read eight at a time.  On B200: tables
-// of 256 sequences with 65 k entries 20 us (96 us as one CTA, half of it atomics),
+// of 256 sequences with 65 k entries 12 us (96 us as one CTA, half of it atomics),
 // of 64 forked rows 9 us, a compaction of 2055 pages 13 us.  The copy moves 266 MB
 // of scattered 16 KB pieces in 48 us, 5.5 TB/s or 85% of a copy's rate; with CTAs
 // that first list the valid pairs together it took 60 us.
@@ -30,7 +30,7 @@ using namespace wal_kv8;
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCluster = 8;
+constexpr int kCluster = 16;  // at most
 
 // Exclusive prefix sum over the CTA; *total gets the sum.  sm: kWarps ints.
 __device__ __forceinline__ int block_scan(int v, int* sm, int* total) {
@@ -433,8 +433,39 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) kv_pages_copy_ke
   }
 }
 
-// CTAs of the table kernels' cluster.
-int table_cluster(int64_t entries, int64_t pages) { return entries + pages > 4 * kThreads ? kCluster : 1; }
+// CTAs of a table kernel's cluster: one for small tables, eight for larger ones, and
+// sixteen, where the device schedules clusters beyond the portable eight, when
+// the entries' atomics and stores outweigh the barriers (256 sequences with 65 k
+// entries: 24.8 us with eight, 16.5 with sixteen; a pool of 2055 pages with 1200: no difference).
+template <typename Kern>
+int table_cluster(Kern kern, int64_t entries, int64_t pages) {
+  if (entries + pages <= 4 * kThreads) return 1;
+  if (entries + pages <= 16 * kThreads) return 8;
+  static std::atomic<int> known[kMaxDevices];  // 1: eight, 2: sixteen
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 8;
+  int can = known[dev].load(std::memory_order_relaxed);
+  if (can == 0) {
+    can = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kCluster);
+    cfg.blockDim = dim3(kThreads);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
+      can = 2;
+    (void)cudaGetLastError();  // a refusal is an answer
+    known[dev].store(can, std::memory_order_relaxed);
+  }
+  return can == 2 ? kCluster : 8;
+}
 
 }  // namespace
 
@@ -455,7 +486,7 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
   const int smem = (3 * (int)rows + 1 + ((int)rows + 31) / 32) * (int)sizeof(int);
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kv_pages_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return WAL_ERR_CUDA;
-  const int cluster = table_cluster(rows * width, num_pages);
+  const int cluster = table_cluster(kv_pages_assign_kernel, rows * width, num_pages);
   return launch_chain(kv_pages_assign_kernel, dim3((unsigned)cluster), kThreads, smem, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
@@ -468,7 +499,7 @@ int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* 
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   CompactParams p = {table, ld_table, lens, (int)rows, (int)width, (int)num_pages, page_size, table_out, ld_out, remap,
                      move_src, move_dst, info};
-  const int cluster = table_cluster(rows * width, num_pages);
+  const int cluster = table_cluster(kv_pages_compact_kernel, rows * width, num_pages);
   return launch_chain(kv_pages_compact_kernel, dim3((unsigned)cluster), kThreads, 0, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
