@@ -45,12 +45,14 @@
 // conversions of the codes (five instructions for four K codes, seven for four V
 // codes, 830 instructions per warp and tile in all) make it 190 us.  Small calls
 // are a chain of latencies: lengths 2 us, pages and first tile 2.5 us, joining
-// runs 3 us; one sequence of 2048 takes 10.5 us where its bytes take 0.7.  More
+// runs 3 us; one sequence of 2048 takes 10.2 us where its bytes take 0.7.  More
 // rows add products: 16 sequences of 4300 on average with 8 / 16 / 24 / 32 / 64
 // rows per kv head take 37 / 49 / 61 / 82 / 148 us (memory: 23), bound by the
-// latency of dependent products and conversions at two warps per scheduler.
+// instructions of conversions and products, which dependent chains at two warps per
+// scheduler issue at half rate.
 // Measured slower: the two products of a tile split between two warps that pass
-// weights through shared memory (24 rows 69 us); 3 stages and 2 CTAs per SM for 8
+// weights through shared memory (24 rows 69 us); four warps of eight rows, each
+// converting for itself (32 rows 108 us); 3 stages and 2 CTAs per SM for 8
 // rows (168 us against 162); three 8-bit digits of q times K codes in integers,
 // which needs no conversion of K (187 us sustained, but 11.1 us for the single
 // sequence).
