@@ -16,7 +16,7 @@
 // kilobytes, bound by the latency of the passes and of the barriers between, so
 // rows are kept in shared memory and pages read eight at a time.  On B200: tables
 // of 256 sequences with 65 k entries 12 us (96 us as one CTA, half of it atomics),
-// of 64 forked rows 9 us, a compaction of 2055 pages 13 us.  The copy moves 266 MB
+// of 64 forked rows 7 us, a compaction of 2055 pages 13 us.  The copy moves 266 MB
 // of scattered 16 KB pieces in 48 us, 5.5 TB/s or 85% of a copy's rate; with CTAs
 // that first list the valid pairs together it took 60 us.
 #include "wal_kv8.cuh"
@@ -433,13 +433,15 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) kv_pages_copy_ke
   }
 }
 
-// CTAs of a table kernel's cluster: one for small tables, eight for larger ones, and
-// sixteen, where the device schedules clusters beyond the portable eight, when
+// CTAs of a table kernel's cluster, with the copy's time: one where each thread has
+// at most one entry or page (36 pages of 6 sequences: 10.3 us with one or eight),
+// eight for more (64 rows forked over 380 pages: 26.8 us with one, 25.2 with eight),
+// and sixteen, where the device schedules clusters beyond the portable eight, when
 // the entries' atomics and stores outweigh the barriers (256 sequences with 65 k
-// entries: 24.8 us with eight, 16.5 with sixteen; a pool of 2055 pages with 1200: no difference).
+// entries: 24.8 us with eight, 16.5 with sixteen; 2055 pages with 1200 entries: 62 us either way).
 template <typename Kern>
 int table_cluster(Kern kern, int64_t entries, int64_t pages) {
-  if (entries + pages <= 4 * kThreads) return 1;
+  if (entries + pages <= kThreads) return 1;
   if (entries + pages <= 16 * kThreads) return 8;
   static std::atomic<int> known[kMaxDevices];  // 1: eight, 2: sixteen
   int dev = 0;
