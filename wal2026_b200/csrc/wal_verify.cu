@@ -114,6 +114,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) verify_kernel(const __grid_con
   const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
   const int b = blockIdx.x / ncta, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   chain();
+  // a CTA's shared memory may be written by the others once it has started
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   const int* x = p.drafts + b * p.ld_drafts;
   const int len = p.draft_lens ? min(max(p.draft_lens[b], 0), p.T) : p.T;
   const unsigned long long place = uniform24(p.u[b * p.ld_u + p.T]);
@@ -163,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) verify_kernel(const __grid_con
     sum = warp_sum(sum);
     if (lane == 0) warps[warp] = sum;
     __syncthreads();
+    if (pass == 0) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
     if (warp == 0) {
       const unsigned long long mine = warp_sum(lane < kWarps ? warps[lane] : 0ull);
       if (lane < ncta) cl.map_shared_rank(&ctas[pass][0], lane)[rank] = mine;
