@@ -1,0 +1,58 @@
+"""Weights of the 8-bit cache attention near their largest, for every row tile and both code types.
+
+Bounds, against the softmax in 64 bits over the cache's own values.  The output
+is rounded once to bf16: 2^-8 of the value.  A weight is the sum of two bf16
+numbers: the first leaves at most 2^-8 of it, the second at most 2^-8 of that,
+so 2^-16 of the weight.  Scores of a few units in fp32 move a weight by 2^-18 or
+so (a product of 128 terms in 8 steps), the base-two exponential by 2^-22, and
+sums over a few hundred positions by 2^-18; together they stay below another
+2^-16.  So an element is off by at most 2^-8 of its size and 2^-15 of the
+weighted mean of |v|.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from wal2026_b200.kv8 import kv8_attention, kv8_attention_workspace
+
+from .test_gpu_kv8 import DEV, E4M3, INT8, _attention64, _filled, _i32
+
+pytestmark = pytest.mark.gpu
+ROWS = [8, 16, 24, 32, 48, 64, 96]  # query rows per kv head: one call of each row tile
+
+
+def _attend(cache, q, table, lens, scale=None):
+    B, hq = table.shape[0], q.shape[1] // cache.head_dim
+    out = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device=DEV)
+    kv8_attention(cache, 0, q, table, _i32(lens), out, kv8_attention_workspace(cache, B, hq, q.shape[0] // B), scale=scale)
+    return out.double()
+
+
+def _bound(want, mag):
+    return 2.0 ** -8 * want.abs() + 2.0 ** -15 * mag + 1e-30
+
+
+def _check(out, want, mag):
+    bad = ~((out - want).abs() <= _bound(want, mag))  # a NaN is bad too
+    assert not bool(bad.any()), (int(bad.sum()), float((out - want).abs().max()))
+
+
+@pytest.mark.parametrize("above", [7.9, 7.9972, 7.998, 7.9999, 8.0, 8.1])
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_later_score_just_above_the_running_maximum(rows, dtype, above):
+    # the running maximum may lag by 8: weights near 2^8, blocks of one V scale.  The tiles of positions 0 and 128 go to
+    # one warp group, whatever the row tile, and one CTA takes the whole sequence.
+    P, n = 64, 160
+    for hd in (64, 128):
+        cache = _filled(1, 3, 1, P, hd, dtype, rows)
+        cache.codes.view(torch.uint8)[0, 0] = 0
+        cache.codes[0, 0, 2, 0, 0, 0] = 1
+        cache.scales[:] = 1.0
+        q = torch.zeros(1, rows * hd, dtype=torch.bfloat16, device=DEV)
+        q.view(rows, hd)[:, 0] = 1.0
+        table, scale = _i32([[0, 1, 2]]), above * math.log(2.0)
+        _check(_attend(cache, q, table, [n - 1], scale), *_attention64(cache, 0, q, table, [n - 1], [1], scale))

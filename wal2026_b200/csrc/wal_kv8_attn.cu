@@ -157,11 +157,18 @@ __device__ __forceinline__ void to_f16(const Masks& k, uint32_t w, uint32_t& p0,
   }
 }
 
-// V codes as bf16, divided by v_unit.
+// V codes as bf16: int8 as they are, e4m3 times 2^-120.  Weights take v_unit of
+// that back, which leaves them room for 2^kSlack and a rounding (the largest bf16
+// number is just below 2^128), and the finished outputs take v_rest.
 template <int KIND>
 __host__ __device__ constexpr float v_unit() {
-  return KIND == WAL_KV_INT8 ? 1.f : 1.329227995784916e36f;  // 2^120
+  return KIND == WAL_KV_INT8 ? 1.f : 5.192296858534828e33f;  // 2^112
 }
+template <int KIND>
+__host__ __device__ constexpr float v_rest() {
+  return KIND == WAL_KV_INT8 ? 1.f : 256.f;
+}
+static_assert(kSlack <= 8.f, "a weight of 2^kSlack * 2^112 stays far from the largest bf16 number");
 template <int KIND>
 __device__ __forceinline__ void to_bf16(const Masks& k, uint32_t w, uint32_t& p0, uint32_t& p1) {
   if (KIND == WAL_KV_INT8) {
@@ -537,10 +544,10 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     float* dst = po + (warp * RW + 8 * hh + 2 * q4) * LDO + r;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      dst[16 * i] = o[i][hh][0] * vref;
-      dst[16 * i + LDO] = o[i][hh][1] * vref;
-      dst[16 * i + 8] = o[i][hh][2] * vref;
-      dst[16 * i + 8 + LDO] = o[i][hh][3] * vref;
+      dst[16 * i] = o[i][hh][0] * v_rest<KIND>() * vref;
+      dst[16 * i + LDO] = o[i][hh][1] * v_rest<KIND>() * vref;
+      dst[16 * i + 8] = o[i][hh][2] * v_rest<KIND>() * vref;
+      dst[16 * i + 8 + LDO] = o[i][hh][3] * v_rest<KIND>() * vref;
     }
     if (r == 0) {
       wstat[warp][8 * hh + 2 * q4] = make_float2(m[hh][0], l[hh][0]);
