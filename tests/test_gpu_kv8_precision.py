@@ -1,4 +1,4 @@
-"""Weights of the 8-bit cache attention near their largest, for every row tile and both code types.
+"""Weights and precision of the 8-bit cache attention, for every row tile and both code types.
 
 Bounds, against the softmax in 64 bits over the cache's own values.  The output
 is rounded once to bf16: 2^-8 of the value.  A weight is the sum of two bf16
@@ -16,9 +16,9 @@ import math
 import pytest
 import torch
 
-from wal2026_b200.kv8 import kv8_attention, kv8_attention_workspace
+from wal2026_b200.kv8 import CODE_MAX, PagedKV8Cache, kv8_attention, kv8_attention_workspace
 
-from .test_gpu_kv8 import DEV, E4M3, INT8, _attention64, _filled, _i32
+from .test_gpu_kv8 import DEV, E4M3, INT8, _attention64, _filled, _gen, _i32, _tables
 
 pytestmark = pytest.mark.gpu
 ROWS = [8, 16, 24, 32, 48, 64, 96]  # query rows per kv head: one call of each row tile
@@ -56,3 +56,35 @@ def test_a_later_score_just_above_the_running_maximum(rows, dtype, above):
         q.view(rows, hd)[:, 0] = 1.0
         table, scale = _i32([[0, 1, 2]]), above * math.log(2.0)
         _check(_attend(cache, q, table, [n - 1], scale), *_attention64(cache, 0, q, table, [n - 1], [1], scale))
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("rows,T", [(r, 1) for r in ROWS] + [(20, 5), (36, 9), (130, 65)])
+def test_outputs_within_the_stated_precision(rows, T, dtype):
+    P, hd, lens = 32, 128, [0, 300, 77]
+    ends = [n + T for n in lens]
+    pages = sum(-(-n // P) for n in ends)
+    cache = _filled(1, pages, 2, P, hd, dtype, rows)
+    table = _tables(ends, P, pages, 2)
+    q = torch.randn(3 * T, 2 * (rows // T) * hd, device=DEV, generator=_gen(rows)).to(torch.bfloat16)
+    _check(_attend(cache, q, table, lens), *_attention64(cache, 0, q, table, lens, [T] * 3, hd ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("rows", ROWS)
+def test_both_parts_of_a_weight_count(rows, dtype):
+    # two positions of opposite values and nearly equal weights: what is left is what one bf16 weight would lose
+    P, hd = 16, 64
+    cache = PagedKV8Cache.allocate(1, 1, 1, hd, page_size=P, dtype=dtype, device=DEV)
+    top = CODE_MAX[dtype]
+    cache.codes[0, 0, 0, 0, 1, 0] = -1
+    cache.codes[0, 1, 0, 0, 0], cache.codes[0, 1, 0, 0, 1] = top, -top
+    cache.scales[:] = 1.0
+    q = torch.zeros(1, rows * hd, dtype=torch.bfloat16, device=DEV)
+    q.view(rows, hd)[:, 0] = torch.linspace(0.001, 0.08, rows, device=DEV)
+    table = _i32([[0]])
+    want, mag = _attention64(cache, 0, q, table, [1], [1], 1.0)
+    _check(_attend(cache, q, table, [1], 1.0), want, mag)
+    x = torch.exp(-q.double().view(rows, hd)[:, :1])  # weight of the second position over the first's
+    once = (top * (1 - x.to(torch.bfloat16).double()) / (1 + x)).expand(rows, hd).reshape(1, -1)
+    assert bool(((once - want).abs() > _bound(want, mag)).any())  # the bound would show a weight of one bf16 number
