@@ -63,6 +63,14 @@ class PagedDecoder:
     ``table`` int32 [rows, max_len / page_size] and ``lens`` int32 [rows] are the
     state; ``info`` after a step holds (pages left free, pages that were wanted
     but not given).
+
+    A step that is not given every page it wants (the pool or a row is full)
+    stores nothing and leaves ``table`` and ``lens`` as they were; its logits mean
+    nothing, and ``advance`` after it does nothing.  It can be repeated once
+    ``fork`` has emptied a row, or with ``new_lens`` 0 for the row that is full.
+    ``missing`` int64 [1] sums such pages over all steps, so that a loop which
+    never waits for the device can look now and then: 0 means that every step
+    was carried out.
     """
 
     def __init__(self, stack: LlamaStack, rows: int, max_len: int, *, num_pages: Optional[int] = None,
@@ -78,6 +86,8 @@ class PagedDecoder:
         self.table = torch.full((rows, width), -1, **i32)
         self.lens = torch.zeros(rows, **i32)
         self.info = torch.zeros(2, **i32)
+        self.missing = torch.zeros(1, dtype=torch.int64, device=dev)
+        self._room = torch.ones(1, dtype=torch.bool, device=dev)  # whether the last step got its pages
         self._next = torch.empty_like(self.table)
         self._self = torch.arange(rows, **i32)
         self._zero = torch.zeros(rows, **i32)
@@ -88,11 +98,18 @@ class PagedDecoder:
         self._bufs: dict[int, _StepBuffers] = {}
 
     def _assign(self, parent: Tensor, keep: Tensor, add: Tensor) -> None:
-        """The next table, copies made, in place of the present one."""
+        """The next table, in ``_next``, and the copies it asks for (into pages that no kept token is in)."""
         kv_pages_assign(self.table, parent, keep, add, self.cache.page_size, self._next, self._ref, self._src, self._dst,
                         self.info)
         kv_pages_copy(self.cache, self._src, self._dst)
-        self.table.copy_(self._next)
+
+    def _reserve(self, add: Tensor) -> Tensor:
+        """Room for add[row] more tokens each, or for none and everything as it was; the tokens that have room."""
+        self._assign(self._self, self.lens, add)
+        torch.eq(self.info[1:], 0, out=self._room)
+        torch.where(self._room, self._next, self.table, out=self.table)
+        self.missing.add_(self.info[1:])
+        return add * self._room
 
     @torch.no_grad()
     def step(self, tokens: Tensor, new_lens: Optional[Tensor] = None) -> Tensor:
@@ -100,8 +117,9 @@ class PagedDecoder:
 
         tokens: int [rows, T]; new_lens int32 [rows]: how many of them are real
         (logits of the others mean nothing).  Pages are reserved, and shared
-        ones copied, as needed.  The rows' lengths stay as they are: ``advance``
-        keeps the tokens, another ``step`` overwrites them.
+        ones copied, as needed; where they run out, nothing is stored (see the
+        class).  The rows' lengths stay as they are: ``advance`` keeps the tokens,
+        another ``step`` overwrites them.
         """
         B, T = tokens.shape
         if B != self.rows:
@@ -110,8 +128,7 @@ class PagedDecoder:
         bufs = self._bufs.get(T)
         if bufs is None:
             bufs = self._bufs[T] = _StepBuffers(st, B, T, self.cache)
-        add = torch.full_like(self.lens, T) if new_lens is None else new_lens
-        self._assign(self._self, self.lens, add)
+        add = self._reserve(torch.full_like(self.lens, T) if new_lens is None else new_lens)
         torch.index_select(st.embed, 0, tokens.reshape(-1), out=bufs.h)
         residual_rmsnorm(bufs.h, st.layers[0].in_norm, s.eps, bufs.x)
         n = len(st.layers)
@@ -137,11 +154,8 @@ class PagedDecoder:
             self.stack._row_parallel_fused(lin, a, 0, norm_w, bufs, "nccl")
 
     def advance(self, count: Optional[Tensor] = None) -> None:
-        """Keep the first count[row] tokens (int32 [rows]; None: one each) of the last step."""
-        if count is None:
-            self.lens.add_(1)
-        else:
-            self.lens.add_(count)
+        """Keep the first count[row] tokens (int32 [rows]; None: one each) of the last step, if it had room for them."""
+        self.lens.add_(self._room if count is None else count * self._room)
 
     @torch.no_grad()
     def speculate(self, drafts: Tensor, uniforms: Tensor, *, last: Tensor, draft_probs: Optional[Tensor] = None,
@@ -154,7 +168,8 @@ class PagedDecoder:
         keeps the drafts that are the most likely token.  Returns (accepted
         [rows], tokens [rows, T + 1]: the kept drafts, the drawn token, -1); the
         last token and the kept drafts stay in the cache, and the drawn token is
-        the next call's ``last``.
+        the next call's ``last``.  Where the step finds no room, accepted is 0 and
+        every token -1.
         """
         B, T = drafts.shape
         tokens = torch.cat([last.view(B, 1), drafts], dim=1)
@@ -167,6 +182,8 @@ class PagedDecoder:
         accepted = torch.empty(B, dtype=torch.int32, device=drafts.device)
         out = torch.empty(B, T + 1, dtype=torch.int32, device=drafts.device)
         verify_drafts(target, draft_probs, drafts, uniforms, accepted, out, draft_lens=draft_lens)
+        accepted.mul_(self._room)
+        out.masked_fill_(~self._room, -1)
         self.advance(accepted + 1)
         return accepted, out
 
@@ -178,7 +195,8 @@ class PagedDecoder:
         if any(not -1 <= int(i) < self.rows for i in parent):
             raise ValueError(f"parents must be rows 0 .. {self.rows - 1}, or -1")
         lens = torch.where(p >= 0, self.lens[p.clamp(min=0).long()], 0)
-        self._assign(p, lens, self._zero)
+        self._assign(p, lens, self._zero)  # wants no page
+        self.table.copy_(self._next)
         self.lens.copy_(lens)
 
     def compact(self) -> None:
