@@ -188,3 +188,26 @@ def test_refusals():
 def test_the_example_runs(capsys):
     main()
     assert "pages used" in capsys.readouterr().out
+
+
+def test_idle_rows_of_a_speculative_step():
+    # draft_lens -1: nothing stored, reserved or drawn; the other rows as if they were alone
+    stack = rvq_llama(SHAPE, seed=9)
+    prompt, lens = _tokens(3, 20), torch.tensor([20, 16, 0], dtype=torch.int32, device=DEV)
+    last, drafts = _tokens(3, 1, 2).int().view(3), _tokens(3, 3, 3).int()
+    u = torch.rand(3, 4, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4))
+    both = []
+    for idle in (True, False):
+        dec = PagedDecoder(stack, rows=3, max_len=64, page_size=16)
+        dec.step(prompt, lens)
+        dec.advance(lens)
+        dl = torch.tensor([3, -1 if idle else 0, -1 if idle else 2], dtype=torch.int32, device=DEV)
+        table = dec.table.clone()
+        accepted, out = dec.speculate(drafts, u, last=last, draft_lens=dl)
+        both.append((accepted, out))
+        if idle:
+            assert accepted.tolist()[1:] == [0, 0] and bool((out[1:] == -1).all())
+            assert dec.lens.tolist()[1:] == [16, 0] and torch.equal(dec.table[1:], table[1:])
+        else:
+            assert dec.lens.tolist()[1] == 17 and bool((out[1:, 0] >= 0).all())
+    assert torch.equal(both[0][0][0], both[1][0][0]) and torch.equal(both[0][1][0], both[1][1][0])

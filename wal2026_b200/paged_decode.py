@@ -164,12 +164,14 @@ class PagedDecoder:
 
         last: int32 [rows], each row's newest token (not stored yet); drafts:
         int32 [rows, T]; uniforms: fp32 [rows, T + 1]; draft_probs: fp32 [rows,
-        T, vocab] or None (drafts chosen without probabilities).  Temperature 0
+        T, vocab] or None (drafts chosen without probabilities); draft_lens int32
+        [rows]: how many drafts of a row are real, -1 for a row that takes no
+        part (accepted 0, every token -1, nothing stored).  Temperature 0
         keeps the drafts that are the most likely token.  Returns (accepted
         [rows], tokens [rows, T + 1]: the kept drafts, the drawn token, -1); the
         last token and the kept drafts stay in the cache, and the drawn token is
-        the next call's ``last``.  Where the step finds no room, accepted is 0 and
-        every token -1.
+        the next call's ``last``.  A step that finds no room is one in which no
+        row takes part.
         """
         B, T = drafts.shape
         tokens = torch.cat([last.view(B, 1), drafts], dim=1)
@@ -182,9 +184,10 @@ class PagedDecoder:
         accepted = torch.empty(B, dtype=torch.int32, device=drafts.device)
         out = torch.empty(B, T + 1, dtype=torch.int32, device=drafts.device)
         verify_drafts(target, draft_probs, drafts, uniforms, accepted, out, draft_lens=draft_lens)
-        accepted.mul_(self._room)
-        out.masked_fill_(~self._room, -1)
-        self.advance(accepted + 1)
+        part = self._room if draft_lens is None else self._room & (draft_lens >= 0)
+        accepted.mul_(part)
+        out.masked_fill_(~part[:, None], -1)
+        self.advance(accepted + part)
         return accepted, out
 
     def fork(self, parent: Sequence[int]) -> None:
