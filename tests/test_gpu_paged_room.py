@@ -107,3 +107,17 @@ def test_a_graph_stops_at_the_end_of_the_pool(stack):
         g.replay()
     assert dec.lens.tolist() == [32] and int(dec.missing) == 4
     assert sorted(dec.table.tolist()[0]) == [-1, -1, 0, 1]
+
+
+def test_the_last_page_of_a_row_is_whole(stack):
+    # max_len inside a page: positions to the page's end have a place, so they have their rotation too
+    tokens, news = _tokens(1, 30), _i32(30)
+    short, long = (PagedDecoder(stack, rows=1, max_len=n, page_size=16) for n in (20, 64))
+    got, want = (dec.step(tokens) for dec in (short, long))
+    assert torch.equal(got, want)
+    for dec in (short, long):
+        dec.advance(news)
+    fed = _tokens(1, 2, 6)
+    assert torch.equal(short.step(fed), long.step(fed)) and short.info.tolist()[1] == 0
+    short.step(_tokens(1, 3, 6))  # past the page: no room
+    assert short.info.tolist()[1] == 1

@@ -58,7 +58,8 @@ def _column(lin, x: Tensor, y: Tensor) -> None:
 class PagedDecoder:
     """Sequences of a ``LlamaStack`` over one paged 8-bit cache.
 
-    rows: sequences decoded together; max_len: most positions of one sequence;
+    rows: sequences decoded together; max_len: most positions of one sequence,
+    rounded up to whole pages;
     num_pages: the pool they share (default: room for every row at max_len).
     ``table`` int32 [rows, max_len / page_size] and ``lens`` int32 [rows] are the
     state; ``info`` after a step holds (pages left free, pages that were wanted
@@ -79,7 +80,7 @@ class PagedDecoder:
             raise ValueError("rows and max_len must be positive")
         dev, l0 = stack.embed.device, stack.layers[0]
         width = -(-max_len // page_size)
-        self.stack, self.rows, self.max_len = stack, rows, max_len
+        self.stack, self.rows, self.max_len = stack, rows, width * page_size
         self.cache = PagedKV8Cache.allocate(len(stack.layers), num_pages or rows * width, l0.hkv, stack.shape.head_dim,
                                             page_size=page_size, dtype=dtype, device=dev)
         i32 = dict(dtype=torch.int32, device=dev)
@@ -93,7 +94,7 @@ class PagedDecoder:
         self._zero = torch.zeros(rows, **i32)
         self._ref = torch.empty(self.cache.num_pages, **i32)
         self._src, self._dst = torch.empty(rows, **i32), torch.empty(rows, **i32)
-        ang = torch.arange(max_len, device=dev, dtype=torch.float32)[:, None] * stack.inv_freq
+        ang = torch.arange(self.max_len, device=dev, dtype=torch.float32)[:, None] * stack.inv_freq
         self.cos, self.sin = ang.cos().contiguous(), ang.sin().contiguous()
         self._bufs: dict[int, _StepBuffers] = {}
 
