@@ -121,3 +121,53 @@ def test_the_last_page_of_a_row_is_whole(stack):
     assert torch.equal(short.step(fed), long.step(fed)) and short.info.tolist()[1] == 0
     short.step(_tokens(1, 3, 6))  # past the page: no room
     assert short.info.tolist()[1] == 1
+
+
+def test_steps_of_many_sizes_hold_one_set_of_buffers(stack):
+    def held(sizes):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        dec = PagedDecoder(stack, rows=2, max_len=64, page_size=16)
+        logits = [dec.step(_tokens(2, n)) for n in sizes]
+        last = logits[-1].clone()
+        del logits
+        return torch.cuda.memory_allocated() - before, last, dec
+
+    held([64])  # what a first call keeps for good
+    one, want, _ = held([64])
+    many, got, dec = held([*range(1, 65), 3, 64])
+    assert many <= one + (1 << 16) and torch.equal(got, want)
+    small, ref, _ = held([3])
+    assert torch.equal(dec.step(_tokens(2, 3)), ref)
+    with pytest.raises(ValueError, match="at least one token"):
+        dec.step(_tokens(2, 1)[:, :0])
+
+
+def test_a_captured_step_keeps_its_buffers(stack):
+    tokens = _tokens(1, 12)
+    fed = tokens[:, :1].clone()
+    dec, eager = (PagedDecoder(stack, rows=1, max_len=64, page_size=16) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        dec.step(fed)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        logits = dec.step(fed)
+        dec.advance()
+    first, other = torch.cuda.CUDAGraph(), _tokens(1, 3, 5)
+    with torch.cuda.graph(first):  # a size that was not run before
+        wide = dec.step(other)
+    for pos in range(12):
+        if pos == 3:  # a larger step, and others who would take memory that it gave back
+            assert torch.equal(dec.step(_tokens(1, 40, 9)), eager.step(_tokens(1, 40, 9)))
+            junk = [torch.full((1 << k,), float("nan"), device=DEV) for k in range(8, 22)]
+        if pos == 6:
+            first.replay()
+            assert torch.equal(wide, eager.step(other))
+        fed.copy_(tokens[:, pos:pos + 1])
+        g.replay()
+        assert torch.equal(logits, eager.step(fed)), pos
+        eager.advance()
+    del junk

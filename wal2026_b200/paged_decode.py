@@ -32,11 +32,12 @@ from .speculative import verify_drafts
 
 
 class _StepBuffers:
-    """Activations of a step of M token rows."""
+    """Activations of steps of up to ``tokens`` tokens per row, and the attention's workspace."""
 
     def __init__(self, stack: LlamaStack, rows: int, tokens: int, cache: PagedKV8Cache):
         s, l0, dev, bf = stack.shape, stack.layers[0], stack.embed.device, torch.bfloat16
         M, hd = rows * tokens, s.head_dim
+        self.tokens = tokens
         self.h = torch.empty(M, s.hidden, device=dev, dtype=bf)
         self.x = torch.empty(M, s.hidden, device=dev, dtype=bf)
         self.qkv = torch.empty(M, (l0.hq + 2 * l0.hkv) * hd, device=dev, dtype=bf)
@@ -46,6 +47,14 @@ class _StepBuffers:
         self.act = torch.empty(M, l0.mlp, device=dev, dtype=bf)
         self.y32 = torch.empty(M, s.hidden, device=dev, dtype=torch.float32)
         self.ws = kv8_attention_workspace(cache, rows, l0.hq, tokens)
+
+    def first(self, M: int) -> "_StepBuffers":
+        """The same buffers for a step of M token rows."""
+        view = object.__new__(_StepBuffers)
+        view.tokens, view.ws = self.tokens, self.ws
+        for name in ("h", "x", "qkv", "q", "attn", "gu", "act", "y32"):
+            setattr(view, name, getattr(self, name)[:M])
+        return view
 
 
 def _column(lin, x: Tensor, y: Tensor) -> None:
@@ -96,7 +105,33 @@ class PagedDecoder:
         self._src, self._dst = torch.empty(rows, **i32), torch.empty(rows, **i32)
         ang = torch.arange(self.max_len, device=dev, dtype=torch.float32)[:, None] * stack.inv_freq
         self.cos, self.sin = ang.cos().contiguous(), ang.sin().contiguous()
-        self._bufs: dict[int, _StepBuffers] = {}
+        self._bufs: Optional[_StepBuffers] = None  # of the largest step so far
+        self._views: dict[int, _StepBuffers] = {}  # its first rows, by step size
+        self._captured: list[_StepBuffers] = []    # sets that a graph uses
+
+    def _buffers(self, T: int) -> _StepBuffers:
+        """Buffers of a step of T tokens per row: one set serves all sizes and grows with the largest.
+
+        A set that a graph captured stays when a larger one replaces it, and a
+        graph that captures a larger step than any before gets one of its own.
+        """
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self._bufs is None or self._bufs.tokens < T:
+            if capturing:
+                self._captured.append(_StepBuffers(self.stack, self.rows, T, self.cache))
+                return self._captured[-1]
+            if self._bufs is not None:
+                for t in vars(self._bufs).values():
+                    if isinstance(t, Tensor):
+                        t.record_stream(torch.cuda.current_stream(t.device))
+            self._bufs, self._views = None, {}
+            self._bufs = _StepBuffers(self.stack, self.rows, T, self.cache)
+        if capturing and not any(b is self._bufs for b in self._captured):
+            self._captured.append(self._bufs)
+        view = self._views.get(T)
+        if view is None:
+            view = self._views[T] = self._bufs.first(self.rows * T)
+        return view
 
     def _assign(self, parent: Tensor, keep: Tensor, add: Tensor) -> None:
         """The next table, in ``_next``, and the copies it asks for (into pages that no kept token is in)."""
@@ -125,10 +160,10 @@ class PagedDecoder:
         B, T = tokens.shape
         if B != self.rows:
             raise ValueError(f"tokens must have {self.rows} rows, got {B}")
+        if T == 0:
+            raise ValueError("a step takes at least one token per row")
         st, s = self.stack, self.stack.shape
-        bufs = self._bufs.get(T)
-        if bufs is None:
-            bufs = self._bufs[T] = _StepBuffers(st, B, T, self.cache)
+        bufs = self._buffers(T)
         add = self._reserve(torch.full_like(self.lens, T) if new_lens is None else new_lens)
         torch.index_select(st.embed, 0, tokens.reshape(-1), out=bufs.h)
         residual_rmsnorm(bufs.h, st.layers[0].in_norm, s.eps, bufs.x)
