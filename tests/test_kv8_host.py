@@ -191,3 +191,27 @@ def test_shapes_and_types_are_checked_before_the_device():
         verify_drafts(_z(2, 2, 9, dtype=f), _z(2, 2, 9, dtype=f), _z(2, 1), _z(2, 2, dtype=f), ln, _z(2, 2))
     with pytest.raises(ValueError, match="tokens"):
         verify_drafts(_z(2, 2, 9, dtype=f), None, _z(2, 1), _z(2, 2, dtype=f), ln, _z(2, 1))
+
+
+def test_nothing_is_launched_where_the_arguments_do_not_fit(monkeypatch):
+    # arguments that the fast checks refuse are refused, whether or not the search for the reason finds one
+    import wal2026_b200.kv8 as kv8
+    import wal2026_b200.speculative as speculative
+
+    launched = []
+    for module in (kv8, speculative):
+        monkeypatch.setattr(module, "_cuda", lambda device: None)  # CPU tensors: the fast checks fail, no reason is found
+        monkeypatch.setattr(module, "_call", lambda *a: launched.append(a))
+    c, bf, f = _cache(), torch.bfloat16, torch.float32
+    tab, ln, out = _z(2, 3), _z(2), _z(2, 3)
+    calls = [lambda: kv8_append(c, 0, _z(2, 512, dtype=bf), 4, tab, ln, _z(2, 256, dtype=bf)),
+             lambda: kv8_read(c, 0, tab, ln, ln, _z(2, 2, 5, 64, dtype=bf), _z(2, 2, 5, 64, dtype=bf)),
+             lambda: kv8_attention(c, 0, _z(2, 256, dtype=bf), tab, ln, _z(2, 256, dtype=bf), _z(256, dtype=torch.uint8)),
+             lambda: kv_pages_assign(tab, ln, ln, ln, 16, out, _z(4), ln, ln, ln),
+             lambda: kv_pages_compact(tab, ln, 16, out, _z(4), _z(4), _z(4), _z(2)),
+             lambda: kv_pages_copy(c, ln, ln),
+             lambda: verify_drafts(_z(2, 2, 9, dtype=f), None, _z(2, 1), _z(2, 2, dtype=f), ln, _z(2, 2))]
+    for call in calls:
+        with pytest.raises(ValueError, match="do not fit together"):
+            call()
+    assert not launched

@@ -208,6 +208,7 @@ def _why_not_read(cache, table, first, count, k_out, v_out) -> None:
         if tuple(t.shape) != (B, cache.kv_heads, L, cache.head_dim) or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous [{B}, {cache.kv_heads}, L, {cache.head_dim}]")
     _on(cache.device, table=table, first=first, count=count, k_out=k_out, v_out=v_out)
+    raise ValueError("kv8_read: arguments do not fit together")
 
 
 def kv8_read(cache: PagedKV8Cache, layer: int, table: Tensor, first: Tensor, count: Tensor, k_out: Tensor,
@@ -283,6 +284,7 @@ def _why_not_assign(table, parent, keep, add, table_out, ref_out, copy_src, copy
     _cuda(table.device)
     _on(table.device, parent=parent, keep=keep, add=add, table_out=table_out, ref_out=ref_out, copy_src=copy_src,
         copy_dst=copy_dst, info=info)
+    raise ValueError("kv_pages_assign: arguments do not fit together")
 
 
 def kv_pages_assign(table: Tensor, parent: Tensor, keep: Tensor, add: Tensor, page_size: int, table_out: Tensor,
@@ -322,6 +324,7 @@ def _why_not_compact(table, lens, table_out, remap, move_src, move_dst, info) ->
     _i32("info", info, 2)
     _cuda(table.device)
     _on(table.device, lens=lens, table_out=table_out, remap=remap, move_src=move_src, move_dst=move_dst, info=info)
+    raise ValueError("kv_pages_compact: arguments do not fit together")
 
 
 def kv_pages_compact(table: Tensor, lens: Tensor, page_size: int, table_out: Tensor, remap: Tensor, move_src: Tensor,
@@ -348,6 +351,7 @@ def _why_not_copy(cache, src, dst) -> None:
     _i32("src", src, src.numel())
     _i32("dst", dst, src.numel())
     _on(cache.device, src=src, dst=dst)
+    raise ValueError("kv_pages_copy: arguments do not fit together")
 
 
 def kv_pages_copy(cache: PagedKV8Cache, src: Tensor, dst: Tensor) -> None:

@@ -15,7 +15,7 @@ def _row_stride(t: Tensor) -> int:
     return t.stride()[1] if t.shape[1] > 1 else t.shape[2]
 
 
-def _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens) -> tuple[int, int, int]:
+def _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens) -> None:
     dev = target.device
     if target.dtype != torch.float32 or target.dim() != 3 or target.stride(2) != 1 or target.shape[1] < 1:
         raise ValueError("target must be fp32 [B, T + 1, V] with contiguous rows")
@@ -31,7 +31,7 @@ def _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens) -> t
         _i32("draft_lens", draft_lens, B)
     _cuda(dev)
     _on(dev, draft=draft, drafts=drafts, uniforms=uniforms, accepted=accepted, tokens=tokens, draft_lens=draft_lens)
-    return B, T, V
+    raise ValueError("verify_drafts: arguments do not fit together")
 
 
 def verify_drafts(target: Tensor, draft: Optional[Tensor], drafts: Tensor, uniforms: Tensor, accepted: Tensor,
@@ -59,7 +59,7 @@ def verify_drafts(target: Tensor, draft: Optional[Tensor], drafts: Tensor, unifo
                and uniforms.shape == (B, T + 1) and uniforms.dtype is torch.float32 and uniforms.is_contiguous()
                and uniforms.get_device() == index and (draft_lens is None or _is_i32(draft_lens, (B,), index)))
     if not fit:
-        B, T, V = _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens)
+        _why_not(target, draft, drafts, uniforms, accepted, tokens, draft_lens)
     if T == 0:
         draft = None
     d0, d1 = (0, V) if draft is None else (draft.stride()[0], _row_stride(draft))
