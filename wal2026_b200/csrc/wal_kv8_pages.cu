@@ -433,6 +433,24 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) kv_pages_copy_ke
   }
 }
 
+// Dynamic shared memory of the assign kernel.
+constexpr int assign_smem(int rows) { return (3 * rows + 1 + (rows + 31) / 32) * (int)sizeof(int); }
+constexpr int kPlainSmem = 40 * 1024;  // a kernel may use this much without leave
+
+// Lets the assign kernel use the shared memory of as many rows as it takes, once per
+// device: an allowance that followed each call would be lowered by one thread between
+// another's setting and launch.
+bool allow_large_assign() {
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+  if (allowed.load(std::memory_order_relaxed) >> dev & 1) return true;
+  if (cudaFuncSetAttribute(kv_pages_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, assign_smem(kMaxRows)) != cudaSuccess)
+    return false;
+  allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return true;
+}
+
 // CTAs of a table kernel's cluster, with the copy's time: one where each thread has
 // at most one entry or page (36 pages of 6 sequences: 10.3 us with one or eight),
 // eight for more (64 rows forked over 380 pages: 26.8 us with one, 25.2 with eight),
@@ -485,9 +503,8 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   AssignParams p = {table, ld_table, (int)rows_in, parent, keep, add, (int)rows, (int)width, (int)num_pages, page_size,
                     table_out, ld_out, reinterpret_cast<unsigned*>(ref_out), copy_src, copy_dst, info};
-  const int smem = (3 * (int)rows + 1 + ((int)rows + 31) / 32) * (int)sizeof(int);
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kv_pages_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return WAL_ERR_CUDA;
+  const int smem = assign_smem((int)rows);
+  if (smem > kPlainSmem && !allow_large_assign()) return WAL_ERR_CUDA;
   const int cluster = table_cluster(kv_pages_assign_kernel, rows * width, num_pages);
   return launch_chain(kv_pages_assign_kernel, dim3((unsigned)cluster), kThreads, smem, static_cast<cudaStream_t>(stream), p, cluster);
 }
