@@ -457,19 +457,23 @@ bool allow_large_assign() {
 // and sixteen, where the device schedules clusters beyond the portable eight, when
 // the entries' atomics and stores outweigh the barriers (256 sequences with 65 k
 // entries: 24.8 us with eight, 16.5 with sixteen; 2055 pages with 1200 entries: 62 us either way).
+// Whether sixteen fit is asked with as much shared memory as such calls use at most, apart
+// for those that need leave for it: with it a CTA has an SM to itself.
 template <typename Kern>
-int table_cluster(Kern kern, int64_t entries, int64_t pages) {
+int table_cluster(Kern kern, int64_t entries, int64_t pages, int smem) {
   if (entries + pages <= kThreads) return 1;
   if (entries + pages <= 16 * kThreads) return 8;
-  static std::atomic<int> known[kMaxDevices];  // 1: eight, 2: sixteen
+  static std::atomic<int> known[2][kMaxDevices];  // 1: eight, 2: sixteen
+  const bool large = smem > kPlainSmem;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 8;
-  int can = known[dev].load(std::memory_order_relaxed);
+  int can = known[large][dev].load(std::memory_order_relaxed);
   if (can == 0) {
     can = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kCluster);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)(large ? assign_smem(kMaxRows) : kPlainSmem);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kCluster;
@@ -482,7 +486,7 @@ int table_cluster(Kern kern, int64_t entries, int64_t pages) {
         cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
       can = 2;
     (void)cudaGetLastError();  // a refusal is an answer
-    known[dev].store(can, std::memory_order_relaxed);
+    known[large][dev].store(can, std::memory_order_relaxed);
   }
   return can == 2 ? kCluster : 8;
 }
@@ -505,7 +509,7 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
                     table_out, ld_out, reinterpret_cast<unsigned*>(ref_out), copy_src, copy_dst, info};
   const int smem = assign_smem((int)rows);
   if (smem > kPlainSmem && !allow_large_assign()) return WAL_ERR_CUDA;
-  const int cluster = table_cluster(kv_pages_assign_kernel, rows * width, num_pages);
+  const int cluster = table_cluster(kv_pages_assign_kernel, rows * width, num_pages, smem);
   return launch_chain(kv_pages_assign_kernel, dim3((unsigned)cluster), kThreads, smem, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
@@ -518,7 +522,7 @@ int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* 
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   CompactParams p = {table, ld_table, lens, (int)rows, (int)width, (int)num_pages, page_size, table_out, ld_out, remap,
                      move_src, move_dst, info};
-  const int cluster = table_cluster(kv_pages_compact_kernel, rows * width, num_pages);
+  const int cluster = table_cluster(kv_pages_compact_kernel, rows * width, num_pages, 0);
   return launch_chain(kv_pages_compact_kernel, dim3((unsigned)cluster), kThreads, 0, static_cast<cudaStream_t>(stream), p, cluster);
 }
 
