@@ -579,7 +579,7 @@ WAL_API int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const u
  *   table_out [rows][width], -1 past a row's pages; ref_out [num_pages]
  *   references after the call; copy_src / copy_dst [rows], -1 where none;
  *   info[0] pages left free, info[1] pages that were wanted but not given (the
- *   pool or the row's width was exhausted; their entries are -1).
+ *   pool or the row's width was exhausted; their entries are -1), at most 2^31 - 1.
  * The old table stays as it is and must not overlap the new one, so a caller
  * who finds info[1] > 0 can make room and call again.  rows <= 16383; a row
  * names a page at most once.

@@ -41,3 +41,15 @@ def test_assign_from_threads_with_different_row_counts():
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("rows,add", [(16, 2 ** 31 - 1), (32, 2 ** 31 - 1), (3, 2 ** 31 - 1), (40, 1 << 20)])
+def test_assign_counts_shortages_past_32_bits(rows, add):
+    # the pages that rows ask for beyond their width, summed: 2^27 each, kept within an int32
+    P, width, pages = 16, 2, 5
+    table = torch.full((1, width), -1, dtype=torch.int32, device=DEV)
+    out, ref = torch.empty(rows, width, dtype=torch.int32, device=DEV), torch.empty(pages, dtype=torch.int32, device=DEV)
+    src, dst, info = (torch.empty(n, dtype=torch.int32, device=DEV) for n in (rows, rows, 2))
+    kv_pages_assign(table, _i32([-1] * rows), _i32([0] * rows), _i32([add] * rows), P, out, ref, src, dst, info)
+    want = rows * -(-add // P) - pages
+    assert info.tolist() == [0, min(want, 2 ** 31 - 1)]

@@ -122,7 +122,7 @@ __device__ __forceinline__ Row load_row(const AssignParams& p, int b) {
 __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_constant__ AssignParams p) {
   extern __shared__ int begin[];  // [rows + 1] first wanted page of each row, [rows] kept pages, [rows] parents, bits of rows that copy
   __shared__ int scan[kWarps], box[kCluster];
-  __shared__ int lost;
+  __shared__ unsigned long long lost;  // pages beyond the rows' width: up to 2^31 each
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
   if (tid < p.rows) {
     if (first.writes) last_page = valid_page(__ldg(p.table + (long long)first.parent * p.ld_table + first.have - 1), p.pages);
   }
-  if (tid == 0) lost = 0;
+  if (tid == 0) lost = 0ull;
   for (int i = gtid; i < p.pages; i += gthreads) p.ref[i] = 0u;
   for (int i = tid; i < (p.rows + 31) / 32; i += kThreads) copies[i] = 0u;
   cl.sync();
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
       const Row r = b0 == 0 ? first : load_row(p, b);
       n = (int)(copies[b >> 5] >> (b & 31) & 1u) + r.want - r.have;
       const long long over = ((long long)r.keep + r.add + p.P - 1) / p.P - r.want;
-      if (r.add && over > 0) atomicAdd(&lost, (int)min(over, 0x3fffffffLL));
+      if (r.add && over > 0) atomicAdd(&lost, (unsigned long long)over);
     }
     const int at = block_scan(n, scan, &total);
     if (b < p.rows) begin[b] = base + at;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
   }
   if (rank == 0 && tid == 0) {
     p.info[0] = max(found - base, 0);
-    p.info[1] = lost + max(base - found, 0);
+    p.info[1] = (int)min(lost + (unsigned long long)max(base - found, 0), 0x7fffffffull);
   }
 }
 
