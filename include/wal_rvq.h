@@ -581,8 +581,9 @@ WAL_API int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const u
  *   info[0] pages left free, info[1] pages that were wanted but not given (the
  *   pool or the row's width was exhausted; their entries are -1), at most 2^31 - 1.
  * The old table stays as it is and must not overlap the new one, so a caller
- * who finds info[1] > 0 can make room and call again.  rows <= 16383; a row
- * names a page at most once.
+ * who finds info[1] > 0 can make room and call again.  rows <= 16383, width and
+ * num_pages <= 2^30, rows x width < 2^31, (width + 1) x page_size <= 2^31; a row names a
+ * page at most once.
  */
 WAL_API int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in, const int32_t* parent,
                         const int32_t* keep, const int32_t* add, int64_t rows, int64_t width,

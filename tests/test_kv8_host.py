@@ -215,3 +215,18 @@ def test_nothing_is_launched_where_the_arguments_do_not_fit(monkeypatch):
         with pytest.raises(ValueError, match="do not fit together"):
             call()
     assert not launched
+
+
+def test_sizes_whose_indexes_would_pass_32_bits_are_refused():
+    big = 1 << 30
+    for name, args in (("wal_kv_pages_assign", ASSIGN), ("wal_kv_pages_compact", COMPACT)):
+        wide = dict(ld_table=1 << 31, ld_out=1 << 31)
+        assert _call(name, args, num_pages=big + 1) == SHAPE            # strided loops over the pages
+        assert _call(name, args, width=big + 1, page_size=1, **wide) == SHAPE  # chunks of 512 entries
+        assert _call(name, args, width=715827882, page_size=3, **wide) == SHAPE  # tokens rounded up to pages
+        assert _call(name, args, width=1, page_size=big + 2) == SHAPE
+    # wanted pages of all rows together
+    assert _call("wal_kv_pages_assign", ASSIGN, rows=16, width=1 << 27, page_size=8, ld_table=1 << 27, ld_out=1 << 27) == SHAPE
+    # the end of an attention tile
+    for pages in ((1 << 27) - 1, (1 << 27) - 2):
+        assert _call("wal_kv8_attention", ATTN, cache=_c(), max_pages=pages, ld_table=1 << 27) == SHAPE

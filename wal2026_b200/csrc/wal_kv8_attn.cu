@@ -822,7 +822,7 @@ int wal_kv8_attention(const wal_kv8_cache* cache, int32_t layer, const uint16_t*
   if (!q || !table || !lens || !out || !workspace) return WAL_ERR_INVALID_ARGUMENT;
   if (B <= 0 || T <= 0 || hq <= 0 || hq % cache->kv_heads || max_pages <= 0 || ld_table < max_pages) return WAL_ERR_SHAPE;
   const int hd = cache->head_dim;
-  if (B > 0x7fffffff || T > 0x7fffffff || max_pages > 0x7fffffff / cache->page_size || B * T > 0x7fffffff / hq) return WAL_ERR_SHAPE;
+  if (B > 0x7fffffff || T > 0x7fffffff || max_pages > (0x7fffffff - kTile) / cache->page_size || B * T > 0x7fffffff / hq) return WAL_ERR_SHAPE;
   if (ld_q < (int64_t)hq * hd || ld_out < (int64_t)hq * hd) return WAL_ERR_SHAPE;
   if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 255) || (ld_q % 8) || (ld_out % 8)) return WAL_ERR_ALIGNMENT;
   if (workspace_bytes < wal_kv8_attention_workspace(cache, B, T, hq)) return WAL_ERR_BUFFER_TOO_SMALL;

@@ -491,6 +491,14 @@ int table_cluster(Kern kern, int64_t entries, int64_t pages, int smem) {
   return can == 2 ? kCluster : 8;
 }
 
+// Sizes whose indexes stay within 32 bits in the table kernels: strided loops over
+// pages and chunks of entries run past their end by less than 2^30, and a row's
+// tokens rounded up to pages are width * page_size + page_size - 1 at most.
+bool table_fits(int64_t width, int64_t num_pages, int64_t page_size) {
+  constexpr int64_t kMost = 1 << 30;
+  return width <= kMost && num_pages <= kMost && width <= ((1LL << 31) - page_size) / page_size;
+}
+
 }  // namespace
 
 extern "C" {
@@ -502,8 +510,8 @@ int wal_kv_pages_assign(const int32_t* table, int64_t ld_table, int64_t rows_in,
   if (!table || !parent || !keep || !add || !table_out || !ref_out || !copy_src || !copy_dst || !info)
     return WAL_ERR_INVALID_ARGUMENT;
   if (rows_in <= 0 || rows <= 0 || width <= 0 || num_pages <= 0 || page_size <= 0) return WAL_ERR_SHAPE;
-  if (rows > kMaxRows || rows_in > 0x7fffffff || num_pages > 0x7fffffff - kThreads || width > 0x7fffffff / page_size)
-    return WAL_ERR_SHAPE;
+  if (rows > kMaxRows || rows_in > 0x7fffffff || !table_fits(width, num_pages, page_size)) return WAL_ERR_SHAPE;
+  if (rows > 0x7fffffff / width) return WAL_ERR_SHAPE;  // wanted pages of all rows
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   AssignParams p = {table, ld_table, (int)rows_in, parent, keep, add, (int)rows, (int)width, (int)num_pages, page_size,
                     table_out, ld_out, reinterpret_cast<unsigned*>(ref_out), copy_src, copy_dst, info};
@@ -518,7 +526,7 @@ int wal_kv_pages_compact(const int32_t* table, int64_t ld_table, const int32_t* 
                          int32_t* move_src, int32_t* move_dst, int32_t* info, void* stream) {
   if (!table || !lens || !table_out || !remap || !move_src || !move_dst || !info) return WAL_ERR_INVALID_ARGUMENT;
   if (rows <= 0 || width <= 0 || num_pages <= 0 || page_size <= 0) return WAL_ERR_SHAPE;
-  if (rows > 0x7fffffff - kThreads || num_pages > 0x7fffffff - kThreads || width > 0x7fffffff / page_size) return WAL_ERR_SHAPE;
+  if (rows > 0x7fffffff || !table_fits(width, num_pages, page_size)) return WAL_ERR_SHAPE;
   if (ld_table < width || ld_out < width) return WAL_ERR_SHAPE;
   CompactParams p = {table, ld_table, lens, (int)rows, (int)width, (int)num_pages, page_size, table_out, ld_out, remap,
                      move_src, move_dst, info};
