@@ -528,7 +528,9 @@ typedef struct wal_kv8_cache {
  * earlier positions of the sequence, else 0; the scale becomes s = max(s0, a
  * times the fp32 number next to 1 / Q) and a new code is round-to-nearest-even of x / s clamped to [-Q, Q] (an
  * infinity saturates, a NaN and every value of a block with s = 0 becomes 0);
- * where s > s0 the earlier codes c become the codes of c * (s0 / s).  Tokens
+ * where s > s0 the earlier codes c become the codes of c * (s0 / s).  This holds
+ * for tokens that a later call overwrites too: a large draft that is not kept
+ * leaves the block its scale and the earlier codes their coarser rounding.  Tokens
  * whose position has no page, or is max_pos or more, are not stored (past
  * max_pos q_out is zeros too).  Pages written here must belong to one sequence alone (wal_kv_pages_assign).
  * qkv, q_out, cos, sin 16-byte aligned; ld_qkv, ld_q multiples of 8.

@@ -1,4 +1,4 @@
-"""Weights and precision of the 8-bit cache attention, for every row tile and both code types.
+"""Precision of the 8-bit cache: weights of the attention for every row tile and code type, and what a rejected token leaves.
 
 Bounds, against the softmax in 64 bits over the cache's own values.  The output
 is rounded once to bf16: 2^-8 of the value.  A weight is the sum of two bf16
@@ -16,7 +16,8 @@ import math
 import pytest
 import torch
 
-from wal2026_b200.kv8 import CODE_MAX, PagedKV8Cache, kv8_attention, kv8_attention_workspace
+from wal2026_b200.kv8 import (CODE_MAX, PagedKV8Cache, kv8_append, kv8_attention, kv8_attention_workspace,
+                              kv8_read)
 
 from .test_gpu_kv8 import DEV, E4M3, INT8, _attention64, _filled, _gen, _i32, _tables
 
@@ -88,3 +89,36 @@ def test_both_parts_of_a_weight_count(rows, dtype):
     x = torch.exp(-q.double().view(rows, hd)[:, :1])  # weight of the second position over the first's
     once = (top * (1 - x.to(torch.bfloat16).double()) / (1 + x)).expand(rows, hd).reshape(1, -1)
     assert bool(((once - want).abs() > _bound(want, mag)).any())  # the bound would show a weight of one bf16 number
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_a_rejected_token_leaves_its_scale(dtype):
+    # a large draft re-rounds the earlier codes of its block once, and later tokens keep its scale; a block that the
+    # draft itself began is begun anew
+    P, hd, top = 16, 64, CODE_MAX[dtype]
+    cache = PagedKV8Cache.allocate(1, 2, 1, hd, page_size=P, dtype=dtype, device=DEV)
+    rows = torch.randn(12, 3 * hd, device=DEV, generator=_gen(4)).to(torch.bfloat16)
+    big, table, q = rows[10:11] * 50, _i32([[1, 0]]), torch.empty(12, hd, dtype=torch.bfloat16, device=DEV)
+
+    def append(x, n):
+        kv8_append(cache, 0, x, 1, table, _i32([n]), q[:x.shape[0]])
+
+    def read(n):
+        k, v = (torch.empty(1, 1, n, hd, device=DEV) for _ in range(2))
+        kv8_read(cache, 0, table, _i32([0]), _i32([n]), k, v)
+        return torch.stack([k, v]).double()
+
+    append(rows[:10], 0)
+    before = read(10)
+    append(big, 10)
+    scale = cache.scales[0, :, 1, 0].clone()
+    assert torch.equal(scale, big.float().view(3, hd)[1:].abs().amax(1) * (torch.ones((), device=DEV) / top))
+    after, s = read(10), scale.double().view(2, 1, 1, 1, 1)
+    step = s if dtype == INT8 else (before.abs() * 2.0 ** -3).clamp(min=2.0 ** -9 * s)  # between codes
+    assert bool(((after - before).abs() <= 0.5 * step + 1e-6 * before.abs()).all())
+    append(rows[11:], 10)  # in the draft's place
+    assert torch.equal(cache.scales[0, :, 1, 0], scale) and torch.equal(read(10).float(), after.float())
+    append(rows[:6], 10)   # up to the block's end
+    append(big, 16)        # begins the next block
+    append(rows[11:], 16)
+    assert torch.equal(cache.scales[0, :, 0, 0], rows[11].float().view(3, hd)[1:].abs().amax(1) * (torch.ones((), device=DEV) / top))

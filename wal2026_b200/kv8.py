@@ -178,7 +178,9 @@ def kv8_append(cache: PagedKV8Cache, layer: int, qkv: Tensor, hq: int, table: Te
     lens[b] + t; q_out: bf16 [B * T, hq * head_dim]; cos / sin: fp32 [max_pos,
     head_dim / 2] (rotate-half pairs), or neither.  Rows t >= new_lens[b] are
     padding.  A block's scale grows with its largest value, and its earlier
-    codes are re-rounded when it does.
+    codes are re-rounded when it does.  A token that a later call overwrites (a
+    draft that was not kept) leaves the scale where it raised it: earlier values
+    then carry the coarser rounding.
     """
     hd, max_pos = cache.head_dim, 0
     step = _step(cache, qkv, (hq + 2 * cache.kv_heads) * hd, q_out, hq, table, lens, new_lens)
