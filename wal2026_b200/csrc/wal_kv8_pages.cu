@@ -237,34 +237,34 @@ __global__ void __launch_bounds__(kThreads) kv_pages_assign_kernel(const __grid_
 #pragma unroll
     for (int x = 0; x < 8; ++x) words[x] = i8 + x < i1 ? __ldcg(p.ref + i8 + x) : 1u;
 #pragma unroll
-   for (int x = 0; x < 8; ++x) {
-    const int i = i8 + x;
-    const unsigned w = words[x];
-    if (i >= i1) break;
-    int count;
-    if (w == 0u) {
-      count = k < base;
-      if (count) {
-        int lo = 0, hi = p.rows - 1;  // the last row whose first wanted page is <= k
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (begin[mid] <= k) lo = mid;
-          else hi = mid - 1;
+    for (int x = 0; x < 8; ++x) {
+      const int i = i8 + x;
+      const unsigned w = words[x];
+      if (i >= i1) break;
+      int count;
+      if (w == 0u) {
+        count = k < base;
+        if (count) {
+          int lo = 0, hi = p.rows - 1;  // the last row whose first wanted page is <= k
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (begin[mid] <= k) lo = mid;
+            else hi = mid - 1;
+          }
+          const int s = k - begin[lo];
+          const bool cow = copies[lo >> 5] >> (lo & 31) & 1u;
+          if (cow && s == 0) p.dst[lo] = i;
+          p.out[(long long)lo * p.ld_out + have[lo] + s - cow] = i;
         }
-        const int s = k - begin[lo];
-        const bool cow = copies[lo >> 5] >> (lo & 31) & 1u;
-        if (cow && s == 0) p.dst[lo] = i;
-        p.out[(long long)lo * p.ld_out + have[lo] + s - cow] = i;
+        ++k;
+      } else if (w & kFlag) {
+        count = 1;
+      } else {
+        const int t = w & 0xffffu, writers = w >> 16;
+        count = t == writers ? 1 : t - writers;
       }
-      ++k;
-    } else if (w & kFlag) {
-      count = 1;
-    } else {
-      const int t = w & 0xffffu, writers = w >> 16;
-      count = t == writers ? 1 : t - writers;
+      p.ref[i] = (unsigned)count;
     }
-    p.ref[i] = (unsigned)count;
-   }
   }
   // copies' sources, and what found no page
   for (int b = gtid; b < p.rows; b += gthreads) {
