@@ -15,8 +15,9 @@
 // workspace, and the last of its CTAs to arrive joins them in CTA order, so
 // results do not depend on timing.  Starting and ending a unit costs a CTA about
 // as much as eight tiles, which the runs count (48 sequences of 0 to 4096
-// positions: 70 us without, 48 us with), and a short unit is not split (64
-// sequences of 256: 23 us split, 18 us whole).  Calls of more than kMaxEntries
+// positions: 67 us without, 48.6 us with), and a short unit is not split (64
+// sequences of 256: 19.7 us split, 17.9 us whole; one sequence of 512 loses, 8.3
+// us split and 10.0 us whole).  Calls of more than kMaxEntries
 // (sequence, row tile) pairs have units enough to give each CTA whole ones.
 //
 // Within a CTA.  One warp group (one warp for each 8, 16 or 24 rows) takes every NS-th
@@ -33,29 +34,31 @@
 // down to 2^-31 of the row's largest keep all of bf16's bits.  Scores, maxima,
 // sums and outputs are fp32.  P, times the block's V scale over the largest V
 // scale seen so far (which moves with the running maximum), enters the second
-// product as the sum of two bf16 numbers: 2^-17 of each weight and fp32's
+// product as the sum of two bf16 numbers: 2^-16 of each weight at most and fp32's
 // range, where one f16 would lose weights below 2^-24 of the largest and one
 // bf16 would add an error the size of the output's own rounding.
 // Scores and weights are computed transposed (tokens or dims are the 16 rows of a
 // tensor-core tile, query rows its 8 columns), so that eight rows waste nothing.
 //
-// Bounds, on B200 (1965 MHz unless said).  4 x 131072 positions, 64 query and 8 kv
-// heads of 128, int8: 157 us in a burst, 6.2 TB/s of cache, 95% of a copy's rate;
+// Bounds, on B200 (1965 MHz unless said).  4 sequences of 100001 to 131071
+// positions (983 MB), 64 query and 8 kv heads of 128, int8: 157 us in a burst,
+// 6.2 TB/s of cache, 95% of a copy's rate (4 x 131072: 171 us, the same rate);
 // under a second of it the power limit lowers the clock to 1.6 GHz and the
 // conversions of the codes (five instructions for four K codes, seven for four V
-// codes, 830 instructions per warp and tile in all) make it 190 us.  Small calls
+// codes, 830 instructions per warp and tile in all) make it 189 us.  Small calls
 // are a chain of latencies: lengths 2 us, pages and first tile 2.5 us, joining
-// runs 3 us; one sequence of 2048 takes 10.2 us where its bytes take 0.7.  More
+// runs 3 us; one sequence of 2048 takes 10.0 us where its bytes take 0.6.  More
 // rows add products: 16 sequences of 4300 on average with 8 / 16 / 24 / 32 / 64
-// rows per kv head take 37 / 49 / 61 / 82 / 148 us (memory: 23), bound by the
+// rows per kv head take 36 / 48 / 61 / 82 / 149 us (memory: 22), bound by the
 // instructions of conversions and products, which dependent chains at two warps per
 // scheduler issue at half rate.
-// Measured slower: the two products of a tile split between two warps that pass
-// weights through shared memory (24 rows 69 us); four warps of eight rows, each
-// converting for itself (32 rows 108 us); 3 stages and 2 CTAs per SM for 8
-// rows (168 us against 162); three 8-bit digits of q times K codes in integers,
-// which needs no conversion of K (187 us sustained, but 11.1 us for the single
-// sequence).
+// Measured slower, with earlier forms of the kernel (61 us for 24 rows, 82 for 32,
+// 162 for the long sequences): the two products of a tile split between two warps
+// that pass weights through shared memory (24 rows 69 us); four warps of eight
+// rows, each converting for itself (32 rows 108 us); 3 stages and 2 CTAs per SM
+// for 8 rows (168 us against 162); three 8-bit digits of q times K codes in
+// integers, which needs no conversion of K (187 us sustained against 190, but
+// 11.1 us for the single sequence).
 #include "wal_kv8.cuh"
 
 #include <cuda_fp16.h>
@@ -68,7 +71,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 32;          // positions of a tile
 constexpr int kMaxEntries = 1024;  // (sequence, row tile) pairs of a balanced call
-constexpr int kMinTiles = 4;       // least tiles of a run: one per warp (one sequence of 2048: 11.1 us, 12.5 with 8)
+constexpr int kMinTiles = 4;       // least tiles of a run: one per warp (one sequence of 2048: 10.0 us, 10.8 with 8; of 8192: 15.3 and 13.7)
 constexpr int kUnitCost = 8;       // what starting and ending a unit costs, in tiles
 constexpr unsigned kWholeCost = 28;  // units of at most this cost are not split
 constexpr float kSlack = 8.f;      // weights may reach 2^8 before the running maximum moves

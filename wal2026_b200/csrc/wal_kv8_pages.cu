@@ -15,9 +15,9 @@
 // sixteen for large ones: what they do is a few dependent passes over a few hundred
 // kilobytes, bound by the latency of the passes and of the barriers between, so
 // rows are kept in shared memory and pages read eight at a time.  On B200: tables
-// of 256 sequences with 65 k entries 12 us (96 us as one CTA, half of it atomics),
-// of 64 forked rows 7 us, a compaction of 2055 pages 13 us.  The copy moves 266 MB
-// of scattered 16 KB pieces in 48 us, 5.5 TB/s or 85% of a copy's rate; with CTAs
+// of 256 sequences with 65 k entries 15 us (96 us as one CTA, half of it atomics),
+// of 64 forked rows 10 us, a compaction of 2055 pages 11 us.  The copy moves 266 MB
+// of scattered 16 KB pieces in 50 us, 5.3 TB/s or 81% of a copy's rate; with CTAs
 // that first list the valid pairs together it took 60 us.
 #include "wal_kv8.cuh"
 

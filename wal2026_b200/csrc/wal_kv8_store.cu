@@ -15,9 +15,9 @@
 //   kv8_read_kernel    values code * scale of a range of positions.
 //
 // Bounds, on B200: four prompts of 1270 tokens on average (64 query and 8 kv heads of 128; 8192 rows
-// with padding): append 55 us for 277 MB, 5.0 TB/s or 77% of a copy's rate, of which
+// with padding): append 54 us for 277 MB, 5.1 TB/s or 78% of a copy's rate, of which
 // 265 MB are q and qkv; read-back 13 us for 48 MB.  A decode step of three
-// sequences takes 4.6 us for both kernels, all of it launch and two dependent
+// sequences takes 4.3 us for both kernels, all of it launch and two dependent
 // loads.  Threads per CTA and CTAs per SM: 256 and 3 against 128 and 5 made no
 // difference to the whole (68 us); fewer looping query warps lose (72 us with 3
 // CTAs per SM, 68 with 16).

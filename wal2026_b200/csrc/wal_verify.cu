@@ -14,8 +14,8 @@
 // warp whose share holds the drawn place reads it once more.  One row of p and,
 // after a rejection, one of q is all that is read.
 //
-// On B200, 128256 tokens: one sequence 6.6 us (1 MB: three dependent loads, the
-// sums, a cluster barrier and the second reading of one share), 64 sequences 20.5 us for 66
+// On B200, 128256 tokens: one sequence 6.9 us (1 MB: three dependent loads, the
+// sums, a cluster barrier and the second reading of one share), 64 sequences 20.4 us for 66
 // MB, 3.2 TB/s: half the time is the same chain before and after the rows stream.
 #include "wal_kv8.cuh"
 
@@ -229,8 +229,8 @@ extern "C" int wal_verify_drafts(const float* target, int64_t target_seq, int64_
                    (!draft || (draft_seq % 4 == 0 && draft_row % 4 == 0 && ((uintptr_t)draft & 15) == 0));
   // Few sequences leave SMs idle: eight CTAs each, one per SM.  A batch pays for
   // each CTA's start and barriers: four each, two per SM.  V = 128256 on B200:
-  // one sequence 7.1 us with eight CTAs one per SM, 7.8 two per SM; 64 sequences
-  // 26.1 us with four CTAs one per SM, 22.9 two per SM, 24.8 with eight of half the threads.
+  // one sequence 6.9 us with eight CTAs one per SM, 7.3 two per SM, 9.6 with four; 64
+  // sequences 25.1 us with four CTAs one per SM, 20.4 two per SM, 26.0 with eight.
   const bool few = B * kMaxCluster <= sm_count();
   const int cluster = few ? kMaxCluster : 4;
   auto kern = few ? (vec ? verify_kernel<true, 1> : verify_kernel<false, 1>) : (vec ? verify_kernel<true, 2> : verify_kernel<false, 2>);
