@@ -631,6 +631,44 @@ WAL_API int wal_verify_drafts(const float* target, int64_t target_seq, int64_t t
                       const int32_t* draft_lens, const float* uniforms, int64_t ld_uniforms, int64_t B,
                       int64_t T, int64_t V, int32_t* accepted, int32_t* tokens, int64_t ld_tokens, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit linear with group scales.  No reference counterpart.
+ *   y[m][n] = sum_g s[n][g] * sum_{k in g} (c[n][k] - z[n][g]) * x[m][k] + bias[n]
+ * over groups of group_size (32, 64 or 128) consecutive columns; codes c in
+ * 0..15, z in 0..15 or 8 everywhere (zeros NULL), s fp16.  Weights enter the
+ * products as the whole numbers c - z and sums are fp32, scaled once per group
+ * (or per 64 columns of one): nothing is rounded but x's own type and y.
+ *
+ * Packed: tiles of 16 rows (the last one filled up), each [ceil(K / 64)][32]
+ * 16-byte pieces.  Word w < 4 of piece 4 r + q of a 64-column chunk holds the
+ * codes of rows r and r + 8, four columns from k = 32 (w / 2) + 8 q + 4 (w % 2)
+ * on: nibbles 0 to 3 are (r, k), (r + 8, k), (r, k + 2), (r + 8, k + 2), nibbles
+ * 4 to 7 the same with k + 1.  Codes past K or past the last row are 0.  scales
+ * [tile][group][8][2] (rows r, r + 8), zeros bytes likewise.
+ * ------------------------------------------------------------------------ */
+typedef struct wal_int4_layer {
+  int64_t out_features;
+  int64_t in_features;   /* multiple of group_size                       */
+  int32_t group_size;    /* 32, 64 or 128                                */
+  const void* packed;    /* device, 16-byte aligned                      */
+  const uint16_t* scales;/* device fp16, 16-byte aligned                 */
+  const uint8_t* zeros;  /* device or NULL                               */
+  const uint16_t* bias;  /* device bf16 [out_features] or NULL           */
+} wal_int4_layer;
+
+/* Bytes of packed codes and entries of scales (and of zeros). */
+WAL_API int wal_int4_packed_size(int64_t out_features, int64_t in_features, int32_t group_size, size_t* packed_bytes,
+                      size_t* entries);
+/* Device codes [N][K] (one byte each, the low four bits), scales [N][K / group_size] fp16 and zeros (bytes, NULL
+ * where the layer has none) into the layer's buffers. */
+WAL_API int wal_int4_pack(const wal_int4_layer* layer, const uint8_t* codes, const uint16_t* scales,
+                      const uint8_t* zeros, void* stream);
+/* The weight s * (c - z), rounded once, as WAL_F32, WAL_BF16 or WAL_F16 rows ldw apart. */
+WAL_API int wal_int4_dequant(const wal_int4_layer* layer, void* w, int64_t ldw, int dtype, void* stream);
+/* x: bf16 or fp16, rows ldx apart (16-byte aligned, ldx a multiple of 8); y: any wal_dtype, rows ldy apart. */
+WAL_API int wal_int4_gemv(const wal_int4_layer* layer, const void* x, int x_dtype, int64_t M, int64_t ldx, void* y,
+                      int64_t ldy, int y_dtype, void* stream);
+
 /*
  * Device memory shared with peer processes: create (cudaMalloc, zero-filled,
  * IPC handle of WAL_IPC_HANDLE_BYTES written to handle_out), open a peer's

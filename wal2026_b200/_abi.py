@@ -129,6 +129,19 @@ class KV8Cache(ctypes.Structure):
     ]
 
 
+class Int4Layer(ctypes.Structure):
+    """``wal_int4_layer``: device buffers of one 4-bit linear."""
+    _fields_ = [
+        ("out_features", ctypes.c_int64),
+        ("in_features", ctypes.c_int64),
+        ("group_size", ctypes.c_int32),
+        ("packed", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+    ]
+
+
 _GP = ctypes.POINTER(Geometry)
 _LP = ctypes.POINTER(Layer)
 _CP = ctypes.POINTER(KV8Cache)
@@ -189,6 +202,11 @@ SIGNATURES: dict[str, tuple] = {
     "wal_kv_pages_copy": (_c_int, [_CP, _vp, _vp, _c_i64, _vp]),
     "wal_verify_drafts": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                    _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "wal_int4_packed_size": (_c_int, [_c_i64, _c_i64, _c_i32, ctypes.POINTER(ctypes.c_size_t),
+                                      ctypes.POINTER(ctypes.c_size_t)]),
+    "wal_int4_pack": (_c_int, [ctypes.POINTER(Int4Layer), _vp, _vp, _vp, _vp]),
+    "wal_int4_dequant": (_c_int, [ctypes.POINTER(Int4Layer), _vp, _c_i64, _c_int, _vp]),
+    "wal_int4_gemv": (_c_int, [ctypes.POINTER(Int4Layer), _vp, _c_int, _c_i64, _c_i64, _vp, _c_i64, _c_int, _vp]),
     "wal_peer_region_create": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "wal_peer_region_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),
     "wal_peer_region_close": (_c_int, [_vp]),

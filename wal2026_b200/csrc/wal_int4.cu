@@ -1,0 +1,352 @@
+// 4-bit linear with group scales: y = x W^T for up to 32 tokens per launch.
+//
+//   y[m, n] = sum_g s[n, g] * sum_{k in g} (c[n, k] - z[n, g]) * x[m, k] + bias[n]
+//
+// The codes are read once and are nearly all of the traffic, so the kernel is
+// built to keep 16-byte loads of them in flight.  They are packed in the order of
+// the A fragments of mma.sync m16n8k16 (16 weight rows; tokens are the eight
+// columns): one 16-byte load of a warp is 16 rows x 64 columns, each of its words
+// a lane's fragment of one product.  A code becomes a 16-bit float with a logic
+// instruction (the code in the low bits of 128 as bf16, of 1024 as f16) and an exact
+// subtraction of 128 + z or 1024 + z, so the products see whole numbers; a group's
+// fp32 sum is scaled once.  The order of k inside a product is free: a lane's
+// columns are chosen so that its activations are two 16-byte loads (they hit L1).
+//
+// Split.  A warp takes one or two row tiles (two from 9 tokens on, which halves
+// the activation reads per weight) and every ks-th chunk of 64 columns; the ks
+// warps of a tile meet in shared memory and are summed in order, so results do
+// not depend on timing.
+#include "wal_kv8.cuh"
+
+#include <cuda_fp16.h>
+
+namespace {
+
+using wal_kv8::launch_chain;
+using wal_kv8::sm_count;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kAhead = 4;  // chunks loaded together
+
+struct Int4Params {
+  const uint4* packed;    // [tiles][chunks][32]
+  const uint32_t* scales; // [tiles][groups][8] pairs of rows r, r + 8
+  const uint16_t* zeros;  // likewise, bytes
+  const uint16_t* bias;
+  const uint16_t* x;
+  void* y;
+  long long ldx, ldy;
+  int M, N, K, tiles, chunks, groups;
+  int per;  // chunks per group as a shift (0 or 1)
+  int ks;   // warps that share a tile
+  int y_dtype;
+};
+
+template <bool F16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (F16) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// 128 (bf16) or 1024 (f16) twice; a code in the low bits adds itself
+template <bool F16>
+__device__ __forceinline__ constexpr uint32_t magic() { return F16 ? 0x64006400u : 0x43004300u; }
+
+// A fragment of one product from a word: rows r (registers 0, 2) and r + 8 (1, 3), minus their zero points.
+template <bool F16>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = sub2<F16>(((w >> (4 * i)) & 0x000f000fu) | magic<F16>(), i & 1 ? z1 : z0);
+}
+
+__device__ __forceinline__ uint4 load_codes(const uint4* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void store(void* y, int dtype, long long at, float v) {
+  if (dtype == WAL_F32) static_cast<float*>(y)[at] = v;
+  else if (dtype == WAL_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+}
+
+// NT: tiles of eight tokens, RT: row tiles per warp, GPC: groups in a chunk of 64 columns (1 or 2)
+template <int NT, int RT, int GPC, bool F16, bool ZEROS>
+__global__ void __launch_bounds__(kThreads) int4_gemv_kernel(const __grid_constant__ Int4Params p) {
+  constexpr int LDR = 8 * NT + 1;
+  __shared__ float red[kWarps][RT * 16][LDR];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, q = lane & 3;
+  const int own = kWarps / p.ks;  // row-tile groups of this CTA
+  const int tile0 = ((int)blockIdx.x * own + warp / p.ks) * RT, kslice = warp % p.ks;
+
+  struct Batch {
+    uint4 w[kAhead][RT];
+    uint32_t s[kAhead][RT][GPC];
+    uint16_t z[kAhead][RT][ZEROS ? GPC : 1];
+  };
+  auto fetch = [&](Batch& b, int c0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int c = c0 + i * p.ks, tile = tile0 + t;
+        const bool real = c < p.chunks && tile < p.tiles;
+        b.w[i][t] = real ? load_codes(p.packed + ((long long)tile * p.chunks + c) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int g = 0; g < GPC; ++g) {
+          const int gi = GPC == 2 ? min(2 * c + g, p.groups - 1) : c >> p.per;
+          const long long at = ((long long)tile * p.groups + gi) * 8 + r;
+          b.s[i][t][g] = real ? __ldg(p.scales + at) : 0u;
+          if (ZEROS) b.z[i][t][g] = real ? __ldg(p.zeros + at) : (uint16_t)0;
+        }
+      }
+  };
+
+  float tot[RT][NT][4];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) tot[t][n][0] = tot[t][n][1] = tot[t][n][2] = tot[t][n][3] = 0.f;
+
+  Batch cur;
+  fetch(cur, kslice);  // weights do not depend on the kernels before this one
+  wal_kv8::chain();
+  for (int c0 = kslice; c0 < p.chunks; c0 += kAhead * p.ks) {
+    Batch next;
+    fetch(next, c0 + kAhead * p.ks);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int c = c0 + i * p.ks;
+      if (c >= p.chunks) break;
+      uint32_t xw[NT][2][4];  // columns 32 h + 8 q .. + 7 of token 8 n + r
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = 64 * c + 32 * h + 8 * q;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (8 * n + r < p.M && k < p.K) v = __ldg(reinterpret_cast<const uint4*>(p.x + (8 * n + r) * p.ldx + k));
+          xw[n][h][0] = v.x;
+          xw[n][h][1] = v.y;
+          xw[n][h][2] = v.z;
+          xw[n][h][3] = v.w;
+        }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const uint32_t w[4] = {cur.w[i][t].x, cur.w[i][t].y, cur.w[i][t].z, cur.w[i][t].w};
+        float acc[NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int g = GPC == 2 ? h : 0;
+          if (h == 0 || GPC == 2)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+          uint32_t z0 = F16 ? 0x64086408u : 0x43084308u, z1 = z0;
+          if (ZEROS) {
+            const uint32_t z = cur.z[i][t][g];
+            z0 = (z & 0xffu) * 0x00010001u + magic<F16>();
+            z1 = (z >> 8) * 0x00010001u + magic<F16>();
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t a[4];
+            unpack<F16>(w[2 * h + e], z0, z1, a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<F16>(acc[n], a, xw[n][h][2 * e], xw[n][h][2 * e + 1]);
+          }
+          if (h == 1 || GPC == 2) {
+            const uint32_t sc = cur.s[i][t][g];
+            const float s0 = __half2float(__ushort_as_half((unsigned short)(sc & 0xffffu))), s1 = __half2float(__ushort_as_half((unsigned short)(sc >> 16)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              tot[t][n][0] = fmaf(s0, acc[n][0], tot[t][n][0]);
+              tot[t][n][1] = fmaf(s0, acc[n][1], tot[t][n][1]);
+              tot[t][n][2] = fmaf(s1, acc[n][2], tot[t][n][2]);
+              tot[t][n][3] = fmaf(s1, acc[n][3], tot[t][n][3]);
+            }
+          }
+        }
+      }
+    }
+    cur = next;
+  }
+
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][16 * t + r + 8 * (e >> 1)][8 * n + 2 * q + (e & 1)] = tot[t][n][e];
+  __syncthreads();
+  const int rows = own * RT * 16, m = min(p.M, 8 * NT);
+  for (int i = tid; i < rows * m; i += kThreads) {
+    const int row = i % rows, tok = i / rows, grp = row / (RT * 16), rr = row % (RT * 16);
+    const long long n = ((long long)blockIdx.x * own + grp) * RT * 16 + rr;
+    if (n >= p.N) continue;
+    float v = 0.f;
+    for (int k = 0; k < p.ks; ++k) v += red[grp * p.ks + k][rr][tok];
+    if (p.bias) v += __uint_as_float((uint32_t)p.bias[n] << 16);
+    store(p.y, p.y_dtype, tok * p.ldy + n, v);
+  }
+}
+
+// One word of packed codes per thread, and the first threads the scales and zeros.
+__global__ void int4_pack_kernel(uint32_t* packed, uint32_t* scales, uint16_t* zeros, const uint8_t* codes, const uint16_t* s,
+                                 const uint8_t* z, long long N, long long K, long long tiles, int chunks, int groups) {
+  const long long words = tiles * chunks * 128, meta = tiles * groups * 8;
+  const long long step = (long long)gridDim.x * blockDim.x;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += step) {
+    const int w = (int)(i & 3), piece = (int)(i >> 2) & 31;
+    const long long rest = i >> 7, c = rest % chunks, tile = rest / chunks;
+    const long long row = tile * 16 + (piece >> 2), k = 64 * c + 32 * (w >> 1) + 8 * (piece & 3) + 4 * (w & 1);
+    uint32_t v = 0;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const long long rr = row + 8 * (n & 1), kk = k + 2 * ((n >> 1) & 1) + (n >> 2);
+      if (rr < N && kk < K) v |= (uint32_t)(codes[rr * K + kk] & 15) << (4 * n);
+    }
+    packed[i] = v;
+  }
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < meta; i += step) {
+    const int r = (int)(i & 7);
+    const long long g = (i >> 3) % groups, row = (i >> 3) / groups * 16 + r;
+    const bool lo = row < N, hi = row + 8 < N;
+    scales[i] = (lo ? (uint32_t)s[row * groups + g] : 0u) | (hi ? (uint32_t)s[(row + 8) * groups + g] << 16 : 0u);
+    if (zeros) zeros[i] = (uint16_t)((lo ? z[row * groups + g] & 15 : 0) | (hi ? (z[(row + 8) * groups + g] & 15) << 8 : 0));
+  }
+}
+
+__global__ void int4_dequant_kernel(const uint32_t* packed, const uint16_t* scales, const uint8_t* zeros, void* w, long long ldw,
+                                    int dtype, long long N, long long K, int chunks, int groups, int group_size) {
+  const long long step = (long long)gridDim.x * blockDim.x;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < N * K; i += step) {
+    const long long row = i / K, k = i % K, tile = row >> 4;
+    const int rr = (int)(row & 15), c = (int)(k >> 6), j = (int)(k & 63);
+    const int word = 2 * (j >> 5) + ((j >> 2) & 1), piece = 4 * (rr & 7) + ((j >> 3) & 3);
+    const int nib = (rr >> 3) + 2 * ((j >> 1) & 1) + 4 * (j & 1);
+    const uint32_t v = packed[((tile * chunks + c) * 32 + piece) * 4 + word];
+    const long long m = ((tile * groups + k / group_size) * 8 + (rr & 7)) * 2 + (rr >> 3);
+    const float z = zeros ? (float)zeros[m] : 8.f;
+    store(w, dtype, row * ldw + k, ((float)((v >> (4 * nib)) & 15) - z) * __half2float(__ushort_as_half(scales[m])));
+  }
+}
+
+int check_layer(const wal_int4_layer* l) {
+  if (!l || !l->packed || !l->scales) return WAL_ERR_INVALID_ARGUMENT;
+  size_t bytes, entries;
+  const int st = wal_int4_packed_size(l->out_features, l->in_features, l->group_size, &bytes, &entries);
+  if (st != WAL_OK) return st;
+  if (((uintptr_t)l->packed & 15) || ((uintptr_t)l->scales & 15) || ((uintptr_t)l->zeros & 1)) return WAL_ERR_ALIGNMENT;
+  return WAL_OK;
+}
+
+template <int NT, int RT>
+int launch(const Int4Params& p, int gpc, bool f16, cudaStream_t st) {
+  const int own = kWarps / p.ks;
+  const dim3 grid((unsigned)((p.tiles + own * RT - 1) / (own * RT)));
+#define WAL_INT4(G, F, Z) launch_chain(int4_gemv_kernel<NT, RT, G, F, Z>, grid, kThreads, 0, st, p)
+  if (gpc == 2) {
+    if (f16) return p.zeros ? WAL_INT4(2, true, true) : WAL_INT4(2, true, false);
+    return p.zeros ? WAL_INT4(2, false, true) : WAL_INT4(2, false, false);
+  }
+  if (f16) return p.zeros ? WAL_INT4(1, true, true) : WAL_INT4(1, true, false);
+  return p.zeros ? WAL_INT4(1, false, true) : WAL_INT4(1, false, false);
+#undef WAL_INT4
+}
+
+}  // namespace
+
+extern "C" {
+
+int wal_int4_packed_size(int64_t out_features, int64_t in_features, int32_t group_size, size_t* packed_bytes, size_t* entries) {
+  if (!packed_bytes || !entries) return WAL_ERR_INVALID_ARGUMENT;
+  if (group_size != 32 && group_size != 64 && group_size != 128) return WAL_ERR_UNSUPPORTED;
+  if (out_features <= 0 || in_features <= 0 || in_features % group_size) return WAL_ERR_SHAPE;
+  if (out_features > (1 << 30) || in_features > (1 << 30)) return WAL_ERR_SHAPE;
+  const size_t tiles = (size_t)((out_features + 15) / 16);
+  *packed_bytes = tiles * (size_t)((in_features + 63) / 64) * 512;
+  *entries = tiles * 16 * (size_t)(in_features / group_size);
+  return WAL_OK;
+}
+
+int wal_int4_pack(const wal_int4_layer* l, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, void* stream) {
+  const int st = check_layer(l);
+  if (st != WAL_OK) return st;
+  if (!codes || !scales || !l->zeros != !zeros) return WAL_ERR_INVALID_ARGUMENT;
+  int4_pack_kernel<<<sm_count() * 8, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<uint32_t*>(const_cast<void*>(l->packed)), reinterpret_cast<uint32_t*>(const_cast<uint16_t*>(l->scales)),
+      reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(l->zeros)), codes, scales, zeros, l->out_features, l->in_features,
+      (l->out_features + 15) / 16, (int)((l->in_features + 63) / 64), (int)(l->in_features / l->group_size));
+  return cudaGetLastError() == cudaSuccess ? WAL_OK : WAL_ERR_CUDA;
+}
+
+int wal_int4_dequant(const wal_int4_layer* l, void* w, int64_t ldw, int dtype, void* stream) {
+  const int st = check_layer(l);
+  if (st != WAL_OK) return st;
+  if (!w) return WAL_ERR_INVALID_ARGUMENT;
+  if (dtype != WAL_BF16 && dtype != WAL_F32 && dtype != WAL_F16) return WAL_ERR_UNSUPPORTED;
+  if (ldw < l->in_features) return WAL_ERR_SHAPE;
+  if ((uintptr_t)w & (dtype == WAL_F32 ? 3 : 1)) return WAL_ERR_ALIGNMENT;
+  int4_dequant_kernel<<<sm_count() * 8, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(l->packed), l->scales, l->zeros, w, ldw, dtype, l->out_features, l->in_features,
+      (int)((l->in_features + 63) / 64), (int)(l->in_features / l->group_size), l->group_size);
+  return cudaGetLastError() == cudaSuccess ? WAL_OK : WAL_ERR_CUDA;
+}
+
+int wal_int4_gemv(const wal_int4_layer* l, const void* x, int x_dtype, int64_t M, int64_t ldx, void* y, int64_t ldy, int y_dtype,
+                  void* stream) {
+  const int st = check_layer(l);
+  if (st != WAL_OK) return st;
+  if (!x || !y) return WAL_ERR_INVALID_ARGUMENT;
+  if (x_dtype != WAL_BF16 && x_dtype != WAL_F16) return WAL_ERR_UNSUPPORTED;
+  if (y_dtype != WAL_BF16 && y_dtype != WAL_F32 && y_dtype != WAL_F16) return WAL_ERR_UNSUPPORTED;
+  if (M <= 0 || M > 0x7fffffff || ldx < l->in_features || ldy < l->out_features) return WAL_ERR_SHAPE;
+  const int ysize = y_dtype == WAL_F32 ? 4 : 2;
+  if (((uintptr_t)x & 15) || (ldx % 8) || ((uintptr_t)y & (ysize - 1)) || (l->bias && ((uintptr_t)l->bias & 1))) return WAL_ERR_ALIGNMENT;
+  Int4Params p = {};
+  p.packed = static_cast<const uint4*>(l->packed);
+  p.scales = reinterpret_cast<const uint32_t*>(l->scales);
+  p.zeros = reinterpret_cast<const uint16_t*>(l->zeros);
+  p.bias = l->bias;
+  p.ldx = ldx;
+  p.ldy = ldy;
+  p.N = (int)l->out_features;
+  p.K = (int)l->in_features;
+  p.tiles = (p.N + 15) / 16;
+  p.chunks = (p.K + 63) / 64;
+  p.groups = p.K / l->group_size;
+  p.per = l->group_size == 128 ? 1 : 0;
+  p.y_dtype = y_dtype;
+  p.ks = 1;
+  while (p.ks < kWarps && p.ks * 2 <= p.chunks) p.ks *= 2;
+  for (int64_t m0 = 0; m0 < M; m0 += 32) {
+    p.x = static_cast<const uint16_t*>(x) + m0 * ldx;
+    p.y = static_cast<uint8_t*>(y) + m0 * ldy * ysize;
+    p.M = (int)(M - m0 < 32 ? M - m0 : 32);
+    const int gpc = l->group_size == 32 ? 2 : 1;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int rc = p.M <= 8    ? launch<1, 1>(p, gpc, x_dtype == WAL_F16, s)
+                   : p.M <= 16 ? launch<2, 2>(p, gpc, x_dtype == WAL_F16, s)
+                               : launch<4, 2>(p, gpc, x_dtype == WAL_F16, s);
+    if (rc != WAL_OK) return rc;
+  }
+  return WAL_OK;
+}
+
+}  // extern "C"
