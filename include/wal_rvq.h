@@ -631,6 +631,49 @@ WAL_API int wal_verify_drafts(const float* target, int64_t target_seq, int64_t t
                       const int32_t* draft_lens, const float* uniforms, int64_t ld_uniforms, int64_t B,
                       int64_t T, int64_t V, int32_t* accepted, int32_t* tokens, int64_t ld_tokens, void* stream);
 
+/*
+ * Rules on logits.  Row (b, t) of logits (wal_dtype; sequences ld_seq, rows
+ * ld_row elements apart) becomes fp32 out[b][t] (contiguous rows out_row
+ * apart), V entries each.  With x the logit in fp32, `before` the tokens
+ * text[b][j], j <= lens[b] + t (bounded by text_len), and `made` those of them
+ * with j >= prompt_lens[b] (NULL: 0):
+ *   v in before:  x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   x -= frequency[b] * (times v is in made);  x -= presence[b] if v is in made
+ *   x += the sum of bias[b][i], in rising i, over bias_ids[b][i] = v
+ *   bit v % 32 of mask word v / 32 of (b, t) clear, or x NaN: left out (-inf)
+ *   x /= temperature[b]  (NULL: 1)
+ * softmax != 0: out = softmax(x): where the largest x is an infinity, the
+ * entries that have it share 1; temperature 0 (or negative, or NaN) gives 1 to
+ * the first of the largest, 0 to the others; a row with nothing left is zeros.
+ * softmax == 0: out = x, with no division at temperature 0.
+ * repetition, frequency, presence, temperature: fp32 [B] or NULL; text int32
+ * (rows ld_text apart; NULL where text_len is 0) and lens [B] may be NULL where the first three are;
+ * bias_ids int32 / bias fp32 [B][num_bias] or NULL; mask: int32 words
+ * (sequences mask_seq, rows mask_row words apart, 0 to share them) or NULL.
+ * Tokens outside [0, V) count nowhere.  Rows t >= new_lens[b] (NULL: T) are
+ * zeros.  V <= 393216, num_bias <= 1024, B * T < 2^27.  out must not overlap logits.
+ */
+typedef struct wal_logit_rules {
+  const int32_t* text;
+  int64_t ld_text, text_len;
+  const int32_t* lens;
+  const int32_t* prompt_lens;
+  const int32_t* new_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;
+  const float* bias;
+  int64_t num_bias;
+  const int32_t* mask;
+  int64_t mask_seq, mask_row;
+  const float* temperature;
+} wal_logit_rules;
+
+WAL_API int wal_logit_rules_apply(const wal_logit_rules* rules, const void* logits, int dtype, int64_t ld_seq,
+                      int64_t ld_row, int64_t B, int64_t T, int64_t V, float* out, int64_t out_seq,
+                      int64_t out_row, int softmax, void* stream);
+
 /* ------------------------------------------------------------------------
  * 4-bit linear with group scales.  No reference counterpart.
  *   y[m][n] = sum_g s[n][g] * sum_{k in g} (c[n][k] - z[n][g]) * x[m][k] + bias[n]

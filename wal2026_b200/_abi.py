@@ -129,6 +129,28 @@ class KV8Cache(ctypes.Structure):
     ]
 
 
+class LogitRules(ctypes.Structure):
+    """``wal_logit_rules``: device arrays of the rules on logits."""
+    _fields_ = [
+        ("text", ctypes.c_void_p),
+        ("ld_text", ctypes.c_int64),
+        ("text_len", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+        ("prompt_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("num_bias", ctypes.c_int64),
+        ("mask", ctypes.c_void_p),
+        ("mask_seq", ctypes.c_int64),
+        ("mask_row", ctypes.c_int64),
+        ("temperature", ctypes.c_void_p),
+    ]
+
+
 class Int4Layer(ctypes.Structure):
     """``wal_int4_layer``: device buffers of one 4-bit linear."""
     _fields_ = [
@@ -202,6 +224,8 @@ SIGNATURES: dict[str, tuple] = {
     "wal_kv_pages_copy": (_c_int, [_CP, _vp, _vp, _c_i64, _vp]),
     "wal_verify_drafts": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                    _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "wal_logit_rules_apply": (_c_int, [ctypes.POINTER(LogitRules), _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
+                                       _c_i64, _c_i64, _c_int, _vp]),
     "wal_int4_packed_size": (_c_int, [_c_i64, _c_i64, _c_i32, ctypes.POINTER(ctypes.c_size_t),
                                       ctypes.POINTER(ctypes.c_size_t)]),
     "wal_int4_pack": (_c_int, [ctypes.POINTER(Int4Layer), _vp, _vp, _vp, _vp]),
