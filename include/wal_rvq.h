@@ -631,6 +631,47 @@ WAL_API int wal_verify_drafts(const float* target, int64_t target_seq, int64_t t
                       const int32_t* draft_lens, const float* uniforms, int64_t ld_uniforms, int64_t B,
                       int64_t T, int64_t V, int32_t* accepted, int32_t* tokens, int64_t ld_tokens, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Several samples of one prompt over the paged cache.  No reference counterpart.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Rows of a page table that share their first positions (forks of one prompt).
+ * A row is able when its whole pages, rounded down to a multiple of 32
+ * positions, hold `least` positions of its lens[b] (at most width * page_size -
+ * 1) and its table entry of position least - 1 is not negative.  Able rows with
+ * the same such entry form a group; what the group shares are the leading table
+ * entries that all its members' whole pages have in common, in positions,
+ * rounded down to a multiple of 32.  A group of one row, or one that shares
+ * fewer than `least` positions, is left out.  groups: int32 [4][rows]:
+ *   [0] the members' rows, group by group, then -1;
+ *   [1] index in [0] of the i-th group's first member, then 0;
+ *   [2] members of the i-th group, then 0;
+ *   [3] positions that row b shares with its group, 0 where it has none.
+ * Groups rise by their lowest member, members rise.  rows <= 4096, least >= 1,
+ * (width + 1) * page_size <= 2^31.
+ */
+WAL_API int wal_kv_pages_groups(const int32_t* table, int64_t ld_table, const int32_t* lens, int64_t rows,
+                        int64_t width, int32_t page_size, int64_t least, int32_t* groups, void* stream);
+
+/*
+ * wal_kv8_attention with the positions that the rows of a group share read
+ * once for all of them (groups: int32 [4][B] as wal_kv_pages_groups writes it,
+ * for this table and these lens).  The same result up to the rounding of 16-bit
+ * weights: every row attends to its own positions j <= lens[b] + t.  Entries of
+ * groups are bounded by the kernels; where they do not belong to the table, the
+ * rows concerned are wrong and nothing else.  B <= 4096.
+ * workspace: at least wal_kv8_attention_shared_workspace bytes, otherwise as in
+ * wal_kv8_attention.  status (NULL allowed): device word that becomes nonzero
+ * where a wait inside the kernel gave up after 2 s.
+ */
+WAL_API size_t wal_kv8_attention_shared_workspace(const wal_kv8_cache* cache, int64_t B, int64_t T, int32_t hq);
+WAL_API int wal_kv8_attention_shared(const wal_kv8_cache* cache, int32_t layer, const uint16_t* q, int64_t ld_q,
+                      int64_t B, int64_t T, int32_t hq, const int32_t* table, int64_t ld_table,
+                      int64_t max_pages, const int32_t* lens, const int32_t* new_lens, const int32_t* groups,
+                      float scale, uint16_t* out, int64_t ld_out, void* workspace, size_t workspace_bytes,
+                      int32_t* status, void* stream);
+
 /*
  * Rules on logits.  Row (b, t) of logits (wal_dtype; sequences ld_seq, rows
  * ld_row elements apart) becomes fp32 out[b][t] (contiguous rows out_row

@@ -224,6 +224,10 @@ SIGNATURES: dict[str, tuple] = {
     "wal_kv_pages_copy": (_c_int, [_CP, _vp, _vp, _c_i64, _vp]),
     "wal_verify_drafts": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                    _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "wal_kv_pages_groups": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _c_i64, _vp, _vp]),
+    "wal_kv8_attention_shared_workspace": (ctypes.c_size_t, [_CP, _c_i64, _c_i64, _c_i32]),
+    "wal_kv8_attention_shared": (_c_int, [_CP, _c_i32, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _c_i64, _vp, _vp,
+                                          _vp, ctypes.c_float, _vp, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
     "wal_logit_rules_apply": (_c_int, [ctypes.POINTER(LogitRules), _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
                                        _c_i64, _c_i64, _c_int, _vp]),
     "wal_int4_packed_size": (_c_int, [_c_i64, _c_i64, _c_i32, ctypes.POINTER(ctypes.c_size_t),

@@ -274,6 +274,72 @@ def kv8_attention(cache: PagedKV8Cache, layer: int, q: Tensor, table: Tensor, le
           out.data_ptr(), ld_o, workspace.data_ptr(), workspace.nbytes)
 
 
+def _why_not_groups(table, lens, groups) -> None:
+    rows, _ = _table("table", table)
+    _i32("lens", lens, rows)
+    _i32("groups", groups, 4, rows)
+    _cuda(table.device)
+    _on(table.device, lens=lens, groups=groups)
+    raise ValueError("kv_pages_groups: arguments do not fit together")
+
+
+def kv_pages_groups(table: Tensor, lens: Tensor, page_size: int, groups: Tensor, *, least: int = 256) -> None:
+    """Groups of rows whose first ``least`` positions (or more) lie in the same pages, for ``kv8_attention_shared``.
+
+    groups: int32 [4, rows]: the members' rows, group by group; each group's
+    first member in that list; its size; and, for each row, how many
+    positions (a multiple of 32, below lens[row]) it shares with its group, 0 where it
+    has none.  Rows that share fewer than ``least`` positions stay alone, so a larger
+    ``least`` keeps a short common beginning from holding together rows that have more in
+    common with some of the others.  One call serves all layers of a step.
+    """
+    index, ts, t1 = table.get_device(), table.shape, table.stride()
+    if not (index >= 0 and len(ts) == 2 and t1[1] == 1 and t1[0] >= ts[1] and table.dtype is _I32 and _is_i32(lens, ts[:1], index)
+            and _is_i32(groups, (4, ts[0]), index)):
+        _why_not_groups(table, lens, groups)
+    _call(index, "wal_kv_pages_groups", table.data_ptr(), t1[0], lens.data_ptr(), ts[0], ts[1], page_size, least,
+          groups.data_ptr())
+
+
+def kv8_attention_shared_workspace(cache: PagedKV8Cache, batch: int, hq: int, tokens: int = 1) -> Tensor:
+    """Zero-filled scratch for ``kv8_attention_shared`` calls of ``batch`` sequences with ``tokens`` new tokens each."""
+    nbytes = int(_abi.load().wal_kv8_attention_shared_workspace(cache._ref, batch, tokens, hq))
+    if nbytes == 0:
+        raise ValueError("invalid attention shape")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=cache.device)
+
+
+def kv8_attention_shared(cache: PagedKV8Cache, layer: int, q: Tensor, table: Tensor, lens: Tensor, groups: Tensor, out: Tensor,
+                         workspace: Tensor, *, new_lens: Optional[Tensor] = None, scale: Optional[float] = None,
+                         status: Optional[Tensor] = None) -> None:
+    """``kv8_attention``, with what the rows of a group share read once for all of them.
+
+    groups: int32 [4, B] from ``kv_pages_groups`` for this table and these lens.
+    The result is that of ``kv8_attention`` up to the rounding of weights to 16 bits.
+    ``workspace`` comes from ``kv8_attention_shared_workspace``, for this many
+    sequences and tokens, and is not shared by overlapping calls; status: int32 [1],
+    set to 1 where a wait inside the kernel gave up (the outputs are wrong then).
+    """
+    hd = cache.head_dim
+    width = q.shape[-1] if q.dim() else 0
+    hq = width // hd
+    step = _step(cache, q, width, out, hq, table, lens, new_lens)
+    if not (step is not None and width > 0 and width % (hd * cache.kv_heads) == 0 and _is_i32(groups, (4, step[0]), cache.index)
+            and workspace.get_device() == cache.index and workspace.is_contiguous()
+            and (status is None or _is_i32(status, (1,), cache.index))):
+        B = table.shape[0] if table.dim() else 0
+        _i32("groups", groups, 4, B)
+        if status is not None:
+            _i32("status", status, 1)
+        _on(cache.device, groups=groups, status=status)
+        _why_not_attention(cache, q, table, lens, out, workspace, new_lens)
+    B, T, pages, ld_q, ld_o, ld_t = step
+    _call(cache.index, "wal_kv8_attention_shared", cache._ref, layer, q.data_ptr(), ld_q, B, T, hq, table.data_ptr(), ld_t, pages,
+          lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), groups.data_ptr(),
+          hd ** -0.5 if scale is None else scale, out.data_ptr(), ld_o, workspace.data_ptr(), workspace.nbytes,
+          None if status is None else status.data_ptr())
+
+
 def _why_not_assign(table, parent, keep, add, table_out, ref_out, copy_src, copy_dst, info) -> None:
     _, width = _table("table", table)
     rows, w2 = _table("table_out", table_out)
