@@ -258,13 +258,18 @@ def test_shared_attention_nan_and_infinity_stay_in_their_row():
     cache = _filled(pages, hkv, P, hd, INT8, 2)
     q = torch.randn(5, hq * hd, device=DEV, generator=_gen(2)).to(torch.bfloat16)
     groups, ws = _groups(table, lens, P, 64), kv8_attention_shared_workspace(cache, 5, hq, 1)
-    clean = _check(cache, q, table, lens, groups, ws=ws)
-    q[1, 5], q[3, 200] = float("nan"), float("inf")
-    out = torch.empty_like(clean)
-    kv8_attention_shared(cache, 0, q, table, _i32(lens), groups, out, ws)
-    assert torch.equal(out[[0, 2, 4]], clean[[0, 2, 4]])
+    _check(cache, q, table, lens, groups, ws=ws)
+    bad = q.clone()
+    bad[1, 5], bad[3, 200] = float("nan"), float("inf")
+    out = torch.empty_like(q)
+    kv8_attention_shared(cache, 0, bad, table, _i32(lens), groups, out, ws)
     assert bool(out[1, :hd].isnan().all()) and bool(out[3, hd:2 * hd].isnan().any())
-    assert torch.equal(out[1, hd:], clean[1, hd:])
+    # the other rows and heads: rows of a warp share when their references move and which form of exp2 they take, so
+    # their bits may differ from the clean call's; their error may not
+    want, mag, most = _attention64(cache, q, table, lens, [1] * 5, hd ** -0.5, 0)
+    off = (out.double() - want).abs() > 1.01 * 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * mag + 2.0 ** -32 * most
+    off[1, :hd] = off[3, hd:2 * hd] = False
+    assert not bool(off.any()) and bool(out[[0, 2, 4]].isfinite().all()) and bool(out[1, hd:].isfinite().all())
 
 
 def test_one_workspace_serves_calls_of_changing_lengths_and_groups():

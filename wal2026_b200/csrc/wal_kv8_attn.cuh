@@ -188,6 +188,21 @@ __device__ __forceinline__ void to_bf16(const Masks& k, uint32_t w, uint32_t& p0
   }
 }
 
+// What the kernel of the shared prefixes leaves, in parts of (reference exponent,
+// sum, weighted sum): a unit of up to 256 query rows of a group and kv head has
+// one part per CTA that took some of its tiles, and two (for alternate tiles) where it
+// has no more than 128 rows.
+constexpr int kSlotRows = 128, kUnitRows = 256;
+struct PrefixParts {
+  float* first;         // [B * T][hq][2][HD] of the first CTA
+  float2* first_stats;  // [B * T][hq][2]
+  float* later;         // [CTA][2][128][HD] of a CTA that is not the unit's first
+  float2* later_stats;  // [CTA][2][128]
+  int4* rows;           // [B] a row's group: number of its first unit, the row's place in it, units of a kv head
+  int4* units;          // first and last CTA of a unit, and whether it has more than 128 rows
+  int max_units, ctas;
+};
+
 struct AttnParams {
   const uint16_t* q;
   long long ld_q;
@@ -207,10 +222,9 @@ struct AttnParams {
   unsigned units;  // (sequence, row tile, kv head)
   bool balanced;
   Masks masks;
-  // with shared prefixes (SH): positions before from[b] were attended to already
-  const int* from;        // [B], or what the caller's groups say
-  const float* pre;       // [B * T][hq][HD] weighted sums over them
-  const float2* pre_stats;  // [B * T][hq] (reference exponent, sum); no sum where there is nothing
+  // with shared prefixes (SH): positions before from[b] are attended to by the kernel before this one
+  const int* from;  // [B], or whatever the caller's groups say
+  PrefixParts parts;
 };
 
 // A tile's rows stand HD bytes apart; their 16-byte pieces are permuted within
@@ -254,20 +268,46 @@ __device__ __forceinline__ int first_tile(const AttnParams& p, int b, int n) {
   return SH ? min(max(p.from[b], 0), max(n - 1, 0)) / kTile : 0;
 }
 
-// Joins what row (sequence row m = b * T + t, head h) has from the shared prefix to (M, L, acc) of dims 4 c .. 4 c + 3.
+// Joins the parts that row (b, t), head g of kv head kvh, has from its group to (M, L, acc) of dims 4 c .. 4 c + 3.
+// Every number read is bounded: groups that do not belong to the table cost the rows concerned and nothing else.
 template <int HD>
-__device__ __forceinline__ void join_prefix(const AttnParams& p, long long m, int h, int c, float& M, float& L, float4& acc) {
-  const long long at = m * p.hq + h;
-  const float2 st = __ldcg(p.pre_stats + at);
-  if (st.y == 0.f) return;
-  const float4 v = __ldcg(reinterpret_cast<const float4*>(p.pre) + at * (HD / 4) + c);
-  const float mn = fmaxf(M, st.x), a = ex2(M - mn), f = ex2(st.x - mn);
-  M = mn;
-  L = fmaf(L, a, f * st.y);
-  acc.x = fmaf(acc.x, a, f * v.x);
-  acc.y = fmaf(acc.y, a, f * v.y);
-  acc.z = fmaf(acc.z, a, f * v.z);
-  acc.w = fmaf(acc.w, a, f * v.w);
+__device__ __forceinline__ void join_prefix(const AttnParams& p, int b, int t, int kvh, int g, int c, float& M, float& L, float4& acc) {
+  const PrefixParts& pp = p.parts;
+  const int4 mine = __ldcg(pp.rows + b);
+  if (mine.y < 0) return;
+  const long long r = ((long long)mine.y * p.T + t) * p.G + g, u = mine.x + (long long)kvh * mine.z + r / kUnitRows;
+  if (u < 0 || u >= pp.max_units) return;
+  const int4 unit = __ldcg(pp.units + u);
+  if (unit.x < 0 || unit.y < unit.x || unit.y >= pp.ctas) return;
+  const bool both = unit.z != 0;
+  const int rr = (int)(r % kUnitRows), parts = (unit.y - unit.x + 1) * (both ? 1 : 2);
+  const long long first = ((((long long)b * p.T + t) * p.hq) + kvh * p.G + g) * 2;
+  constexpr int N = 8;  // parts whose loads are in flight together
+  for (int i0 = 0; i0 < parts; i0 += N) {
+    float2 st[N];
+    float4 v[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      st[x] = make_float2(0.f, 0.f);
+      if (i0 + x < parts) {
+        const int k = both ? i0 + x : (i0 + x) >> 1, slot = both ? rr / kSlotRows : (i0 + x) & 1;
+        const long long at = k == 0 ? first + (both ? 0 : slot) : ((unit.x + k) * 2ll + slot) * kSlotRows + rr % kSlotRows;
+        st[x] = __ldcg((k == 0 ? pp.first_stats : pp.later_stats) + at);
+        v[x] = __ldcg(reinterpret_cast<const float4*>(k == 0 ? pp.first : pp.later) + at * (HD / 4) + c);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      if (st[x].y == 0.f) continue;  // no position seen
+      const float mn = fmaxf(M, st[x].x), a = ex2(M - mn), f = ex2(st[x].x - mn);
+      M = mn;
+      L = fmaf(L, a, f * st[x].y);
+      acc.x = fmaf(acc.x, a, f * v[x].x);
+      acc.y = fmaf(acc.y, a, f * v[x].y);
+      acc.z = fmaf(acc.z, a, f * v[x].z);
+      acc.w = fmaf(acc.w, a, f * v[x].w);
+    }
+  }
 }
 
 // Attended positions of sequence b by its last real token of row tile rt; 0 where the tile has none.
@@ -607,7 +647,7 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     }
     if (whole) {
       const int grow = sg.rt * RT + row, t = grow / p.G, g = grow - t * p.G;
-      if (SH && first_tile<SH>(p, sg.b, n) > 0) join_prefix<HD>(p, (long long)sg.b * p.T + t, sg.kvh * p.G + g, c, M, L, acc);
+      if (SH && first_tile<SH>(p, sg.b, n) > 0) join_prefix<HD>(p, sg.b, t, sg.kvh, g, c, M, L, acc);
       const float inv = L == 0.f ? 0.f : 1.f / L;
       uint16_t* dst = p.out + ((long long)sg.b * p.T + t) * p.ld_out + (long long)(sg.kvh * p.G + g) * HD + 4 * c;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -656,7 +696,7 @@ __device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg
       }
     }
     const int grow = sg.rt * RT + row, t = grow / p.G, g = grow - t * p.G;
-    if (SH && first_tile<SH>(p, sg.b, n) > 0) join_prefix<HD>(p, (long long)sg.b * p.T + t, sg.kvh * p.G + g, c, M, L, acc);
+    if (SH && first_tile<SH>(p, sg.b, n) > 0) join_prefix<HD>(p, sg.b, t, sg.kvh, g, c, M, L, acc);
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t* dst = p.out + ((long long)sg.b * p.T + t) * p.ld_out + (long long)(sg.kvh * p.G + g) * HD + 4 * c;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
