@@ -692,7 +692,7 @@ WAL_API int wal_kv8_attention_shared(const wal_kv8_cache* cache, int32_t layer, 
  * bias_ids int32 / bias fp32 [B][num_bias] or NULL; mask: int32 words
  * (sequences mask_seq, rows mask_row words apart, 0 to share them) or NULL.
  * Tokens outside [0, V) count nowhere.  Rows t >= new_lens[b] (NULL: T) are
- * zeros.  V <= 393216, num_bias <= 1024, B * T < 2^27.  out must not overlap logits.
+ * zeros.  V <= 393216, num_bias <= 1024, text_len < 2^20, B * T < 2^27.  out must not overlap logits.
  */
 typedef struct wal_logit_rules {
   const int32_t* text;

@@ -30,7 +30,7 @@ def _call(rules, **change):
 @pytest.mark.parametrize("change,want", [
     (dict(text=None), ARG), (dict(lens=None), ARG), (dict(bias=None), ARG), (dict(bias_ids=None), ARG),
     (dict(bias=None, bias_ids=None), ARG), (dict(num_bias=1025), SHAPE), (dict(num_bias=-1), SHAPE), (dict(ld_text=49), SHAPE),
-    (dict(text_len=-1), SHAPE), (dict(text_len=1 << 31, ld_text=1 << 31), SHAPE), (dict(mask_seq=-1), SHAPE), (dict(mask_row=-1), SHAPE)])
+    (dict(text_len=-1), SHAPE), (dict(text_len=1 << 20, ld_text=1 << 20), SHAPE), (dict(mask_seq=-1), SHAPE), (dict(mask_row=-1), SHAPE)])
 def test_rules_refused(change, want):
     assert _call(_rules(**change)) == want
 

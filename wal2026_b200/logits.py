@@ -20,6 +20,7 @@ from .kv8 import _call, _cuda, _i32, _on
 
 MAX_VOCAB = 393216
 MAX_BIAS = 1024
+MAX_TEXT = (1 << 20) - 1
 
 
 @dataclass
@@ -89,6 +90,8 @@ def logit_rules(logits: Tensor, out: Tensor, *, text: Optional[Tensor] = None, l
     if text is not None and (text.dtype != torch.int32 or text.dim() != 2 or text.shape[0] != B
                              or (text.stride(1) != 1 and text.shape[1] > 1)):
         raise ValueError("text must be int32 [B, L] with contiguous rows")
+    if text is not None and text.shape[1] > MAX_TEXT:
+        raise ValueError(f"logit_rules takes texts of at most {MAX_TEXT} tokens, got {text.shape[1]}")
     for name, t in (("lens", lens), ("prompt_lens", prompt_lens), ("new_lens", new_lens)):
         if t is not None:
             _i32(name, t, B)
