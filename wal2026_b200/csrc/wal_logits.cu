@@ -1,14 +1,17 @@
 // Rules on logits (penalties for repeated tokens, biases, masks, temperature) and
 // their softmax, for the T rows of each sequence that a step makes.
 //
-// A cluster of CTAs takes one row and each thread some groups of four entries of
-// it, in registers, so logits are read and outputs written once.  What the rules
+// A cluster of CTAs takes one row, dealt out in blocks of 128 entries (frequent
+// tokens have neighbouring numbers), and each thread some groups of four entries, in registers, so logits are read and outputs written once.  What the rules
 // know of an entry is a word in shared memory: how often the text has it, whether
 // the prompt does, and which bias it has; most words are zero and cost a test per
 // group.  Every CTA reads the text and counts what falls into its share while its
 // logits are on their way.  The CTAs exchange (maximum, sum) through distributed
 // shared memory once: entries are held as exp(x - the CTA's maximum), and the
-// factor to the cluster's maximum and sum is one number per CTA.
+// factor to the cluster's maximum and sum is one number per CTA.  Clusters that fill
+// the GPU take the rows in order: the T rows of a sequence need one count of the
+// text and then a token more each, and the next row's logits are asked into L2
+// while this one is worked on.
 //
 // Numerics: fp32 in the order of the definition.  The temperature goes into the
 // exponent: exp(x / t - m / t) = exp2(x k - m k), k = log2(e) / t, in one fused
@@ -19,7 +22,9 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace {
 
@@ -37,7 +42,8 @@ struct RulesParams {
   long long ld_seq, ld_row;
   float* out;
   long long out_seq, out_row;
-  int B, T, V, share;  // entries per CTA, a multiple of 4
+  int B, T, V, share;  // entries per CTA, a multiple of 128
+  int shift;           // log2 of the cluster's CTAs
   int softmax;
 };
 
@@ -91,51 +97,68 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
   __shared__ float adds[kMaxBias];
   __shared__ float wv[W], wsum[W];
   __shared__ int wi[W];
-  __shared__ float cmax[kMaxCluster], csum[kMaxCluster];
-  __shared__ int cidx[kMaxCluster];
+  // by the row's parity: what one CTA tells the others is read before any of them can be two rows further
+  __shared__ float cmax[2][kMaxCluster], csum[2][kMaxCluster];
+  __shared__ int cidx[2][kMaxCluster];
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), ncta = (int)cl.num_blocks();
-  const long long row = blockIdx.x / ncta;
-  const int b = (int)(row / p.T), t = (int)(row % p.T);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // entry i of this CTA is entry at(i) of the row; place(v) is where entry v is here, if it is
+  auto at = [&](int i) { return ((i >> 7 << p.shift) + rank) << 7 | (i & 127); };
+  auto place = [&](unsigned v) -> unsigned {
+    return v < (unsigned)p.V && ((v >> 7) & (unsigned)(ncta - 1)) == (unsigned)rank ? (v >> 7 >> p.shift) << 7 | (v & 127) : 0xffffffffu;
+  };
+  const int v0 = at(4 * tid), step = NT / 32 << p.shift << 7;  // this thread's group k starts at entry v0 + k * step
+  const bool counted = p.r.repetition || p.r.presence || p.r.frequency;
+  const int nb = (int)p.r.num_bias;
+  const int clusters = (int)gridDim.x / ncta, mine = (int)blockIdx.x / ncta, rows = p.B * p.T;
+  const int row0 = (int)((long long)rows * mine / clusters), row1 = (int)((long long)rows * (mine + 1) / clusters);
   wal_kv8::chain();
-  // a CTA's shared memory may be written by the others once it has started
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
-  const int v0 = min(rank * p.share, p.V), n = min(p.share, p.V - v0);
-  float* const out = p.out + b * p.out_seq + t * p.out_row + v0;
-  const bool idle = p.r.new_lens && t >= p.r.new_lens[b];
-  auto write = [&](int i, const float (&v)[4]) {
+  cl.sync();  // a CTA's shared memory may be written by the others once it has started
+  int held = -1, upto = 0;  // the sequence whose words are there, and how much of its text they count
+  for (int row = row0; row < row1; ++row) {
+  const int b = row / p.T, t = row - b * p.T, parity = row & 1;
+  float* const out = p.out + b * p.out_seq + t * p.out_row;
+  auto write = [&](int k, const float (&x)[4]) {
+    const int v = v0 + k * step;
     if (VEC) {
-      if (i < n) __stcs(reinterpret_cast<float4*>(out + i), make_float4(v[0], v[1], v[2], v[3]));
+      if (v < p.V) __stcs(reinterpret_cast<float4*>(out + v), make_float4(x[0], x[1], x[2], x[3]));
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < n) out[i + e] = v[e];
+        if (v + e < p.V) out[v + e] = x[e];
     }
   };
-  if (idle) {
+  if (p.r.new_lens && t >= p.r.new_lens[b]) {  // for all CTAs of the row
     const float none[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < K; ++k) write(4 * (tid + NT * k), none);
-    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
-    return;  // all CTAs of the row do
+    for (int k = 0; k < K; ++k) write(k, none);
+    continue;
   }
   float x[K][4];
-  const long long base = b * p.ld_seq + t * p.ld_row + v0;
+  const long long base = b * p.ld_seq + t * p.ld_row;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int i = 4 * (tid + NT * k);
+    const int v = v0 + k * step;
     if (VEC) {
-      const float4 f = i < n ? load4<DT>(p.logits, base + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float4 f = v < p.V ? load4<DT>(p.logits, base + v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       x[k][0] = f.x, x[k][1] = f.y, x[k][2] = f.z, x[k][3] = f.w;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = i + e < n ? load1<DT>(p.logits, base + i + e) : -INFINITY;
+      for (int e = 0; e < 4; ++e) x[k][e] = v + e < p.V ? load1<DT>(p.logits, base + v + e) : -INFINITY;
     }
   }
-  const bool counted = p.r.repetition || p.r.presence || p.r.frequency;
-  const int nb = (int)p.r.num_bias;
-  if (counted || nb) {
-    for (int i = tid; i < (n + 3) / 4; i += NT) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (row + 1 < row1) {
+    const int nb2 = (row + 1) / p.T, nt = row + 1 - nb2 * p.T;
+    constexpr int kLine = 128 / (DT == WAL_F32 ? 4 : 2);
+    const long long first = nb2 * p.ld_seq + nt * p.ld_row;
+    for (int i = kLine * tid; i < p.share && at(i) < p.V; i += kLine * NT) {
+      const char* line = static_cast<const char*>(p.logits) + (first + at(i)) * (DT == WAL_F32 ? 4 : 2);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+    }
+  }
+  if ((counted || nb) && held != b) {
+    __syncthreads();  // the words of the sequence before have been read
+    for (int i = tid; i < p.share / 4; i += NT) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
     for (int i = tid; i < nb; i += NT) {
       ids[i] = p.r.bias_ids[(long long)b * nb + i];
       adds[i] = p.r.bias[(long long)b * nb + i];
@@ -143,83 +166,109 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
     __syncthreads();
     if (counted) {
       const int* text = p.r.text + b * p.r.ld_text;
-      const int upto = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
+      upto = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
       const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
 #pragma unroll 4
       for (int j = tid; j < upto; j += NT) {
-        const unsigned at = (unsigned)text[j] - (unsigned)v0;
-        if (at < (unsigned)n) {
-          if (j < prompt) atomicOr(words + at, kPrompt);
-          else atomicAdd(words + at, 1u);
+        const unsigned w = place((unsigned)text[j]);
+        if (w != 0xffffffffu) {
+          if (j < prompt) atomicOr(words + w, kPrompt);
+          else atomicAdd(words + w, 1u);
         }
       }
     }
     float sum = 0.f;
     for (int i = tid; i < nb; i += NT) {
-      const unsigned at = (unsigned)ids[i] - (unsigned)v0;
-      if (at >= (unsigned)n) continue;
+      const unsigned w = place((unsigned)ids[i]);
+      if (w == 0xffffffffu) continue;
       bool first = true;
       for (int j = 0; j < i && first; ++j) first = ids[j] != ids[i];
       if (!first) continue;  // the first of equal ones adds them all, in order
       sum = adds[i];
       for (int j = i + 1; j < nb; ++j)
         if (ids[j] == ids[i]) sum += adds[j];
-      atomicOr(words + at, (unsigned)(i + 1) << kBiasBit);
+      atomicOr(words + w, (unsigned)(i + 1) << kBiasBit);
       if (sum != adds[i]) adds[i] = sum;  // no other thread reads the first one's
     }
+    held = b;
+    __syncthreads();
+  } else if (counted) {  // the row's own token, if the text has it
+    const int now = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
+    __syncthreads();
+    if (tid == 0 && now > upto) {
+      const unsigned w = place((unsigned)p.r.text[b * p.r.ld_text + now - 1]);
+      const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
+      if (w != 0xffffffffu) words[w] = now - 1 < prompt ? words[w] | kPrompt : words[w] + 1u;
+    }
+    upto = now;
     __syncthreads();
   }
   const float rep = p.r.repetition ? p.r.repetition[b] : 1.f, pres = p.r.presence ? p.r.presence[b] : 0.f;
   const float freq = p.r.frequency ? p.r.frequency[b] : 0.f, temp = p.r.temperature ? p.r.temperature[b] : 1.f;
   const bool greedy = !(temp > 0.f);
+  const float inv = 1.f / rep;
   const int* const mask = p.r.mask ? p.r.mask + b * p.r.mask_seq + t * p.r.mask_row : nullptr;
+  // a separate copy for the repetitions that have to be divided by
+  auto penalise = [&](auto divide) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = 4 * (tid + NT * k);
+      if (i >= p.share) break;
+      const uint4 c = *reinterpret_cast<const uint4*>(words + i);
+      const unsigned w[4] = {c.x, c.y, c.z, c.w}, any = c.x | c.y | c.z | c.w;
+      if (any == 0u) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = x[k][e] > 0.f ? (divide.value ? x[k][e] / rep : x[k][e] * inv) : x[k][e] * rep;
+        const float z = y - freq * (float)(w[e] & kCount) - pres;
+        x[k][e] = w[e] & kCount ? z : w[e] & kPrompt ? y : x[k][e];
+      }
+      if (any >> kBiasBit)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (w[e] >> kBiasBit) x[k][e] += adds[(w[e] >> kBiasBit) - 1];
+    }
+  };
+  if (counted || nb) {
+    if (rep >= 9.0949470177292824e-13f && rep <= 1.099511627776e12f) penalise(std::false_type{});
+    else penalise(std::true_type{});
+  }
+  if (mask) {
+    const int* const mine = mask + (v0 >> 5);  // groups of a thread have the same place in their words
+    unsigned bits[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) bits[k] = v0 + k * step < p.V ? (unsigned)__ldg(mine + k * (step >> 5)) >> (v0 & 31) : 0u;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] = (bits[k] >> e) & 1 ? x[k][e] : -INFINITY;
+  }
   float top = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = 4 * (tid + NT * k);
-    if ((counted || nb) && i < n) {
-      const uint4 c = *reinterpret_cast<const uint4*>(words + i);
-      if (c.x | c.y | c.z | c.w) {
-        const unsigned w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (w[e] & (kCount | kPrompt)) {
-            x[k][e] = x[k][e] > 0.f ? x[k][e] / rep : x[k][e] * rep;
-            if (w[e] & kCount) x[k][e] = x[k][e] - freq * (float)(w[e] & kCount) - pres;
-          }
-          if (w[e] >> kBiasBit) x[k][e] += adds[(w[e] >> kBiasBit) - 1];
-        }
-      }
-    }
-    if (mask) {
-      const unsigned bits = i < n ? (unsigned)__ldg(mask + ((v0 + i) >> 5)) >> ((v0 + i) & 31) : 0u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = (bits >> e) & 1 ? x[k][e] : -INFINITY;
-    }
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       x[k][e] = number(x[k][e]);
       top = fmaxf(top, x[k][e]);
     }
-  }
   if (!p.softmax) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!greedy && p.r.temperature)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[k][e] = number(x[k][e] / temp);
-      write(4 * (tid + NT * k), x[k]);
+      write(k, x[k]);
     }
-    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
-    return;
+    continue;
   }
   // this CTA's largest, and its sum relative to it
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) wv[warp] = top;
   __syncthreads();
+  top = wv[lane % W];
 #pragma unroll
-  for (int w = 0; w < W; ++w) top = fmaxf(top, wv[w]);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float scale = 1.4426950408889634f / temp, off = -top * scale;
   const bool usual = temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(off) < 1e30f;
   float sum = 0.f, ref = top;  // ref: what this CTA's entries are relative to, divided by the temperature
@@ -229,7 +278,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
     for (int k = K - 1; k >= 0; --k)
 #pragma unroll
       for (int e = 3; e >= 0; --e)
-        if (x[k][e] == top) where = v0 + 4 * (tid + NT * k) + e;
+        if (x[k][e] == top) where = v0 + k * step + e;
   } else if (usual) {
     ref = top / temp;
 #pragma unroll
@@ -258,32 +307,43 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
   }
   if (lane == 0) wsum[warp] = sum, wi[warp] = where;
   __syncthreads();
-  asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
-  if (tid < ncta) {
-    float s = 0.f;
-    int first = 0x7fffffff;
-    for (int w = 0; w < W; ++w) {
-      s += wsum[w];
-      first = min(first, wi[w]);
+  if (warp == 0) {
+    float total = lane < W ? wsum[lane] : 0.f;
+    int first = wi[lane % W];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
     }
-    *cl.map_shared_rank(&cmax[rank], tid) = ref;
-    *cl.map_shared_rank(&csum[rank], tid) = s;
-    *cl.map_shared_rank(&cidx[rank], tid) = first;
+    if (lane < ncta) {
+      *cl.map_shared_rank(&cmax[parity][rank], lane) = ref;
+      *cl.map_shared_rank(&csum[parity][rank], lane) = total;
+      *cl.map_shared_rank(&cidx[parity][rank], lane) = first;
+    }
   }
   cl.sync();
-  float all = -INFINITY, total = 0.f;
-  int best = 0x7fffffff;
-  for (int c = 0; c < ncta; ++c) better(all, best, cmax[c], cidx[c]);
-  for (int c = 0; c < ncta; ++c)
-    if (cmax[c] > -INFINITY) total += csum[c] * (cmax[c] == all ? 1.f : expf(cmax[c] - all));
+  // a lane per CTA (the lanes beyond repeat them): the cluster's largest, and its sum relative to it
+  const float its = cmax[parity][lane & (ncta - 1)];
+  float all = its;
+  int best = cidx[parity][lane & (ncta - 1)];
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
+  float total = lane < ncta && its > -INFINITY ? csum[parity][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const float factor = greedy || !(ref > -INFINITY) ? 0.f : (ref == all ? 1.f : expf(ref - all)) / total;
-  const int one = greedy && all > -INFINITY ? best - v0 : -1;
+  const int one = greedy && all > -INFINITY ? best : -1;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int i = 4 * (tid + NT * k);
+    if (factor == 0.f) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[k][e] = factor == 0.f ? (i + e == one ? 1.f : 0.f) : x[k][e] * factor;
-    write(i, x[k]);
+      for (int e = 0; e < 4; ++e) x[k][e] = v0 + k * step + e == one ? 1.f : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] *= factor;
+    }
+    write(k, x[k]);
+  }
   }
 }
 
@@ -298,7 +358,9 @@ int launch(const RulesParams& p, int cluster, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * NT * K * 4) != cudaSuccess) return WAL_ERR_CUDA;
     allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  return wal_kv8::launch_chain(kern, dim3((unsigned)(p.B * p.T * cluster)), NT, words ? p.share * 4 : 0, st, p, cluster);
+  // what eight GPCs of 16 to 18 SMs hold of clusters of eight
+  const int resident = std::max(1, 128 * (NT == 512 ? 2 : 1) / cluster);
+  return wal_kv8::launch_chain(kern, dim3((unsigned)(std::min(p.B * p.T, resident) * cluster)), NT, words ? p.share * 4 : 0, st, p, cluster);
 }
 
 // A thread holds as few groups as its CTA's share needs; shares beyond 16384 take twice the threads.
@@ -347,7 +409,8 @@ int wal_logit_rules_apply(const wal_logit_rules* rules, const void* logits, int 
   p.softmax = softmax;
   int cluster = 1;
   while (cluster < kMaxCluster && V > cluster * 2048) cluster *= 2;
-  p.share = (int)(((V + cluster - 1) / cluster + 31) & ~31);
+  p.share = (int)((V + 128 * cluster - 1) / (128 * cluster)) * 128;
+  p.shift = cluster == 8 ? 3 : cluster == 4 ? 2 : cluster == 2 ? 1 : 0;
   const bool vec = V % 4 == 0 && ld_row % 4 == 0 && ld_seq % 4 == 0 && out_row % 4 == 0 && out_seq % 4 == 0 &&
                    !((uintptr_t)logits & (4 * size - 1)) && !((uintptr_t)out & 15);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
