@@ -19,7 +19,9 @@ with one all-reduce each; the lm_head is split by vocabulary rows and its
 logits all-gathered.  Block boundaries (d = 8) divide every split.
 
 A ``DenseLlama`` twin with bf16 ``F.linear`` projections (cuBLAS) runs the same
-glue code, so the two decode rates differ only in the linears.
+glue code, so the two decode rates differ only in the linears; ``int4_llama``
+is that twin with 4-bit projections.  ``LlamaStack.quantize_head`` replaces the
+vocabulary projection of any of them by a 4-bit one.
 """
 from __future__ import annotations
 
@@ -32,6 +34,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from .decode_ops import decode_attention, decode_attention_workspace, residual_rmsnorm, rope_kv_append, silu_mul
+from .int4 import Int4Linear
 from .runtime import PackedGroupedBlockRVQLinear
 from .tp import COLUMN, ROW, shard_bounds, shard_packed
 
@@ -110,7 +113,7 @@ class DecoderLayer(nn.Module):
     def _row_parallel(self, lin: nn.Module, x: Tensor) -> Tensor:
         if self.tp.size == 1:
             return lin(x)
-        if isinstance(lin, PackedGroupedBlockRVQLinear):  # fp32 partial straight from the GEMV
+        if isinstance(lin, (PackedGroupedBlockRVQLinear, Int4Linear)):  # fp32 partial straight from the GEMV
             y = torch.empty((x.shape[0], lin.out_features), device=x.device, dtype=torch.float32)
             lin.gemv_into(x, y)
         else:
@@ -198,7 +201,19 @@ class LlamaStack(nn.Module):
         self.k_cache: list[Tensor] = []
         self.v_cache: list[Tensor] = []
         self.exchange = None  # PeerExchange for exchange="push"
+        self.head: Optional[Int4Linear] = None  # in place of lm_head, from quantize_head()
         self._bufs: dict[int, _DecodeBuffers] = {}
+
+    def quantize_head(self, group_size: int = 128, *, zero_points: bool = False) -> None:
+        """Compute logits from a 4-bit copy of this rank's lm_head (nearest codes, a scale per group of columns).
+
+        The dense lm_head stays where it was (it may be the embedding); ``self.head = None`` returns to it.
+        """
+        self.head = Int4Linear.from_dense(self.lm_head, group_size, zero_points=zero_points)
+
+    def logits(self, x: Tensor) -> Tensor:
+        """Logits [M, vocab] (bf16) of normed hidden rows x [M, hidden], gathered over the ranks."""
+        return self.tp.all_gather_last(F.linear(x, self.lm_head) if self.head is None else self.head(x))
 
     def allocate_cache(self, batch: int, max_len: int, *, fill_random: bool = True, seed: int = 1,
                        consistent: bool = False) -> None:
@@ -239,8 +254,7 @@ class LlamaStack(nn.Module):
         for layer, kc, vc in zip(self.layers, self.k_cache, self.v_cache):
             h = layer(h, cos, sin, kc, vc, pos)
         h = F.rms_norm(h, (self.shape.hidden,), self.final_norm, self.shape.eps)
-        logits = F.linear(h, self.lm_head)
-        return self.tp.all_gather_last(logits)
+        return self.logits(h)
 
     def enable_push_exchange(self, max_batch: int) -> None:
         """Create the peer-memory exchange used by ``decode_step_fused(exchange="push")``."""
@@ -267,11 +281,11 @@ class LlamaStack(nn.Module):
             if isinstance(lin, PackedGroupedBlockRVQLinear):
                 self.exchange.push_gemv(lin, a, slot)  # the GEMV's epilogue stores the tagged words
             else:
-                torch.matmul(a, lin.weight.t(), out=bufs.ybf)
+                _linear_into(lin, a, bufs.ybf)
                 self.exchange.push_rows(bufs.ybf, slot)
             self.exchange.reduce_residual_norm(slot, bufs.h, norm_w, eps, bufs.x)
             return
-        if isinstance(lin, PackedGroupedBlockRVQLinear):
+        if isinstance(lin, (PackedGroupedBlockRVQLinear, Int4Linear)):
             lin.gemv_into(a, bufs.y32)
         else:
             bufs.y32.copy_(F.linear(a, lin.weight))
@@ -305,14 +319,15 @@ class LlamaStack(nn.Module):
             silu_mul(bufs.gu, bufs.act)
             nxt = self.layers[i + 1].in_norm if i + 1 < n else self.final_norm
             self._row_parallel_fused(layer.down, bufs.act, 2 * i + 1, nxt, bufs, exchange)
-        logits = F.linear(bufs.x, self.lm_head)
-        return self.tp.all_gather_last(logits)
+        return self.logits(bufs.x)
 
     def linear_bytes(self) -> int:
         """Bytes of the projection weights a decode step streams (packed or dense)."""
         total = 0
         for m in self.modules():
-            if isinstance(m, PackedGroupedBlockRVQLinear):
+            if m is self.head:  # not a projection
+                continue
+            if isinstance(m, (PackedGroupedBlockRVQLinear, Int4Linear)):
                 total += m.compressed_bytes()
             elif isinstance(m, DenseLinear):
                 total += m.weight.numel() * 2
@@ -320,7 +335,7 @@ class LlamaStack(nn.Module):
 
 
 def _linear_into(lin: nn.Module, x: Tensor, y: Tensor) -> None:
-    if isinstance(lin, PackedGroupedBlockRVQLinear):
+    if isinstance(lin, (PackedGroupedBlockRVQLinear, Int4Linear)):
         lin.gemv_into(x, y)
     else:
         torch.matmul(x, lin.weight.t(), out=y)
@@ -379,6 +394,20 @@ def dense_llama(shape: LlamaShape, *, device="cuda", seed: int = 0, tp: Optional
     def make(rows: list[int], k: int, mode: str) -> nn.Module:
         w = (torch.randn(int(sum(rows)), k, device=device, generator=gen) * 0.02).to(torch.bfloat16)
         return DenseLinear(_shard_rows_cols(w, rows, mode, ctx))
+
+    return LlamaStack(shape, make, device=device, seed=seed, tp=ctx)
+
+
+def int4_llama(shape: LlamaShape, *, group_size: int = 128, zero_points: bool = False, device="cuda", seed: int = 0,
+               tp: Optional[TPContext] = None) -> LlamaStack:
+    """The stack of ``dense_llama`` (same seed, same weights) with 4-bit projections; the head stays dense."""
+    device = torch.device(device)
+    gen = torch.Generator(device=device).manual_seed(int(seed) + 2000)
+    ctx = tp or TPContext()
+
+    def make(rows: list[int], k: int, mode: str) -> nn.Module:
+        w = (torch.randn(int(sum(rows)), k, device=device, generator=gen) * 0.02).to(torch.bfloat16)
+        return Int4Linear.from_dense(_shard_rows_cols(w, rows, mode, ctx), group_size, zero_points=zero_points)
 
     return LlamaStack(shape, make, device=device, seed=seed, tp=ctx)
 

@@ -13,6 +13,11 @@ without waiting for the host and can be captured into a CUDA graph:
     accepted, out = dec.speculate(drafts, uniforms, last=tokens, temperature=0.8)
     dec.fork([0, 0])                              # both rows continue sequence 0
 
+With ``share`` the attention reads what forked rows have in common once for all
+of them; with ``text`` the decoder keeps the rows' tokens, which the penalties of
+``LogitRules`` need (``speculate(..., rules=rules)``, or ``logit_rules`` on the
+logits of a step).
+
 ``python -m wal2026_b200.paged_decode`` runs a small random stack that way.
 """
 from __future__ import annotations
@@ -20,13 +25,13 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
-import torch.nn.functional as F
 from torch import Tensor
 
 from .decode_ops import residual_rmsnorm, silu_mul
-from .kv8 import (PagedKV8Cache, kv8_append, kv8_attention, kv8_attention_workspace, kv_pages_assign, kv_pages_compact,
-                  kv_pages_copy)
+from .kv8 import (PagedKV8Cache, kv8_append, kv8_attention, kv8_attention_shared, kv8_attention_shared_workspace,
+                  kv8_attention_workspace, kv_pages_assign, kv_pages_compact, kv_pages_copy, kv_pages_groups)
 from .llama import LlamaStack, _linear_into
+from .logits import MAX_TEXT, LogitRules, logit_rules
 from .runtime import PREFILL_MIN_TOKENS, PackedGroupedBlockRVQLinear
 from .speculative import verify_drafts
 
@@ -34,7 +39,7 @@ from .speculative import verify_drafts
 class _StepBuffers:
     """Activations of steps of up to ``tokens`` tokens per row, and the attention's workspace."""
 
-    def __init__(self, stack: LlamaStack, rows: int, tokens: int, cache: PagedKV8Cache):
+    def __init__(self, stack: LlamaStack, rows: int, tokens: int, cache: PagedKV8Cache, shared: bool):
         s, l0, dev, bf = stack.shape, stack.layers[0], stack.embed.device, torch.bfloat16
         M, hd = rows * tokens, s.head_dim
         self.tokens = tokens
@@ -46,7 +51,7 @@ class _StepBuffers:
         self.gu = torch.empty(M, 2 * l0.mlp, device=dev, dtype=bf)
         self.act = torch.empty(M, l0.mlp, device=dev, dtype=bf)
         self.y32 = torch.empty(M, s.hidden, device=dev, dtype=torch.float32)
-        self.ws = kv8_attention_workspace(cache, rows, l0.hq, tokens)
+        self.ws = (kv8_attention_shared_workspace if shared else kv8_attention_workspace)(cache, rows, l0.hq, tokens)
 
     def first(self, M: int) -> "_StepBuffers":
         """The same buffers for a step of M token rows."""
@@ -81,12 +86,20 @@ class PagedDecoder:
     ``missing`` int64 [1] sums such pages over all steps, so that a loop which
     never waits for the device can look now and then: 0 means that every step
     was carried out.
+
+    share: rows whose first ``share`` positions (or more) lie in the same pages are
+    a group, whose common positions each step reads once (``kv_pages_groups``);
+    None: every row reads its own.  text: keep the rows' tokens in ``text`` int32
+    [rows, max_len], by position; ``prompt_lens`` int32 [rows] (0 to begin with, the
+    caller's to set) says where what the rows generated starts.
     """
 
     def __init__(self, stack: LlamaStack, rows: int, max_len: int, *, num_pages: Optional[int] = None,
-                 page_size: int = 64, dtype: torch.dtype = torch.int8):
+                 page_size: int = 64, dtype: torch.dtype = torch.int8, share: Optional[int] = None, text: bool = False):
         if rows < 1 or max_len < 1:
             raise ValueError("rows and max_len must be positive")
+        if share is not None and share < 1:
+            raise ValueError("share must be positive, or None")
         dev, l0 = stack.embed.device, stack.layers[0]
         width = -(-max_len // page_size)
         self.stack, self.rows, self.max_len = stack, rows, width * page_size
@@ -103,6 +116,14 @@ class PagedDecoder:
         self._zero = torch.zeros(rows, **i32)
         self._ref = torch.empty(self.cache.num_pages, **i32)
         self._src, self._dst = torch.empty(rows, **i32), torch.empty(rows, **i32)
+        self.share = share
+        self.groups = None if share is None else torch.zeros(4, rows, **i32)
+        self.text = self.prompt_lens = None
+        if text:
+            if self.max_len > MAX_TEXT:
+                raise ValueError(f"a decoder keeps texts of at most {MAX_TEXT} tokens, max_len is {self.max_len}")
+            self._text = torch.zeros(rows, self.max_len + 1, **i32)  # the last place takes tokens that are not kept
+            self.text, self.prompt_lens = self._text[:, :self.max_len], torch.zeros(rows, **i32)
         ang = torch.arange(self.max_len, device=dev, dtype=torch.float32)[:, None] * stack.inv_freq
         self.cos, self.sin = ang.cos().contiguous(), ang.sin().contiguous()
         self._bufs: Optional[_StepBuffers] = None  # of the largest step so far
@@ -118,14 +139,14 @@ class PagedDecoder:
         capturing = torch.cuda.is_current_stream_capturing()
         if self._bufs is None or self._bufs.tokens < T:
             if capturing:
-                self._captured.append(_StepBuffers(self.stack, self.rows, T, self.cache))
+                self._captured.append(_StepBuffers(self.stack, self.rows, T, self.cache, self.share is not None))
                 return self._captured[-1]
             if self._bufs is not None:
                 for t in vars(self._bufs).values():
                     if isinstance(t, Tensor):
                         t.record_stream(torch.cuda.current_stream(t.device))
             self._bufs, self._views = None, {}
-            self._bufs = _StepBuffers(self.stack, self.rows, T, self.cache)
+            self._bufs = _StepBuffers(self.stack, self.rows, T, self.cache, self.share is not None)
         if capturing and not any(b is self._bufs for b in self._captured):
             self._captured.append(self._bufs)
         view = self._views.get(T)
@@ -165,6 +186,12 @@ class PagedDecoder:
         st, s = self.stack, self.stack.shape
         bufs = self._buffers(T)
         add = self._reserve(torch.full_like(self.lens, T) if new_lens is None else new_lens)
+        if self.share is not None:  # the table as it is now serves all layers
+            kv_pages_groups(self.table, self.lens, self.cache.page_size, self.groups, least=self.share)
+        if self.text is not None:
+            t = torch.arange(T, device=self.lens.device)
+            at = torch.where(t < add[:, None], self.lens[:, None] + t, self.max_len)
+            self._text.scatter_(1, at.long(), tokens.to(torch.int32))
         torch.index_select(st.embed, 0, tokens.reshape(-1), out=bufs.h)
         residual_rmsnorm(bufs.h, st.layers[0].in_norm, s.eps, bufs.x)
         n = len(st.layers)
@@ -172,13 +199,15 @@ class PagedDecoder:
             _column(layer.qkv, bufs.x, bufs.qkv)
             kv8_append(self.cache, i, bufs.qkv, layer.hq, self.table, self.lens, bufs.q, cos=self.cos, sin=self.sin,
                        new_lens=add)
-            kv8_attention(self.cache, i, bufs.q, self.table, self.lens, bufs.attn, bufs.ws, new_lens=add)
+            if self.share is None:
+                kv8_attention(self.cache, i, bufs.q, self.table, self.lens, bufs.attn, bufs.ws, new_lens=add)
+            else:
+                kv8_attention_shared(self.cache, i, bufs.q, self.table, self.lens, self.groups, bufs.attn, bufs.ws, new_lens=add)
             self._row_parallel(layer.o, bufs.attn, layer.post_norm, bufs)
             _column(layer.gate_up, bufs.x, bufs.gu)
             silu_mul(bufs.gu, bufs.act)
             self._row_parallel(layer.down, bufs.act, st.layers[i + 1].in_norm if i + 1 < n else st.final_norm, bufs)
-        logits = F.linear(bufs.x, st.lm_head)
-        return st.tp.all_gather_last(logits).view(B, T, -1)
+        return st.logits(bufs.x).view(B, T, -1)
 
     def _row_parallel(self, lin, a: Tensor, norm_w: Tensor, bufs: _StepBuffers) -> None:
         if (isinstance(lin, PackedGroupedBlockRVQLinear) and a.shape[0] >= PREFILL_MIN_TOKENS
@@ -195,7 +224,8 @@ class PagedDecoder:
 
     @torch.no_grad()
     def speculate(self, drafts: Tensor, uniforms: Tensor, *, last: Tensor, draft_probs: Optional[Tensor] = None,
-                  temperature: float = 1.0, draft_lens: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+                  temperature: float = 1.0, draft_lens: Optional[Tensor] = None,
+                  rules: Optional[LogitRules] = None) -> tuple[Tensor, Tensor]:
         """One speculative step: run the rows' last tokens and their drafts, keep what the stack's probabilities allow.
 
         last: int32 [rows], each row's newest token (not stored yet); drafts:
@@ -207,15 +237,30 @@ class PagedDecoder:
         [rows], tokens [rows, T + 1]: the kept drafts, the drawn token, -1); the
         last token and the kept drafts stay in the cache, and the drawn token is
         the next call's ``last``.  A step that finds no room is one in which no
-        row takes part.
+        row takes part.  rules: penalties, biases, masks and temperatures of the rows
+        (``logit_rules``; penalties need a decoder with ``text``); their temperatures
+        take the place of ``temperature``.
         """
         B, T = drafts.shape
+        if rules is not None and rules.penalises() and self.text is None:
+            raise ValueError("penalties need a decoder that keeps its text (text=True)")
         tokens = torch.cat([last.view(B, 1), drafts], dim=1)
         news = torch.full_like(self.lens, T + 1) if draft_lens is None else (draft_lens + 1).to(torch.int32)
-        logits = self.step(tokens.clamp(0, self.stack.shape.vocab - 1), news).float()  # a draft outside is refused below
-        if temperature > 0:
+        logits = self.step(tokens.clamp(0, self.stack.shape.vocab - 1), news)  # a draft outside is refused below
+        if rules is not None:
+            heat = rules.temperature
+            if heat is None and temperature != 1.0:
+                heat = torch.full((B,), float(temperature), device=logits.device)
+            mask = rules.mask if rules.mask is None else rules.mask.expand(B, T + 1, -1)
+            target = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+            logit_rules(logits, target, text=self.text, lens=self.lens, prompt_lens=self.prompt_lens, new_lens=news,
+                        repetition=rules.repetition, presence=rules.presence, frequency=rules.frequency,
+                        bias_ids=rules.bias_ids, bias=rules.bias, mask=mask, temperature=heat)
+        elif temperature > 0:
+            logits = logits.float()
             target = torch.softmax(logits / temperature, dim=-1)
         else:
+            logits = logits.float()
             target = torch.zeros_like(logits).scatter_(2, logits.argmax(-1, keepdim=True), 1.0)
         accepted = torch.empty(B, dtype=torch.int32, device=drafts.device)
         out = torch.empty(B, T + 1, dtype=torch.int32, device=drafts.device)
@@ -237,6 +282,10 @@ class PagedDecoder:
         self._assign(p, lens, self._zero)  # wants no page
         self.table.copy_(self._next)
         self.lens.copy_(lens)
+        if self.text is not None:
+            i = p.clamp(min=0).long()
+            self._text.copy_(self._text[i])
+            self.prompt_lens.copy_(torch.where(p >= 0, self.prompt_lens[i], 0))
 
     def compact(self) -> None:
         """Move the used pages to the front of the pool (``info``: used pages, moves)."""
