@@ -721,7 +721,7 @@ WAL_API int wal_logit_rules_apply(const wal_logit_rules* rules, const void* logi
  * over groups of group_size (32, 64 or 128) consecutive columns; codes c in
  * 0..15, z in 0..15 or 8 everywhere (zeros NULL), s fp16.  Weights enter the
  * products as the whole numbers c - z and sums are fp32, scaled once per group
- * (or per 64 columns of one): nothing is rounded but x's own type and y.
+ * (or per 64 columns of one): nothing is rounded but y.
  *
  * Packed: tiles of 16 rows (the last one filled up), each [ceil(K / 64)][32]
  * 16-byte pieces.  Word w < 4 of piece 4 r + q of a 64-column chunk holds the

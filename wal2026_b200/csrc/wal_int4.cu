@@ -10,11 +10,14 @@
 // instruction (the code in the low bits of 128 as bf16, of 1024 as f16) and an exact
 // subtraction of 128 + z or 1024 + z, so the products see whole numbers; a group's
 // fp32 sum is scaled once.  The order of k inside a product is free: a lane's
-// columns are chosen so that its activations are two 16-byte loads (they hit L1).
+// columns are chosen so that its activations are two 16-byte loads.
 //
-// Split.  A warp takes one or two row tiles (two from 9 tokens on, which halves
-// the activation reads per weight) and every ks-th chunk of 64 columns; the ks
-// warps of a tile meet in shared memory and are summed in order, so results do
+// Split.  CTAs that fill the GPU twice take groups of row tiles in turn, and keep
+// the activations in shared memory for all of them, rows 64 bytes out of step so
+// that the matrix fragments meet no bank twice; where they do not fit they are read
+// through L1.  A warp takes a row tile and every ks-th chunk of 64
+// columns, loading the next chunks, the next group's first ones among them, while
+// it multiplies.  What the ks warps have of a tile is added in order, so results do
 // not depend on timing.
 #include "wal_kv8.cuh"
 
@@ -22,26 +25,13 @@
 
 namespace {
 
+using wal_kv8::kMaxDevices;
 using wal_kv8::launch_chain;
 using wal_kv8::sm_count;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kAhead = 4;  // chunks loaded together
-
-struct Int4Params {
-  const uint4* packed;    // [tiles][chunks][32]
-  const uint32_t* scales; // [tiles][groups][8] pairs of rows r, r + 8
-  const uint16_t* zeros;  // likewise, bytes
-  const uint16_t* bias;
-  const uint16_t* x;
-  void* y;
-  long long ldx, ldy;
-  int M, N, K, tiles, chunks, groups;
-  int per;  // chunks per group as a shift (0 or 1)
-  int ks;   // warps that share a tile
-  int y_dtype;
-};
 
 template <bool F16>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -65,13 +55,39 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
 
 // 128 (bf16) or 1024 (f16) twice; a code in the low bits adds itself
 template <bool F16>
-__device__ __forceinline__ constexpr uint32_t magic() { return F16 ? 0x64006400u : 0x43004300u; }
+__host__ __device__ __forceinline__ constexpr uint32_t magic() { return F16 ? 0x64006400u : 0x43004300u; }
+
+// Passed as a parameter: a logic instruction takes one immediate, and two known constants cost a move each time.
+struct Masks {
+  uint32_t nibbles = 0x000f000fu, bf16 = magic<false>(), f16 = magic<true>();
+};
+
+struct Int4Params {
+  const uint4* packed;    // [tiles][chunks][32]
+  const uint32_t* scales; // [tiles][groups][8] pairs of rows r, r + 8
+  const uint16_t* zeros;  // likewise, bytes
+  const uint16_t* bias;
+  const uint16_t* x;
+  void* y;
+  long long ldx, ldy;
+  int M, N, K, tiles, chunks, groups;
+  int per;  // chunks per group as a shift (0 or 1)
+  int ks;   // warps that share a tile
+  int stride;        // bytes between activation rows in shared memory
+  int f16;           // activations
+  Masks masks;
+  int y_dtype;
+};
 
 // A fragment of one product from a word: rows r (registers 0, 2) and r + 8 (1, 3), minus their zero points.
 template <bool F16>
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+__device__ __forceinline__ void unpack(const Masks& k, uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a[i] = sub2<F16>(((w >> (4 * i)) & 0x000f000fu) | magic<F16>(), i & 1 ? z1 : z0);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;  // (w >> 4 i & nibbles) | magic
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * i)), "r"(k.nibbles), "r"(F16 ? k.f16 : k.bf16));
+    a[i] = sub2<F16>(v, i & 1 ? z1 : z0);
+  }
 }
 
 __device__ __forceinline__ uint4 load_codes(const uint4* p) {
@@ -86,70 +102,94 @@ __device__ __forceinline__ void store(void* y, int dtype, long long at, float v)
   else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
 }
 
-// NT: tiles of eight tokens, RT: row tiles per warp, GPC: groups in a chunk of 64 columns (1 or 2)
-template <int NT, int RT, int GPC, bool F16, bool ZEROS>
-__global__ void __launch_bounds__(kThreads) int4_gemv_kernel(const __grid_constant__ Int4Params p) {
+// NT: tiles of eight tokens, GPC: groups in a chunk of 64 columns (1 or 2), F16: activations, STAGED: they are
+// in shared memory
+template <int NT, int GPC, bool F16, bool ZEROS, bool STAGED>
+__global__ void __launch_bounds__(kThreads, 2) int4_gemv_kernel(const __grid_constant__ Int4Params p) {
   constexpr int LDR = 8 * NT + 1;
-  __shared__ float red[kWarps][RT * 16][LDR];
+  __shared__ float red[kWarps][16][LDR];
+  extern __shared__ __align__(16) uint8_t xs[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, q = lane & 3;
-  const int own = kWarps / p.ks;  // row-tile groups of this CTA
-  const int tile0 = ((int)blockIdx.x * own + warp / p.ks) * RT, kslice = warp % p.ks;
+  const int own = kWarps / p.ks, groups = (p.tiles + own - 1) / own;  // row tiles of a group, and groups
+  const int step = (int)gridDim.x, part = (int)blockIdx.x, chunks = p.chunks;
+  const int wtile = warp / p.ks, kslice = warp % p.ks;
+  const Masks masks = p.masks;
 
   struct Batch {
-    uint4 w[kAhead][RT];
-    uint32_t s[kAhead][RT][GPC];
-    uint16_t z[kAhead][RT][ZEROS ? GPC : 1];
+    uint4 w[kAhead];
+    uint32_t s[kAhead][GPC];
+    uint16_t z[kAhead][ZEROS ? GPC : 1];
   };
-  auto fetch = [&](Batch& b, int c0) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int c = c0 + i * p.ks, tile = tile0 + t;
-        const bool real = c < p.chunks && tile < p.tiles;
-        b.w[i][t] = real ? load_codes(p.packed + ((long long)tile * p.chunks + c) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int g = 0; g < GPC; ++g) {
-          const int gi = GPC == 2 ? min(2 * c + g, p.groups - 1) : c >> p.per;
-          const long long at = ((long long)tile * p.groups + gi) * 8 + r;
-          b.s[i][t][g] = real ? __ldg(p.scales + at) : 0u;
-          if (ZEROS) b.z[i][t][g] = real ? __ldg(p.zeros + at) : (uint16_t)0;
-        }
-      }
+  // where a group's row tile of this warp begins: codes, scales and zeros of row r; a tile past the last one reads the last
+  // one's (its rows are not written)
+  struct Place {
+    const uint4* w;
+    const uint32_t* s;
+    const uint16_t* z;
   };
-
-  float tot[RT][NT][4];
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) tot[t][n][0] = tot[t][n][1] = tot[t][n][2] = tot[t][n][3] = 0.f;
-
-  Batch cur;
-  fetch(cur, kslice);  // weights do not depend on the kernels before this one
-  wal_kv8::chain();
-  for (int c0 = kslice; c0 < p.chunks; c0 += kAhead * p.ks) {
-    Batch next;
-    fetch(next, c0 + kAhead * p.ks);
+  auto place = [&](int group) {
+    const long long tile = min(group * own + wtile, p.tiles - 1);
+    return Place{p.packed + tile * p.chunks * 32 + lane, p.scales + tile * p.groups * 8 + r, ZEROS ? p.zeros + tile * p.groups * 8 + r : nullptr};
+  };
+  auto fetch = [&](Batch& b, const Place& l, int c0) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int c = c0 + i * p.ks;
-      if (c >= p.chunks) break;
-      uint32_t xw[NT][2][4];  // columns 32 h + 8 q .. + 7 of token 8 n + r
+      const int c = min(c0 + i * p.ks, chunks - 1);  // past the end: the last chunk's again, which nothing multiplies
+      b.w[i] = load_codes(l.w + c * 32);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int g = 0; g < GPC; ++g) {
+        const int gi = GPC == 2 ? min(2 * c + g, p.groups - 1) : c >> p.per;
+        b.s[i][g] = __ldg(l.s + gi * 8);
+        if (ZEROS) b.z[i][g] = __ldg(l.z + gi * 8);
+      }
+    }
+  };
+
+  Batch cur;
+  Place here = place(part);
+  fetch(cur, here, kslice);  // weights do not depend on the kernels before this one
+  wal_kv8::chain();
+  if (STAGED) {
+    for (int row = warp; row < p.M; row += kWarps) {
+      const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
+      for (int i = lane; i < chunks * 8; i += 32)  // zeros past K
+        *reinterpret_cast<uint4*>(xs + row * p.stride + 16 * i) = i < p.K / 8 ? __ldg(from + i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncthreads();
+  }
+  // this lane's activations of chunk 0, tokens r, r + 8, ..
+  const uint8_t* const xl = STAGED ? xs + r * p.stride + 16 * q : reinterpret_cast<const uint8_t*>(p.x + r * p.ldx) + 16 * q;
+  const long long xrows = STAGED ? 8ll * p.stride : 16 * p.ldx;  // bytes between them
+
+  for (int group = part; group < groups; group += step) {
+    float tot[NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = 64 * c + 32 * h + 8 * q;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (8 * n + r < p.M && k < p.K) v = __ldg(reinterpret_cast<const uint4*>(p.x + (8 * n + r) * p.ldx + k));
-          xw[n][h][0] = v.x;
-          xw[n][h][1] = v.y;
-          xw[n][h][2] = v.z;
-          xw[n][h][3] = v.w;
-        }
+    for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.f;
+    for (int c0 = kslice; c0 < chunks; c0 += kAhead * p.ks) {
+      Batch next;
+      const bool more = c0 + kAhead * p.ks < chunks;
+      if (!more) here = place(min(group + step, groups - 1));
+      fetch(next, here, more ? c0 + kAhead * p.ks : kslice);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const uint32_t w[4] = {cur.w[i][t].x, cur.w[i][t].y, cur.w[i][t].z, cur.w[i][t].w};
+      for (int i = 0; i < kAhead; ++i) {
+        const int c = c0 + i * p.ks;
+        if (c >= chunks) break;
+        uint32_t xw[NT][2][4];  // columns 32 h + 8 q .. + 7 of token 8 n + r
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (8 * n + r < p.M && (STAGED || 64 * c + 32 * h + 8 * q < p.K)) {
+              const uint4* from = reinterpret_cast<const uint4*>(xl + n * xrows + 128 * c + 64 * h);
+              v = STAGED ? *from : __ldg(from);
+            }
+            xw[n][h][0] = v.x;
+            xw[n][h][1] = v.y;
+            xw[n][h][2] = v.z;
+            xw[n][h][3] = v.w;
+          }
+        const uint32_t w[4] = {cur.w[i].x, cur.w[i].y, cur.w[i].z, cur.w[i].w};
         float acc[NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -159,50 +199,51 @@ __global__ void __launch_bounds__(kThreads) int4_gemv_kernel(const __grid_consta
             for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
           uint32_t z0 = F16 ? 0x64086408u : 0x43084308u, z1 = z0;
           if (ZEROS) {
-            const uint32_t z = cur.z[i][t][g];
+            const uint32_t z = cur.z[i][g];
             z0 = (z & 0xffu) * 0x00010001u + magic<F16>();
             z1 = (z >> 8) * 0x00010001u + magic<F16>();
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t a[4];
-            unpack<F16>(w[2 * h + e], z0, z1, a);
+            unpack<F16>(masks, w[2 * h + e], z0, z1, a);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma<F16>(acc[n], a, xw[n][h][2 * e], xw[n][h][2 * e + 1]);
           }
           if (h == 1 || GPC == 2) {
-            const uint32_t sc = cur.s[i][t][g];
-            const float s0 = __half2float(__ushort_as_half((unsigned short)(sc & 0xffffu))), s1 = __half2float(__ushort_as_half((unsigned short)(sc >> 16)));
+            const uint32_t sc = cur.s[i][g];
+            const float s0 = __half2float(__ushort_as_half((unsigned short)(sc & 0xffffu)));
+            const float s1 = __half2float(__ushort_as_half((unsigned short)(sc >> 16)));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              tot[t][n][0] = fmaf(s0, acc[n][0], tot[t][n][0]);
-              tot[t][n][1] = fmaf(s0, acc[n][1], tot[t][n][1]);
-              tot[t][n][2] = fmaf(s1, acc[n][2], tot[t][n][2]);
-              tot[t][n][3] = fmaf(s1, acc[n][3], tot[t][n][3]);
+              tot[n][0] = fmaf(s0, acc[n][0], tot[n][0]);
+              tot[n][1] = fmaf(s0, acc[n][1], tot[n][1]);
+              tot[n][2] = fmaf(s1, acc[n][2], tot[n][2]);
+              tot[n][3] = fmaf(s1, acc[n][3], tot[n][3]);
             }
           }
         }
       }
+      cur = next;
     }
-    cur = next;
-  }
 
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
+    // the warps' sums
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][16 * t + r + 8 * (e >> 1)][8 * n + 2 * q + (e & 1)] = tot[t][n][e];
-  __syncthreads();
-  const int rows = own * RT * 16, m = min(p.M, 8 * NT);
-  for (int i = tid; i < rows * m; i += kThreads) {
-    const int row = i % rows, tok = i / rows, grp = row / (RT * 16), rr = row % (RT * 16);
-    const long long n = ((long long)blockIdx.x * own + grp) * RT * 16 + rr;
-    if (n >= p.N) continue;
-    float v = 0.f;
-    for (int k = 0; k < p.ks; ++k) v += red[grp * p.ks + k][rr][tok];
-    if (p.bias) v += __uint_as_float((uint32_t)p.bias[n] << 16);
-    store(p.y, p.y_dtype, tok * p.ldy + n, v);
+      for (int e = 0; e < 4; ++e) red[warp][r + 8 * (e >> 1)][8 * n + 2 * q + (e & 1)] = tot[n][e];
+    __syncthreads();
+    const int rows = own * 16;
+    for (int i = tid; i < rows * p.M; i += kThreads) {
+      const int row = i % rows, tok = i / rows;
+      const long long n = (long long)group * rows + row;
+      if (n >= p.N) continue;
+      float v = 0.f;
+      for (int k = 0; k < p.ks; ++k) v += red[(row >> 4) * p.ks + k][row & 15][tok];
+      if (p.bias) v += __uint_as_float((uint32_t)p.bias[n] << 16);
+      store(p.y, p.y_dtype, tok * p.ldy + n, v);
+    }
+    __syncthreads();
   }
 }
 
@@ -256,18 +297,50 @@ int check_layer(const wal_int4_layer* l) {
   return WAL_OK;
 }
 
-template <int NT, int RT>
-int launch(const Int4Params& p, int gpc, bool f16, cudaStream_t st) {
-  const int own = kWarps / p.ks;
-  const dim3 grid((unsigned)((p.tiles + own * RT - 1) / (own * RT)));
-#define WAL_INT4(G, F, Z) launch_chain(int4_gemv_kernel<NT, RT, G, F, Z>, grid, kThreads, 0, st, p)
-  if (gpc == 2) {
-    if (f16) return p.zeros ? WAL_INT4(2, true, true) : WAL_INT4(2, true, false);
-    return p.zeros ? WAL_INT4(2, false, true) : WAL_INT4(2, false, false);
+// What a CTA has for activations, two CTAs to an SM.
+template <int NT>
+constexpr int room() { return 227 * 1024 / 2 - 1024 - kWarps * 16 * (8 * NT + 1) * 4; }
+
+template <int NT, int GPC, bool F16, bool ZEROS, bool STAGED>
+int launch_one(const Int4Params& p, unsigned grid, cudaStream_t st) {
+  auto kern = int4_gemv_kernel<NT, GPC, F16, ZEROS, STAGED>;
+  if (STAGED) {
+    static std::atomic<uint64_t> allowed{0};  // devices where the kernel may use its shared memory
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WAL_ERR_CUDA;
+    if (!(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, room<NT>()) != cudaSuccess) return WAL_ERR_CUDA;
+      allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
   }
-  if (f16) return p.zeros ? WAL_INT4(1, true, true) : WAL_INT4(1, true, false);
-  return p.zeros ? WAL_INT4(1, false, true) : WAL_INT4(1, false, false);
-#undef WAL_INT4
+  return launch_chain(kern, dim3(grid), kThreads, STAGED ? p.M * p.stride : 0, st, p);
+}
+
+template <int NT, int GPC, bool ZEROS>
+int launch_type(const Int4Params& p, unsigned grid, cudaStream_t st) {
+  if ((long long)p.M * p.stride <= room<NT>())
+    return p.f16 ? launch_one<NT, GPC, true, ZEROS, true>(p, grid, st) : launch_one<NT, GPC, false, ZEROS, true>(p, grid, st);
+  return p.f16 ? launch_one<NT, GPC, true, ZEROS, false>(p, grid, st) : launch_one<NT, GPC, false, ZEROS, false>(p, grid, st);
+}
+
+template <int NT>
+int launch(Int4Params p, int gpc, cudaStream_t st) {
+  const int resident = 2 * sm_count();
+  // the warps of a CTA share a tile or take several: what takes the fewest rounds of chunks (adding up costs about as much
+  // as four)
+  long long best = -1;
+  unsigned grid = 1;
+  for (int ks = 1; ks <= kWarps; ks *= 2) {
+    const int own = kWarps / ks, groups = (p.tiles + own - 1) / own;
+    const long long cost = (long long)((groups + resident - 1) / resident) * ((p.chunks + ks - 1) / ks + 4);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p.ks = ks;
+      grid = (unsigned)(groups < resident ? groups : resident);
+    }
+  }
+  if (gpc == 2) return p.zeros ? launch_type<NT, 2, true>(p, grid, st) : launch_type<NT, 2, false>(p, grid, st);
+  return p.zeros ? launch_type<NT, 1, true>(p, grid, st) : launch_type<NT, 1, false>(p, grid, st);
 }
 
 }  // namespace
@@ -333,17 +406,15 @@ int wal_int4_gemv(const wal_int4_layer* l, const void* x, int x_dtype, int64_t M
   p.groups = p.K / l->group_size;
   p.per = l->group_size == 128 ? 1 : 0;
   p.y_dtype = y_dtype;
-  p.ks = 1;
-  while (p.ks < kWarps && p.ks * 2 <= p.chunks) p.ks *= 2;
+  p.f16 = x_dtype == WAL_F16;
+  const int gpc = l->group_size == 32 ? 2 : 1;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  p.stride = 128 * p.chunks + 64;
   for (int64_t m0 = 0; m0 < M; m0 += 32) {
+    p.M = (int)(M - m0 < 32 ? M - m0 : 32);
     p.x = static_cast<const uint16_t*>(x) + m0 * ldx;
     p.y = static_cast<uint8_t*>(y) + m0 * ldy * ysize;
-    p.M = (int)(M - m0 < 32 ? M - m0 : 32);
-    const int gpc = l->group_size == 32 ? 2 : 1;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int rc = p.M <= 8    ? launch<1, 1>(p, gpc, x_dtype == WAL_F16, s)
-                   : p.M <= 16 ? launch<2, 2>(p, gpc, x_dtype == WAL_F16, s)
-                               : launch<4, 2>(p, gpc, x_dtype == WAL_F16, s);
+    const int rc = p.M <= 8 ? launch<1>(p, gpc, s) : p.M <= 16 ? launch<2>(p, gpc, s) : launch<4>(p, gpc, s);
     if (rc != WAL_OK) return rc;
   }
   return WAL_OK;
