@@ -98,9 +98,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // Programmatic dependent launch: a kernel waits for the grids before it in the
 // stream before it touches memory, and lets the next one start launching.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void chain() {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  wait_for_previous();
+  let_next_start();
 }
 
 constexpr int kMaxDevices = 64;

@@ -625,6 +625,7 @@ __device__ __forceinline__ void run_segment(const AttnParams& p, const Segment& 
     }
   }
   __syncthreads();
+  if (SH && whole && first_tile<SH>(p, sg.b, n) > 0) wait_for_previous();
   const int rows = min(RT, news * p.G - sg.rt * RT);
   for (int i = tid; i < rows * (HD / 4); i += kThreads) {
     const int row = i / (HD / 4), c = i % (HD / 4), w0 = row / RW, rr = row % RW;
@@ -665,6 +666,7 @@ __device__ __forceinline__ void join_runs(const AttnParams& p, const Segment& sg
   constexpr int RT = Shape<HD, RW, WM>::kRows;
   int news, len;
   const int n = positions<RT>(p, sg.b, sg.rt, &news, &len);
+  if (SH && first_tile<SH>(p, sg.b, n) > 0) wait_for_previous();
   const int rows = min(RT, news * p.G - sg.rt * RT);
   for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
     const int row = i / (HD / 4), c = i % (HD / 4);
@@ -713,7 +715,10 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  chain();
+  // The kernel of the shared prefixes has waited for everything before it, so what is read here is there; only its own
+  // results are waited for, where they are joined, and at the end (what follows this kernel counts on both).
+  if (SH) let_next_start();
+  else chain();
   // a run of position tiles (with kUnitCost more before each unit's), or every gridDim-th unit
   unsigned per = 0, at = blockIdx.x, end = p.units;
   int e = 0, kvh = 0;
@@ -835,6 +840,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, RW, WM>::kCtas) kv8_attent
       for (int i = tid; i < p.hq * HD / 8; i += kThreads)
         *reinterpret_cast<uint4*>(p.out + m * p.ld_out + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
   }
+  if (SH) wait_for_previous();
 }
 
 // Row tile of a call: the smallest of 8, 16, 24, 32, 48, 64 that holds the rows
