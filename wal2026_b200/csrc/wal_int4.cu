@@ -409,7 +409,7 @@ int wal_int4_gemv(const wal_int4_layer* l, const void* x, int x_dtype, int64_t M
   p.f16 = x_dtype == WAL_F16;
   const int gpc = l->group_size == 32 ? 2 : 1;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  p.stride = 128 * p.chunks + 64;
+  p.stride = p.chunks < 4096 ? 128 * p.chunks + 64 : 1 << 20;  // rows beyond are not staged anyway
   for (int64_t m0 = 0; m0 < M; m0 += 32) {
     p.M = (int)(M - m0 < 32 ? M - m0 : 32);
     p.x = static_cast<const uint16_t*>(x) + m0 * ldx;

@@ -16,6 +16,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _abi
+from .kv8 import _call
 
 GROUP_SIZES = (32, 64, 128)
 
@@ -107,28 +108,20 @@ class Int4Linear(nn.Module):
 
     def gemv_into(self, x2: Tensor, y: Tensor) -> None:
         """y[M, N] <- x2[M, K] @ W^T (+ bias) on the current stream; x2 bf16 or fp16, y bf16, fp16 or fp32."""
-        dev, s, o = x2.device, x2.stride(), y.stride()
-        if (not x2.is_cuda or x2.dim() != 2 or y.shape != (x2.shape[0], self.out_features) or x2.shape[1] != self.in_features
-                or s[1] != 1 or (o[1] != 1 and self.out_features > 1) or y.device != dev or self.packed.device != dev):
+        index, shape, s, o = x2.get_device(), x2.shape, x2.stride(), y.stride()
+        M = shape[0] if len(shape) == 2 else 0
+        if (index < 0 or shape != (M, self.in_features) or y.shape != (M, self.out_features) or s[1] != 1
+                or (o[1] != 1 and self.out_features > 1) or y.get_device() != index or self.packed.get_device() != index):
             raise ValueError(f"x2 [M, {self.in_features}] and y [M, {self.out_features}] must have contiguous rows on the "
                              f"layer's CUDA device ({self.packed.device})")
         if x2.dtype not in (torch.bfloat16, torch.float16) or y.dtype not in _abi.DTYPE_CODE:
             raise ValueError(f"Int4Linear supports bfloat16 and float16 activations (outputs in float32 too), got {x2.dtype}, {y.dtype}")
-        M = x2.shape[0]
         if M == 0:
             return
         # the stride of a single row says nothing
-        args = (ctypes.byref(self.layer_struct()), x2.data_ptr(), _abi.DTYPE_CODE[x2.dtype], M,
-                s[0] if M > 1 else -(-self.in_features // 8) * 8, y.data_ptr(), o[0] if M > 1 else self.out_features,
-                _abi.DTYPE_CODE[y.dtype])
-        lib = _abi.load()
-        if dev.index == torch.cuda.current_device():
-            st = lib.wal_int4_gemv(*args, _abi.stream_handle(dev))
-        else:
-            with torch.cuda.device(dev):
-                st = lib.wal_int4_gemv(*args, _abi.stream_handle(dev))
-        if st:
-            _abi.check(st, "wal_int4_gemv")
+        _call(index, "wal_int4_gemv", ctypes.byref(self.layer_struct()), x2.data_ptr(), _abi.DTYPE_CODE[x2.dtype], M,
+              s[0] if M > 1 else -(-self.in_features // 8) * 8, y.data_ptr(), o[0] if M > 1 else self.out_features,
+              _abi.DTYPE_CODE[y.dtype])
 
     def forward(self, x: Tensor) -> Tensor:
         if not x.is_cuda:
