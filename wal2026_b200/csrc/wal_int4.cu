@@ -19,6 +19,15 @@
 // columns, loading the next chunks, the next group's first ones among them, while
 // it multiplies.  What the ks warps have of a tile is added in order, so results do
 // not depend on timing.
+//
+// On B200: 128256 x 4096 for five tokens 75 us, 3.65 TB/s (its bytes at a copy's rate:
+// 41).  In a graph, for sixteen tokens 119, for 32 214; 28672 x 4096 for one 22.5 (copy: 9);
+// 4096 x 4096 for one 5.7; 4096 x 14336 for sixteen, with zero points, 18 (copy: 5).
+// Bound by instructions: 23 for each fragment of 256 weights, of which unpacking takes
+// eleven.  Not kept: two row tiles per warp for 9 to 16 tokens (126 against 118 at
+// 128256 x 4096, 26 against 18 at 4096 x 14336, no different at 28672 x 4096); a
+// cluster that splits the columns (37 against 18 at 4096 x 14336); activations as f16, whose
+// longer fraction saves shifts (no gain, slower for one token).
 #include "wal_kv8.cuh"
 
 #include <cuda_fp16.h>

@@ -887,7 +887,7 @@ int launch_rows(const AttnParams& p, int rows, int grid, cudaStream_t st) {
   }
 }
 
-// What a call's arguments come to, its row tile among them; the workspace's parts follow `ws`.
+// What a call's arguments come to, its row tile and where its parts lie in the workspace among them.
 struct Plan {
   AttnParams p;
   int rows, grid;

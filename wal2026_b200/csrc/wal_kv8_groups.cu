@@ -6,6 +6,10 @@
 // of a group's rows is what it shares.  One cluster: each CTA builds the same
 // small table for itself, the comparisons (the only real reading) are dealt out to
 // all warps, and the first CTA writes the groups down in order.
+//
+// On B200: 8 rows 5.9 us, 296 rows of up to 8700 positions in pages of 16 11.5 us (the
+// comparisons read 0.3 MB): a chain of memory round trips and barriers.  Calls of more
+// than 4096 table entries take the cluster, smaller ones a single CTA.
 #include "wal_kv8.cuh"
 
 #include <climits>

@@ -18,6 +18,13 @@
 // multiply-add, off by 2^-24 of the exponent and a rounding of m k that all of the CTA's
 // entries share.  Temperatures outside [2^-40, 2^40] and maxima near fp32's ends
 // divide and subtract instead.
+//
+// On B200, 128256 tokens: 576 rows with every rule 217 us (453 MB, 2.1 TB/s; a copy
+// would take 69), 80 fp32 rows with masks and biases 46 us, one row 12 us, most of it the
+// host's call.  The long calls are bound by the rules' instructions and by a row's
+// exchanges between its CTAs, with two CTAs per SM to hide them.  Earlier forms of the
+// long one: entries in shared memory and a division for each 418 us; a cluster per row
+// 324; clusters that stay, neighbouring tokens in one CTA 442, and dealt out in blocks 273.
 #include "wal_kv8.cuh"
 
 #include <cuda_fp16.h>
