@@ -219,6 +219,24 @@ def test_padding_rows_strides_and_shared_masks():
     assert bool((out == 7.0).all())  # nothing else was written
 
 
+@pytest.mark.parametrize("T,keep", [(2, (1,)), (3, (2, 1, 3, 0)), (5, (1, 3))])
+def test_skipped_rows_between_rows_of_several_ctas(T, keep):
+    # more rows than clusters of CTAs run at a time, so that a cluster goes from one sequence's rows to the next one's
+    B, V = 150, 33000
+    logits = torch.randn(B, T, V, device=DEV, generator=_gen(T))
+    scale = torch.arange(1, B + 1, device=DEV).view(B, 1, 1) / 20.0  # maxima and sums differ from row to row
+    logits = (logits * scale).contiguous()
+    news = _i32([keep[b % len(keep)] for b in range(B)])
+    live = (torch.arange(T, device=DEV) < news[:, None]).unsqueeze(-1)
+    want = torch.softmax(logits.double(), -1) * live
+    most = logits.abs().amax(-1, keepdim=True).double()
+    bound = want * (16 * 2.0 ** -24 * most + (V / 512 + 24) * 2.0 ** -23) + 2.0 ** -126
+    for _ in range(5):
+        out = torch.full((B, T, V), 7.0, device=DEV)
+        logit_rules(logits, out, new_lens=news)
+        assert bool(((out.double() - want).abs() <= bound).all())
+
+
 def test_the_largest_vocabulary_and_as_many_biases_as_are_allowed():
     V = 393216
     g = _gen(1)

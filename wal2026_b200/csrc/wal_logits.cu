@@ -19,8 +19,8 @@
 // entries share.  Temperatures outside [2^-40, 2^40] and maxima near fp32's ends
 // divide and subtract instead.
 //
-// On B200, 128256 tokens: 576 rows with every rule 217 us (453 MB, 2.1 TB/s; a copy
-// would take 69), 80 fp32 rows with masks and biases 46 us, one row 12 us, most of it the
+// On B200, 128256 tokens: 576 rows with every rule 209 us (453 MB, 2.2 TB/s; a copy
+// would take 69), 80 fp32 rows with masks and biases 45 us, one row 12 us, most of it the
 // host's call.  The long calls are bound by the rules' instructions and by a row's
 // exchanges between its CTAs, with two CTAs per SM to hide them.  Earlier forms of the
 // long one: entries in shared memory and a division for each 418 us; a cluster per row
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
   __shared__ float adds[kMaxBias];
   __shared__ float wv[W], wsum[W];
   __shared__ int wi[W];
-  // by the row's parity: what one CTA tells the others is read before any of them can be two rows further
+  // two in turn: what one CTA tells the others is read before any of them can be two exchanges further
   __shared__ float cmax[2][kMaxCluster], csum[2][kMaxCluster];
   __shared__ int cidx[2][kMaxCluster];
   cg::cluster_group cl = cg::this_cluster();
@@ -122,9 +122,10 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
   const int row0 = (int)((long long)rows * mine / clusters), row1 = (int)((long long)rows * (mine + 1) / clusters);
   wal_kv8::chain();
   cl.sync();  // a CTA's shared memory may be written by the others once it has started
+  int turn = 1;  // changes with each row that exchanges: skipped ones have no barrier
   int held = -1, upto = 0;  // the sequence whose words are there, and how much of its text they count
   for (int row = row0; row < row1; ++row) {
-  const int b = row / p.T, t = row - b * p.T, parity = row & 1;
+  const int b = row / p.T, t = row - b * p.T;
   float* const out = p.out + b * p.out_seq + t * p.out_row;
   auto write = [&](int k, const float (&x)[4]) {
     const int v = v0 + k * step;
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
     }
     continue;
   }
+  turn ^= 1;
   // this CTA's largest, and its sum relative to it
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -323,19 +325,19 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
       first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
     }
     if (lane < ncta) {
-      *cl.map_shared_rank(&cmax[parity][rank], lane) = ref;
-      *cl.map_shared_rank(&csum[parity][rank], lane) = total;
-      *cl.map_shared_rank(&cidx[parity][rank], lane) = first;
+      *cl.map_shared_rank(&cmax[turn][rank], lane) = ref;
+      *cl.map_shared_rank(&csum[turn][rank], lane) = total;
+      *cl.map_shared_rank(&cidx[turn][rank], lane) = first;
     }
   }
   cl.sync();
   // a lane per CTA (the lanes beyond repeat them): the cluster's largest, and its sum relative to it
-  const float its = cmax[parity][lane & (ncta - 1)];
+  const float its = cmax[turn][lane & (ncta - 1)];
   float all = its;
-  int best = cidx[parity][lane & (ncta - 1)];
+  int best = cidx[turn][lane & (ncta - 1)];
 #pragma unroll
   for (int o = kMaxCluster / 2; o > 0; o >>= 1) better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
-  float total = lane < ncta && its > -INFINITY ? csum[parity][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
+  float total = lane < ncta && its > -INFINITY ? csum[turn][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const float factor = greedy || !(ref > -INFINITY) ? 0.f : (ref == all ? 1.f : expf(ref - all)) / total;
