@@ -82,6 +82,22 @@ def test_int4_gemv_strided_rows_and_their_surroundings():
     assert bool((out == 5.0).all())  # nothing else was written
 
 
+def test_int4_weights_written_just_before_the_call():
+    N, K, M = 4096, 2048, 3
+    one, other = _layer(N, K, 128, True, 21)[0], _layer(N, K, 128, True, 22)[0]
+    layer = _layer(N, K, 128, True, 23)[0]
+    x = torch.randn(M, K, device=DEV, generator=_gen(2)).to(BF)
+    want = [torch.empty(M, N, device=DEV) for _ in range(2)]
+    one.gemv_into(x, want[0])
+    other.gemv_into(x, want[1])
+    got = [torch.empty(M, N, device=DEV) for _ in range(40)]
+    for i, y in enumerate(got):
+        for name in ("packed", "zeros", "scales"):
+            getattr(layer, name).copy_(getattr((one, other)[i % 2], name))
+        layer.gemv_into(x, y)
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+
+
 def test_int4_infinities_and_nan_stay_in_their_token():
     layer, w = _layer(64, 256, 32, True, 9)
     x = torch.randn(5, 256, device=DEV, generator=_gen(2)).to(BF)

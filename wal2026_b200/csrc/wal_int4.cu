@@ -21,8 +21,8 @@
 // not depend on timing.
 //
 // On B200: 128256 x 4096 for five tokens 75 us, 3.65 TB/s (its bytes at a copy's rate:
-// 41).  In a graph, for sixteen tokens 119, for 32 214; 28672 x 4096 for one 22.5 (copy: 9);
-// 4096 x 4096 for one 5.7; 4096 x 14336 for sixteen, with zero points, 18 (copy: 5).
+// 41).  In a graph, for sixteen tokens 119, for 32 217; 28672 x 4096 for one 23 (copy: 9);
+// 4096 x 4096 for one 5.8; 4096 x 14336 for sixteen, with zero points, 18 (copy: 5).
 // Bound by instructions: 23 for each fragment of 256 weights, of which unpacking takes
 // eleven.  Not kept: two row tiles per warp for 9 to 16 tokens (126 against 118 at
 // 128256 x 4096, 26 against 18 at 4096 x 14336, no different at 28672 x 4096); a
@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(kThreads, 2) int4_gemv_kernel(const __grid_con
 
   Batch cur;
   Place here = place(part);
-  fetch(cur, here, kslice);  // weights do not depend on the kernels before this one
-  wal_kv8::chain();
+  wal_kv8::chain();  // the weights, too: the kernel before may be the one that packed or copied them
+  fetch(cur, here, kslice);
   if (STAGED) {
     for (int row = warp; row < p.M; row += kWarps) {
       const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
