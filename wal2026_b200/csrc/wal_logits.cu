@@ -125,234 +125,235 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
   int turn = 1;  // changes with each row that exchanges: skipped ones have no barrier
   int held = -1, upto = 0;  // the sequence whose words are there, and how much of its text they count
   for (int row = row0; row < row1; ++row) {
-  const int b = row / p.T, t = row - b * p.T;
-  float* const out = p.out + b * p.out_seq + t * p.out_row;
-  auto write = [&](int k, const float (&x)[4]) {
-    const int v = v0 + k * step;
-    if (VEC) {
-      if (v < p.V) __stcs(reinterpret_cast<float4*>(out + v), make_float4(x[0], x[1], x[2], x[3]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v + e < p.V) out[v + e] = x[e];
-    }
-  };
-  if (p.r.new_lens && t >= p.r.new_lens[b]) {  // for all CTAs of the row
-    const float none[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < K; ++k) write(k, none);
-    continue;
-  }
-  float x[K][4];
-  const long long base = b * p.ld_seq + t * p.ld_row;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int v = v0 + k * step;
-    if (VEC) {
-      const float4 f = v < p.V ? load4<DT>(p.logits, base + v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      x[k][0] = f.x, x[k][1] = f.y, x[k][2] = f.z, x[k][3] = f.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = v + e < p.V ? load1<DT>(p.logits, base + v + e) : -INFINITY;
-    }
-  }
-  if (row + 1 < row1) {
-    const int nb2 = (row + 1) / p.T, nt = row + 1 - nb2 * p.T;
-    constexpr int kLine = 128 / (DT == WAL_F32 ? 4 : 2);
-    const long long first = nb2 * p.ld_seq + nt * p.ld_row;
-    for (int i = kLine * tid; i < p.share && at(i) < p.V; i += kLine * NT) {
-      const char* line = static_cast<const char*>(p.logits) + (first + at(i)) * (DT == WAL_F32 ? 4 : 2);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
-    }
-  }
-  if ((counted || nb) && held != b) {
-    __syncthreads();  // the words of the sequence before have been read
-    for (int i = tid; i < p.share / 4; i += NT) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = tid; i < nb; i += NT) {
-      ids[i] = p.r.bias_ids[(long long)b * nb + i];
-      adds[i] = p.r.bias[(long long)b * nb + i];
-    }
-    __syncthreads();
-    if (counted) {
-      const int* text = p.r.text + b * p.r.ld_text;
-      upto = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
-      const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
-#pragma unroll 4
-      for (int j = tid; j < upto; j += NT) {
-        const unsigned w = place((unsigned)text[j]);
-        if (w != 0xffffffffu) {
-          if (j < prompt) atomicOr(words + w, kPrompt);
-          else atomicAdd(words + w, 1u);
-        }
-      }
-    }
-    float sum = 0.f;
-    for (int i = tid; i < nb; i += NT) {
-      const unsigned w = place((unsigned)ids[i]);
-      if (w == 0xffffffffu) continue;
-      bool first = true;
-      for (int j = 0; j < i && first; ++j) first = ids[j] != ids[i];
-      if (!first) continue;  // the first of equal ones adds them all, in order
-      sum = adds[i];
-      for (int j = i + 1; j < nb; ++j)
-        if (ids[j] == ids[i]) sum += adds[j];
-      atomicOr(words + w, (unsigned)(i + 1) << kBiasBit);
-      if (sum != adds[i]) adds[i] = sum;  // no other thread reads the first one's
-    }
-    held = b;
-    __syncthreads();
-  } else if (counted) {  // the row's own token, if the text has it
-    const int now = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
-    __syncthreads();
-    if (tid == 0 && now > upto) {
-      const unsigned w = place((unsigned)p.r.text[b * p.r.ld_text + now - 1]);
-      const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
-      if (w != 0xffffffffu) words[w] = now - 1 < prompt ? words[w] | kPrompt : words[w] + 1u;
-    }
-    upto = now;
-    __syncthreads();
-  }
-  const float rep = p.r.repetition ? p.r.repetition[b] : 1.f, pres = p.r.presence ? p.r.presence[b] : 0.f;
-  const float freq = p.r.frequency ? p.r.frequency[b] : 0.f, temp = p.r.temperature ? p.r.temperature[b] : 1.f;
-  const bool greedy = !(temp > 0.f);
-  const float inv = 1.f / rep;
-  const int* const mask = p.r.mask ? p.r.mask + b * p.r.mask_seq + t * p.r.mask_row : nullptr;
-  // a separate copy for the repetitions that have to be divided by
-  auto penalise = [&](auto divide) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = 4 * (tid + NT * k);
-      if (i >= p.share) break;
-      const uint4 c = *reinterpret_cast<const uint4*>(words + i);
-      const unsigned w[4] = {c.x, c.y, c.z, c.w}, any = c.x | c.y | c.z | c.w;
-      if (any == 0u) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y = x[k][e] > 0.f ? (divide.value ? x[k][e] / rep : x[k][e] * inv) : x[k][e] * rep;
-        const float z = y - freq * (float)(w[e] & kCount) - pres;
-        x[k][e] = w[e] & kCount ? z : w[e] & kPrompt ? y : x[k][e];
-      }
-      if (any >> kBiasBit)
+    const int b = row / p.T, t = row - b * p.T;
+    float* const out = p.out + b * p.out_seq + t * p.out_row;
+    auto write = [&](int k, const float (&x)[4]) {
+      const int v = v0 + k * step;
+      if (VEC) {
+        if (v < p.V) __stcs(reinterpret_cast<float4*>(out + v), make_float4(x[0], x[1], x[2], x[3]));
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (w[e] >> kBiasBit) x[k][e] += adds[(w[e] >> kBiasBit) - 1];
+          if (v + e < p.V) out[v + e] = x[e];
+      }
+    };
+    if (p.r.new_lens && t >= p.r.new_lens[b]) {  // for all CTAs of the row
+      const float none[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < K; ++k) write(k, none);
+      continue;
     }
-  };
-  if (counted || nb) {
-    if (rep >= 9.0949470177292824e-13f && rep <= 1.099511627776e12f) penalise(std::false_type{});
-    else penalise(std::true_type{});
-  }
-  if (mask) {
-    const int* const mine = mask + (v0 >> 5);  // groups of a thread have the same place in their words
-    unsigned bits[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) bits[k] = v0 + k * step < p.V ? (unsigned)__ldg(mine + k * (step >> 5)) >> (v0 & 31) : 0u;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = (bits[k] >> e) & 1 ? x[k][e] : -INFINITY;
-  }
-  float top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[k][e] = number(x[k][e]);
-      top = fmaxf(top, x[k][e]);
-    }
-  if (!p.softmax) {
+    float x[K][4];
+    const long long base = b * p.ld_seq + t * p.ld_row;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!greedy && p.r.temperature)
+      const int v = v0 + k * step;
+      if (VEC) {
+        const float4 f = v < p.V ? load4<DT>(p.logits, base + v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        x[k][0] = f.x, x[k][1] = f.y, x[k][2] = f.z, x[k][3] = f.w;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[k][e] = number(x[k][e] / temp);
-      write(k, x[k]);
+        for (int e = 0; e < 4; ++e) x[k][e] = v + e < p.V ? load1<DT>(p.logits, base + v + e) : -INFINITY;
+      }
     }
-    continue;
-  }
-  turn ^= 1;
-  // this CTA's largest, and its sum relative to it
+    if (row + 1 < row1) {
+      const int nb2 = (row + 1) / p.T, nt = row + 1 - nb2 * p.T;
+      constexpr int kLine = 128 / (DT == WAL_F32 ? 4 : 2);
+      const long long first = nb2 * p.ld_seq + nt * p.ld_row;
+      for (int i = kLine * tid; i < p.share && at(i) < p.V; i += kLine * NT) {
+        const char* line = static_cast<const char*>(p.logits) + (first + at(i)) * (DT == WAL_F32 ? 4 : 2);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+      }
+    }
+    if ((counted || nb) && held != b) {
+      __syncthreads();  // the words of the sequence before have been read
+      for (int i = tid; i < p.share / 4; i += NT) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = tid; i < nb; i += NT) {
+        ids[i] = p.r.bias_ids[(long long)b * nb + i];
+        adds[i] = p.r.bias[(long long)b * nb + i];
+      }
+      __syncthreads();
+      if (counted) {
+        const int* text = p.r.text + b * p.r.ld_text;
+        upto = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
+        const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
+#pragma unroll 4
+        for (int j = tid; j < upto; j += NT) {
+          const unsigned w = place((unsigned)text[j]);
+          if (w != 0xffffffffu) {
+            if (j < prompt) atomicOr(words + w, kPrompt);
+            else atomicAdd(words + w, 1u);
+          }
+        }
+      }
+      float sum = 0.f;
+      for (int i = tid; i < nb; i += NT) {
+        const unsigned w = place((unsigned)ids[i]);
+        if (w == 0xffffffffu) continue;
+        bool first = true;
+        for (int j = 0; j < i && first; ++j) first = ids[j] != ids[i];
+        if (!first) continue;  // the first of equal ones adds them all, in order
+        sum = adds[i];
+        for (int j = i + 1; j < nb; ++j)
+          if (ids[j] == ids[i]) sum += adds[j];
+        atomicOr(words + w, (unsigned)(i + 1) << kBiasBit);
+        if (sum != adds[i]) adds[i] = sum;  // no other thread reads the first one's
+      }
+      held = b;
+      __syncthreads();
+    } else if (counted) {  // the row's own token, if the text has it
+      const int now = (int)min((long long)max(p.r.lens[b], -1 - t) + t + 1, (long long)p.r.text_len);
+      __syncthreads();
+      if (tid == 0 && now > upto) {
+        const unsigned w = place((unsigned)p.r.text[b * p.r.ld_text + now - 1]);
+        const int prompt = p.r.prompt_lens ? p.r.prompt_lens[b] : 0;
+        if (w != 0xffffffffu) words[w] = now - 1 < prompt ? words[w] | kPrompt : words[w] + 1u;
+      }
+      upto = now;
+      __syncthreads();
+    }
+    const float rep = p.r.repetition ? p.r.repetition[b] : 1.f, pres = p.r.presence ? p.r.presence[b] : 0.f;
+    const float freq = p.r.frequency ? p.r.frequency[b] : 0.f, temp = p.r.temperature ? p.r.temperature[b] : 1.f;
+    const bool greedy = !(temp > 0.f);
+    const float inv = 1.f / rep;
+    const int* const mask = p.r.mask ? p.r.mask + b * p.r.mask_seq + t * p.r.mask_row : nullptr;
+    // a separate copy for the repetitions that have to be divided by
+    auto penalise = [&](auto divide) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) wv[warp] = top;
-  __syncthreads();
-  top = wv[lane % W];
+      for (int k = 0; k < K; ++k) {
+        const int i = 4 * (tid + NT * k);
+        if (i >= p.share) break;
+        const uint4 c = *reinterpret_cast<const uint4*>(words + i);
+        const unsigned w[4] = {c.x, c.y, c.z, c.w}, any = c.x | c.y | c.z | c.w;
+        if (any == 0u) continue;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = 1.4426950408889634f / temp, off = -top * scale;
-  const bool usual = temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(off) < 1e30f;
-  float sum = 0.f, ref = top;  // ref: what this CTA's entries are relative to, divided by the temperature
-  int where = 0x7fffffff;
-  if (greedy) {
+        for (int e = 0; e < 4; ++e) {
+          const float y = x[k][e] > 0.f ? (divide.value ? x[k][e] / rep : x[k][e] * inv) : x[k][e] * rep;
+          const float z = y - freq * (float)(w[e] & kCount) - pres;
+          x[k][e] = w[e] & kCount ? z : w[e] & kPrompt ? y : x[k][e];
+        }
+        if (any >> kBiasBit)
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k)
+          for (int e = 0; e < 4; ++e)
+            if (w[e] >> kBiasBit) x[k][e] += adds[(w[e] >> kBiasBit) - 1];
+      }
+    };
+    if (counted || nb) {
+      if (rep >= 9.0949470177292824e-13f && rep <= 1.099511627776e12f) penalise(std::false_type{});
+      else penalise(std::true_type{});
+    }
+    if (mask) {
+      const int* const mine = mask + (v0 >> 5);  // groups of a thread have the same place in their words
+      unsigned bits[K];
 #pragma unroll
-      for (int e = 3; e >= 0; --e)
-        if (x[k][e] == top) where = v0 + k * step + e;
-  } else if (usual) {
-    ref = top / temp;
+      for (int k = 0; k < K; ++k) bits[k] = v0 + k * step < p.V ? (unsigned)__ldg(mine + k * (step >> 5)) >> (v0 & 31) : 0u;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][e] = (bits[k] >> e) & 1 ? x[k][e] : -INFINITY;
+    }
+    float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[k][e] = ex2(fmaf(x[k][e], scale, off));
-        sum += x[k][e];
+        x[k][e] = number(x[k][e]);
+        top = fmaxf(top, x[k][e]);
       }
-  } else {
-    ref = number(top / temp);
-    // a temperature can make the largest infinite, or a NaN of an infinite one: then what is equal to it shares
+    if (!p.softmax) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
+        if (!greedy && p.r.temperature)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y = number(x[k][e] / temp);
-        x[k][e] = y == -INFINITY ? 0.f : y == ref ? 1.f : expf(y - ref);
-        sum += x[k][e];
+          for (int e = 0; e < 4; ++e) x[k][e] = number(x[k][e] / temp);
+        write(k, x[k]);
       }
-  }
+      continue;
+    }
+    turn ^= 1;
+    // this CTA's largest, and its sum relative to it
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    where = min(where, __shfl_xor_sync(0xffffffffu, where, o));
-  }
-  if (lane == 0) wsum[warp] = sum, wi[warp] = where;
-  __syncthreads();
-  if (warp == 0) {
-    float total = lane < W ? wsum[lane] : 0.f;
-    int first = wi[lane % W];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) wv[warp] = top;
+    __syncthreads();
+    top = wv[lane % W];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = 1.4426950408889634f / temp, off = -top * scale;
+    const bool usual = temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(off) < 1e30f;
+    float sum = 0.f, ref = top;  // ref: what this CTA's entries are relative to, divided by the temperature
+    int where = 0x7fffffff;
+    if (greedy) {
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k)
+#pragma unroll
+        for (int e = 3; e >= 0; --e)
+          if (x[k][e] == top) where = v0 + k * step + e;
+    } else if (usual) {
+      ref = top / temp;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[k][e] = ex2(fmaf(x[k][e], scale, off));
+          sum += x[k][e];
+        }
+    } else {
+      ref = number(top / temp);
+      // a temperature can make the largest infinite, or a NaN of an infinite one: then what is equal to it shares
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = number(x[k][e] / temp);
+          x[k][e] = y == -INFINITY ? 0.f : y == ref ? 1.f : expf(y - ref);
+          sum += x[k][e];
+        }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      where = min(where, __shfl_xor_sync(0xffffffffu, where, o));
     }
-    if (lane < ncta) {
-      *cl.map_shared_rank(&cmax[turn][rank], lane) = ref;
-      *cl.map_shared_rank(&csum[turn][rank], lane) = total;
-      *cl.map_shared_rank(&cidx[turn][rank], lane) = first;
+    if (lane == 0) wsum[warp] = sum, wi[warp] = where;
+    __syncthreads();
+    if (warp == 0) {
+      float total = lane < W ? wsum[lane] : 0.f;
+      int first = wi[lane % W];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      }
+      if (lane < ncta) {
+        *cl.map_shared_rank(&cmax[turn][rank], lane) = ref;
+        *cl.map_shared_rank(&csum[turn][rank], lane) = total;
+        *cl.map_shared_rank(&cidx[turn][rank], lane) = first;
+      }
     }
-  }
-  cl.sync();
-  // a lane per CTA (the lanes beyond repeat them): the cluster's largest, and its sum relative to it
-  const float its = cmax[turn][lane & (ncta - 1)];
-  float all = its;
-  int best = cidx[turn][lane & (ncta - 1)];
+    cl.sync();
+    // a lane per CTA (the lanes beyond repeat them): the cluster's largest, and its sum relative to it
+    const float its = cmax[turn][lane & (ncta - 1)];
+    float all = its;
+    int best = cidx[turn][lane & (ncta - 1)];
 #pragma unroll
-  for (int o = kMaxCluster / 2; o > 0; o >>= 1) better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
-  float total = lane < ncta && its > -INFINITY ? csum[turn][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1)
+      better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
+    float total = lane < ncta && its > -INFINITY ? csum[turn][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const float factor = greedy || !(ref > -INFINITY) ? 0.f : (ref == all ? 1.f : expf(ref - all)) / total;
-  const int one = greedy && all > -INFINITY ? best : -1;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float factor = greedy || !(ref > -INFINITY) ? 0.f : (ref == all ? 1.f : expf(ref - all)) / total;
+    const int one = greedy && all > -INFINITY ? best : -1;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (factor == 0.f) {
+    for (int k = 0; k < K; ++k) {
+      if (factor == 0.f) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = v0 + k * step + e == one ? 1.f : 0.f;
-    } else {
+        for (int e = 0; e < 4; ++e) x[k][e] = v0 + k * step + e == one ? 1.f : 0.f;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] *= factor;
+        for (int e = 0; e < 4; ++e) x[k][e] *= factor;
+      }
+      write(k, x[k]);
     }
-    write(k, x[k]);
-  }
   }
 }
 
