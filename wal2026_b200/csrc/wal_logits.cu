@@ -7,17 +7,20 @@
 // the prompt does, and which bias it has; most words are zero and cost a test per
 // group.  Every CTA reads the text and counts what falls into its share while its
 // logits are on their way.  The CTAs exchange (maximum, sum) through distributed
-// shared memory once: entries are held as exp(x - the CTA's maximum), and the
+// shared memory once: entries are held as exp((x - the CTA's maximum) / t), and the
 // factor to the cluster's maximum and sum is one number per CTA.  Clusters that fill
 // the GPU take the rows in order: the T rows of a sequence need one count of the
 // text and then a token more each, and the next row's logits are asked into L2
 // while this one is worked on.
 //
-// Numerics: fp32 in the order of the definition.  The temperature goes into the
-// exponent: exp(x / t - m / t) = exp2(x k - m k), k = log2(e) / t, in one fused
-// multiply-add, off by 2^-24 of the exponent and a rounding of m k that all of the CTA's
-// entries share.  Temperatures outside [2^-40, 2^40] and maxima near fp32's ends
-// divide and subtract instead.
+// Numerics: fp32 in the order of the definition, with one change: of exp(x / t - m / t) the
+// difference is taken before the division, exp2((x - m) * k), k = log2(e) / t, so that an
+// exponent is off by 4 * 2^-24 of itself however far from zero the logits lie.  Maxima
+// are exchanged as they are, undivided: every CTA's entries stand relative to a number that
+// all know exactly.  (The fused exp2(x k - round(m k)), with each CTA's maximum divided
+// anew for the exchange, was off by 2^-24 of m k between CTAs, and took a CTA of masked
+// logits around -1e10 to an infinite sum.)  Temperatures outside [2^-40, 2^40] and quotients
+// near fp32's ends divide each difference instead; quotients that leave the range count as infinities.
 //
 // On B200, 128256 tokens: 576 rows with every rule 209 us (453 MB, 2.2 TB/s; a copy
 // would take 69), 80 fp32 rows with masks and biases 45 us, one row 12 us, most of it the
@@ -30,6 +33,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -85,6 +89,23 @@ __device__ __forceinline__ float number(float x) {
   float y;
   asm("max.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(-INFINITY));
   return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Whether exp((x - top) / temp), x <= top, is ex2((x - top) * (kLog2e / temp)): what leaves fp32's range there counts as 0.
+__device__ __forceinline__ bool usual(float top, float temp) {
+  return temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(top * (kLog2e / temp)) < 1e30f;
+}
+
+// exp((x - top) / temp), x <= top, anywhere: quotients that leave fp32's range are infinities, and infinite ones equal.
+__device__ __noinline__ float weight(float x, float top, float temp) {
+  const float q = number(x / temp);
+  if (q == -INFINITY) return 0.f;
+  if (x == top) return 1.f;
+  if (top / temp == INFINITY) return q == INFINITY ? 1.f : 0.f;
+  const float half = top > 1e30f ? 0.5f : 1.f;  // the difference may pass the largest number
+  return ex2((x * half - top * half) / temp * (kLog2e / half));
 }
 
 // (value, index) of the larger value, the lower index among equals
@@ -251,6 +272,12 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[k][e] = (bits[k] >> e) & 1 ? x[k][e] : -INFINITY;
     }
+    if (p.softmax && temp > FLT_MAX) {  // an infinite logit over an infinite temperature is no number
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][e] = fabsf(x[k][e]) <= FLT_MAX ? x[k][e] : -INFINITY;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -278,9 +305,8 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
     top = wv[lane % W];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = 1.4426950408889634f / temp, off = -top * scale;
-    const bool usual = temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(off) < 1e30f;
-    float sum = 0.f, ref = top;  // ref: what this CTA's entries are relative to, divided by the temperature
+    const float scale = kLog2e / temp;
+    float sum = 0.f;
     int where = 0x7fffffff;
     if (greedy) {
 #pragma unroll
@@ -288,24 +314,20 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
 #pragma unroll
         for (int e = 3; e >= 0; --e)
           if (x[k][e] == top) where = v0 + k * step + e;
-    } else if (usual) {
-      ref = top / temp;
+    } else if (usual(top, temp)) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[k][e] = ex2(fmaf(x[k][e], scale, off));
+          x[k][e] = ex2((x[k][e] - top) * scale);
           sum += x[k][e];
         }
-    } else {
-      ref = number(top / temp);
-      // a temperature can make the largest infinite, or a NaN of an infinite one: then what is equal to it shares
+    } else if (top > -INFINITY) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y = number(x[k][e] / temp);
-          x[k][e] = y == -INFINITY ? 0.f : y == ref ? 1.f : expf(y - ref);
+          x[k][e] = weight(x[k][e], top, temp);
           sum += x[k][e];
         }
     }
@@ -325,7 +347,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
         first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
       }
       if (lane < ncta) {
-        *cl.map_shared_rank(&cmax[turn][rank], lane) = ref;
+        *cl.map_shared_rank(&cmax[turn][rank], lane) = top;
         *cl.map_shared_rank(&csum[turn][rank], lane) = total;
         *cl.map_shared_rank(&cidx[turn][rank], lane) = first;
       }
@@ -338,10 +360,13 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
 #pragma unroll
     for (int o = kMaxCluster / 2; o > 0; o >>= 1)
       better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
-    float total = lane < ncta && its > -INFINITY ? csum[turn][lane & (ncta - 1)] * (its == all ? 1.f : expf(its - all)) : 0.f;
+    const bool near = usual(all, temp);
+    auto relative = [&](float m) { return near ? ex2((m - all) * scale) : weight(m, all, temp); };
+    float total = lane < ncta ? csum[turn][lane & (ncta - 1)] * relative(its) : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float factor = greedy || !(ref > -INFINITY) ? 0.f : (ref == all ? 1.f : expf(ref - all)) / total;
+    // a CTA with nothing left has entries of -inf, which are not multiplied
+    const float factor = greedy || !(total > 0.f) || top == -INFINITY ? 0.f : relative(top) / total;
     const int one = greedy && all > -INFINITY ? best : -1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
