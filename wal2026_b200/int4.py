@@ -19,6 +19,7 @@ from . import _abi
 from .kv8 import _call
 
 GROUP_SIZES = (32, 64, 128)
+_BUFFERS = {"packed": torch.uint8, "scales": torch.float16, "zeros": torch.uint8, "bias": torch.bfloat16}
 
 
 def quantize_int4(weight: Tensor, group_size: int = 128, *, zero_points: bool = False) -> tuple[Tensor, Tensor, Optional[Tensor]]:
@@ -51,7 +52,7 @@ class Int4Linear(nn.Module):
 
     codes: uint8 [N, K], 0 .. 15; scales: fp16 [N, K / group_size]; zeros: uint8
     like scales, 0 .. 15, or None (8); all on one CUDA device, where they are
-    packed once.  bias is kept in bf16.
+    packed once.  bias is kept in bf16; casts of the module change none of this.
     """
 
     def __init__(self, codes: Tensor, scales: Tensor, zeros: Optional[Tensor] = None, bias: Optional[Tensor] = None):
@@ -102,9 +103,24 @@ class Int4Linear(nn.Module):
     def layer_struct(self) -> _abi.Int4Layer:
         key = (self.packed.data_ptr(), self.scales.data_ptr(), _abi.ptr(self.zeros), _abi.ptr(self.bias))
         if self._layer_cache is None or self._layer_cache[0] != key:
+            self._check_types()
             layer = _abi.Int4Layer(self.out_features, self.in_features, self.group_size, *key)
             self._layer_cache = (key, layer)
         return self._layer_cache[1]
+
+    def _check_types(self) -> None:
+        for name, dtype in _BUFFERS.items():
+            t = getattr(self, name)
+            if t is not None and t.dtype != dtype:
+                raise ValueError(f"Int4Linear keeps {name} as {dtype}, got {t.dtype}")
+
+    def _apply(self, fn, recurse: bool = True):
+        """Moves of the module; casts (``to(dtype)``, ``half``, ..) leave the weight as it is, for the kernels read these types only."""
+        def move(t: Tensor) -> Tensor:
+            moved = fn(t)
+            return moved if moved.dtype == t.dtype else t.to(moved.device)
+
+        return super()._apply(move, recurse)
 
     def gemv_into(self, x2: Tensor, y: Tensor) -> None:
         """y[M, N] <- x2[M, K] @ W^T (+ bias) on the current stream; x2 bf16 or fp16, y bf16, fp16 or fp32."""
