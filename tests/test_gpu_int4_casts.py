@@ -1,6 +1,8 @@
 """4-bit linears on the GPU after their module, or the stack that holds them, was cast, copied or moved."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -33,3 +35,14 @@ def test_a_cast_stack_keeps_its_4_bit_head():
     want = stack.logits(x)
     stack.to(torch.bfloat16)
     assert torch.equal(stack.logits(x), want)
+
+
+def test_int4_copies_multiply_alone():
+    layer, _ = _layer(48, 256, 32, True, 2, bias=True)
+    x = torch.randn(2, 256, device=DEV, generator=_gen(3)).to(BF)
+    want, y = torch.empty(2, 48, device=DEV), torch.empty(2, 48, device=DEV)
+    layer.gemv_into(x, want)
+    other = copy.deepcopy(layer)
+    layer.packed.zero_()
+    other.gemv_into(x, y)
+    assert torch.equal(y, want)

@@ -1,6 +1,9 @@
 """What casts, copies and replaced buffers do to a 4-bit linear, without a GPU."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 from torch import nn
@@ -63,3 +66,11 @@ def test_buffers_of_another_type_are_refused(name, dtype):
     setattr(layer, name, getattr(layer, name).to(dtype))
     with pytest.raises(ValueError):
         layer.layer_struct()
+
+
+def test_copies_have_their_own_buffers():
+    layer = _linear(zeros=False)
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        _same(other, layer)
+        assert other.layer_struct().packed == other.packed.data_ptr() != layer.packed.data_ptr()
+    assert layer.layer_struct().packed == layer.packed.data_ptr()

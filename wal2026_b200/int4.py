@@ -108,6 +108,9 @@ class Int4Linear(nn.Module):
             self._layer_cache = (key, layer)
         return self._layer_cache[1]
 
+    def __getstate__(self) -> dict:
+        return self.__dict__ | {"_layer_cache": None}  # addresses are not copied
+
     def _check_types(self) -> None:
         for name, dtype in _BUFFERS.items():
             t = getattr(self, name)
