@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from tests.test_gpu_int4 import BF, DEV, F32, HF, _check, _gen, _layer
+from wal2026_b200.int4 import Int4Linear
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,16 @@ def test_int4_rows_do_not_depend_on_the_rows_beside_them():
     for i in range(7):
         layer.gemv_into(x[i:i + 1], one)
         assert torch.equal(one[0], y[i])
+
+
+@pytest.mark.parametrize("K", [32, 96, 160, 256])
+def test_int4_an_infinite_scale_of_the_last_group(K):
+    g = _gen(K)
+    codes = torch.randint(0, 16, (33, K), device=DEV, generator=g, dtype=torch.uint8)
+    scales = torch.rand(33, K // 32, device=DEV, generator=g).to(HF)
+    scales[::2, -1] = float("inf")
+    codes[:, K - 32:] = 11  # all three above the zero point
+    x = torch.rand(3, K, device=DEV, generator=g).to(BF) + 1
+    y = torch.empty(3, 33, device=DEV)
+    Int4Linear(codes, scales).gemv_into(x, y)
+    assert bool((y[:, ::2] == float("inf")).all()) and bool(y[:, 1::2].isfinite().all())

@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(kThreads, 2) int4_gemv_kernel(const __grid_con
 #pragma unroll
       for (int g = 0; g < GPC; ++g) {
         const int gi = GPC == 2 ? min(2 * c + g, p.groups - 1) : c >> p.per;
-        b.s[i][g] = __ldg(l.s + gi * 8);
+        // the half chunk behind K adds 0, not 0 times the last scale, which may be infinite
+        b.s[i][g] = GPC == 2 && 2 * c + g >= p.groups ? 0u : __ldg(l.s + gi * 8);
         if (ZEROS) b.z[i][g] = __ldg(l.z + gi * 8);
       }
     }
