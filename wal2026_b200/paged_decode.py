@@ -89,7 +89,9 @@ class PagedDecoder:
 
     share: rows whose first ``share`` positions (or more) lie in the same pages are
     a group, whose common positions each step reads once (``kv_pages_groups``);
-    None: every row reads its own.  text: keep the rows' tokens in ``text`` int32
+    None: every row reads its own.  ``status`` int32 [1] becomes 1, and stays so until
+    the caller clears it, where that attention gave up a wait (after 2 s): what the steps
+    since its last 0 returned and stored is wrong.  text: keep the rows' tokens in ``text`` int32
     [rows, max_len], by position; ``prompt_lens`` int32 [rows] (0 to begin with, the
     caller's to set) says where what the rows generated starts.
     """
@@ -110,6 +112,7 @@ class PagedDecoder:
         self.lens = torch.zeros(rows, **i32)
         self.info = torch.zeros(2, **i32)
         self.missing = torch.zeros(1, dtype=torch.int64, device=dev)
+        self.status = torch.zeros(1, **i32)
         self._room = torch.ones(1, dtype=torch.bool, device=dev)  # whether the last step got its pages
         self._next = torch.empty_like(self.table)
         self._self = torch.arange(rows, **i32)
@@ -202,7 +205,8 @@ class PagedDecoder:
             if self.share is None:
                 kv8_attention(self.cache, i, bufs.q, self.table, self.lens, bufs.attn, bufs.ws, new_lens=add)
             else:
-                kv8_attention_shared(self.cache, i, bufs.q, self.table, self.lens, self.groups, bufs.attn, bufs.ws, new_lens=add)
+                kv8_attention_shared(self.cache, i, bufs.q, self.table, self.lens, self.groups, bufs.attn, bufs.ws, new_lens=add,
+                                     status=self.status)
             self._row_parallel(layer.o, bufs.attn, layer.post_norm, bufs)
             _column(layer.gate_up, bufs.x, bufs.gu)
             silu_mul(bufs.gu, bufs.act)
