@@ -92,9 +92,10 @@ __device__ __forceinline__ float number(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Whether exp((x - top) / temp), x <= top, is ex2((x - top) * (kLog2e / temp)): what leaves fp32's range there counts as 0.
+// Whether exp((x - top) / temp), x <= top, top not -inf, is ex2((x - top) * (kLog2e / temp)): differences that leave fp32's
+// range count as 0 there, and no quotient is beyond its upper end.
 __device__ __forceinline__ bool usual(float top, float temp) {
-  return temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && fabsf(top * (kLog2e / temp)) < 1e30f;
+  return temp >= 9.0949470177292824e-13f && temp <= 1.099511627776e12f && top * (kLog2e / temp) < 1e30f;
 }
 
 // exp((x - top) / temp), x <= top, anywhere: quotients that leave fp32's range are infinities, and infinite ones equal.
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
 #pragma unroll
         for (int e = 3; e >= 0; --e)
           if (x[k][e] == top) where = v0 + k * step + e;
-    } else if (usual(top, temp)) {
+    } else if (top > -INFINITY && usual(top, temp)) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1) logit_rules_kernel(cons
 #pragma unroll
     for (int o = kMaxCluster / 2; o > 0; o >>= 1)
       better(all, best, __shfl_xor_sync(0xffffffffu, all, o), __shfl_xor_sync(0xffffffffu, best, o));
-    const bool near = usual(all, temp);
+    const bool near = usual(all, temp) && usual(-all, temp);  // nor beyond the lower one, where nothing is left of the row
     auto relative = [&](float m) { return near ? ex2((m - all) * scale) : weight(m, all, temp); };
     float total = lane < ncta ? csum[turn][lane & (ncta - 1)] * relative(its) : 0.f;
 #pragma unroll
