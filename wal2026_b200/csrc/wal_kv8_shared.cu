@@ -449,8 +449,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefix_kernel(const __grid
           }
         }
         const int e2 = min(max(14 + 127 - (int)(__float_as_uint(mx) >> 23), -112), 126);
-        const float up = __uint_as_float((uint32_t)(e2 + 127) << 23);
-        unscale = p.qscale * __uint_as_float((uint32_t)(127 - e2) << 23);
+        // q takes the scale's sign, so that the largest product stays the largest score
+        const float up = copysignf(__uint_as_float((uint32_t)(e2 + 127) << 23), p.qscale);
+        unscale = fabsf(p.qscale) * __uint_as_float((uint32_t)(127 - e2) << 23);
         if (slot == 0 || both) {
 #pragma unroll 1
           for (int i0 = 0; i0 < HD / 8; i0 += 4) {
