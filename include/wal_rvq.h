@@ -657,8 +657,10 @@ WAL_API int wal_kv_pages_groups(const int32_t* table, int64_t ld_table, const in
 /*
  * wal_kv8_attention with the positions that the rows of a group share read
  * once for all of them (groups: int32 [4][B] as wal_kv_pages_groups writes it,
- * for this table and these lens).  The same result up to the rounding of 16-bit
- * weights: every row attends to its own positions j <= lens[b] + t.  Entries of
+ * for this table and these lens).  Every row attends to its own positions j <=
+ * lens[b] + t.  The same result but for the weights of shared positions, which enter
+ * the product as one f16 each (off by 2^-11 of it; one whose product with its block's V scale
+ * is below 2^-32 of the largest is 0) where wal_kv8_attention keeps 2^-16.  Entries of
  * groups are bounded by the kernels; where they do not belong to the table, the
  * rows concerned are wrong and nothing else.  B <= 4096.
  * workspace: at least wal_kv8_attention_shared_workspace bytes, otherwise as in
@@ -683,6 +685,9 @@ WAL_API int wal_kv8_attention_shared(const wal_kv8_cache* cache, int32_t layer, 
  *   x += the sum of bias[b][i], in rising i, over bias_ids[b][i] = v
  *   bit v % 32 of mask word v / 32 of (b, t) clear, or x NaN: left out (-inf)
  *   x /= temperature[b]  (NULL: 1)
+ * x / repetition is the nearest fp32 number.  Of the softmax, differences of logits are
+ * taken before the division by the temperature, so that neither large logits nor small temperatures
+ * cost accuracy.
  * softmax != 0: out = softmax(x): where the largest x is an infinity, the
  * entries that have it share 1; temperature 0 (or negative, or NaN) gives 1 to
  * the first of the largest, 0 to the others; a row with nothing left is zeros.

@@ -28,7 +28,7 @@
 // each half, which share the converted codes; fewer give the slots alternate tiles.
 // P is exp2(x - m + 7) times the block's V scale over a power of two that bounds
 // the V scales so far: at most 2^15, so that f16 keeps weights down to 2^-32 of
-// the largest; each is rounded by 2^-12 at most.  Maxima, sums and outputs are fp32.
+// the largest; each is rounded by 2^-11 at most.  Maxima, sums and outputs are fp32.
 //
 // The position tiles of all units are cut into equal runs, one per SM.  Each run of
 // a unit, and each slot that had some of its tiles, leaves a partial result; the
@@ -43,8 +43,11 @@
 // about 6000 cycles on a tile of 128 positions and 256 rows, of which the tensor cores
 // need 2048.  A slot's tile is a chain: its products and their commit 1400 cycles,
 // maxima 600, exponentials 2400 (the special function units need 1024, twice where
-// both slots are at it), P stored and its barrier 430.  Few rows: the same chain;
-// four samples of 2000 positions 20 us.
+// both slots are at it), P stored and its barrier 430.  Few rows: the same chain, and 16
+// of a slot's 128 lanes at work; four samples of 2000 positions 20 us, where every row reading the
+// prefix for itself takes 12.  Reading it once pays from about 100000 positions saved per call
+// on (positions times members less one, 8 kv heads of 128); a call without groups costs 9 us more than
+// kv8_attention.
 // Steps of that case: first form 607 us; parts joined by the second kernel, 336; a
 // warp that deals out the segments, 296; pages and scales by a warp of their own, 292;
 // no spills in the loops and no clock read while polling, 250.  Not kept: sixteen softmax

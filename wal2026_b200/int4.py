@@ -5,7 +5,9 @@
 scale * (code - zero).  It stands beside the Block-RVQ linears where a plain
 format is wanted, first of all as the vocabulary projection of a stack
 (``LlamaStack.quantize_head``), and as the linears of a whole stack
-(``llama.int4_llama``).  No counterpart in the reference.
+(``llama.int4_llama``).  It is made for decoding: a call reads the weight once for
+every 32 tokens, so from about 32 tokens on a dense linear is faster (2048 tokens of a
+prompt through 128256 x 4096: 13.8 ms, dense bf16 1.4).  No counterpart in the reference.
 """
 from __future__ import annotations
 

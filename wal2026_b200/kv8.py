@@ -288,7 +288,7 @@ def kv_pages_groups(table: Tensor, lens: Tensor, page_size: int, groups: Tensor,
 
     groups: int32 [4, rows]: the members' rows, group by group; each group's
     first member in that list; its size; and, for each row, how many
-    positions (a multiple of 32, below lens[row]) it shares with its group, 0 where it
+    positions (a multiple of 32, at most lens[row]) it shares with its group, 0 where it
     has none.  Rows that share fewer than ``least`` positions stay alone, so a larger
     ``least`` keeps a short common beginning from holding together rows that have more in
     common with some of the others.  One call serves all layers of a step.
@@ -315,7 +315,12 @@ def kv8_attention_shared(cache: PagedKV8Cache, layer: int, q: Tensor, table: Ten
     """``kv8_attention``, with what the rows of a group share read once for all of them.
 
     groups: int32 [4, B] from ``kv_pages_groups`` for this table and these lens.
-    The result is that of ``kv8_attention`` up to the rounding of weights to 16 bits.
+    The result is that of ``kv8_attention`` but for the weights of shared positions:
+    one f16 each (off by 2^-11, and 0 where weight times V scale is below 2^-32 of the
+    largest) where the other keeps 2^-16.  It pays for many rows of a long prefix: from
+    about 100000 positions saved on (positions times members less one; 8 kv heads of
+    128), later for several small groups.  Below that ``kv8_attention`` is faster, twice as
+    fast for a few short prompts.
     ``workspace`` comes from ``kv8_attention_shared_workspace``, for this many
     sequences and tokens, and is not shared by overlapping calls; status: int32 [1],
     set to 1 where a wait inside the kernel gave up (the outputs are wrong then).

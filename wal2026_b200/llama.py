@@ -207,7 +207,8 @@ class LlamaStack(nn.Module):
     def quantize_head(self, group_size: int = 128, *, zero_points: bool = False) -> None:
         """Compute logits from a 4-bit copy of this rank's lm_head (nearest codes, a scale per group of columns).
 
-        The dense lm_head stays where it was (it may be the embedding); ``self.head = None`` returns to it.
+        The dense lm_head stays where it was (it may be the embedding); ``self.head = None`` returns to it,
+        which is faster for steps of more than about 32 token rows (``int4``).
         """
         self.head = Int4Linear.from_dense(self.lm_head, group_size, zero_points=zero_points)
 

@@ -121,7 +121,8 @@ def logit_rules(logits: Tensor, out: Tensor, *, text: Optional[Tensor] = None, l
     generated (position prompt_lens[b] or later; None: all); bias[b, i] (fp32 [B,
     n]) is added to token bias_ids[b, i] (int32; equal ones add up); tokens whose
     bit of ``mask`` (int32 words [B, T, ceil(V / 32)], expanded axes allowed) is
-    clear, and NaN, are left out; the rest is divided by temperature[b].
+    clear, and NaN, are left out; the rest is divided by temperature[b].  out must not
+    overlap logits.
     Temperature 0 (or below) gives the first of the largest logits probability 1, and leaves
     logits undivided.  A row with no token left is all zeros (logits: -inf), rows
     t >= new_lens[b] are zeros.  Tokens outside [0, V) count nowhere.

@@ -14,7 +14,7 @@ without waiting for the host and can be captured into a CUDA graph:
     dec.fork([0, 0])                              # both rows continue sequence 0
 
 With ``share`` the attention reads what forked rows have in common once for all
-of them; with ``text`` the decoder keeps the rows' tokens, which the penalties of
+of them, which pays for many rows of a long prompt; with ``text`` the decoder keeps the rows' tokens, which the penalties of
 ``LogitRules`` need (``speculate(..., rules=rules)``, or ``logit_rules`` on the
 logits of a step).
 
@@ -63,7 +63,7 @@ class _StepBuffers:
 
 
 def _column(lin, x: Tensor, y: Tensor) -> None:
-    """y = x w^T: the GEMV for decode-sized calls, the prefill GEMM for prompts."""
+    """y = x w^T: the GEMV for decode-sized calls, the prefill GEMM for prompts of Block-RVQ linears (4-bit ones have none)."""
     if isinstance(lin, PackedGroupedBlockRVQLinear) and x.shape[0] >= PREFILL_MIN_TOKENS and lin.gemm_into(x, y):
         return
     _linear_into(lin, x, y)
@@ -88,8 +88,9 @@ class PagedDecoder:
     was carried out.
 
     share: rows whose first ``share`` positions (or more) lie in the same pages are
-    a group, whose common positions each step reads once (``kv_pages_groups``);
-    None: every row reads its own.  ``status`` int32 [1] becomes 1, and stays so until
+    a group, whose common positions each step reads once (``kv_pages_groups``, and
+    ``kv8_attention_shared`` for what that rounds and from where on it pays: a small
+    ``share`` makes steps of few rows or short prompts slower); None: every row reads its own.  ``status`` int32 [1] becomes 1, and stays so until
     the caller clears it, where that attention gave up a wait (after 2 s): what the steps
     since its last 0 returned and stored is wrong.  text: keep the rows' tokens in ``text`` int32
     [rows, max_len], by position; ``prompt_lens`` int32 [rows] (0 to begin with, the
