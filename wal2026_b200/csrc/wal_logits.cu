@@ -19,12 +19,12 @@
 // are exchanged as they are, undivided: every CTA's entries stand relative to a number that
 // all know exactly.  (The fused exp2(x k - round(m k)), with each CTA's maximum divided
 // anew for the exchange, was off by 2^-24 of m k between CTAs, and took a CTA of masked
-// logits around -1e10 to an infinite sum.)  Temperatures outside [2^-40, 2^40] and quotients
-// near fp32's ends divide each difference instead; quotients that leave the range count as infinities.
+// logits around -1e10 to an infinite sum.)  Temperatures outside [2^-40, 2^40] and maxima whose
+// quotient is near fp32's upper end divide each difference instead; quotients that leave the range count as infinities.
 //
 // On B200, 128256 tokens: 576 rows with every rule 208 us (453 MB, 2.2 TB/s; a copy
 // would take 69), 80 fp32 rows with masks and biases 45 us, one row 12 us, most of it the
-// host's call (11 in a graph).  The long calls are bound by the rules' instructions and by a row's
+// host's call (11 in a graph); 128 rows of 151936 tokens, on one CTA per SM with a few spilled words, 216 us (116 MB).  The long calls are bound by the rules' instructions and by a row's
 // exchanges between its CTAs, with two CTAs per SM to hide them.  Earlier forms of the
 // long one: entries in shared memory and a division for each 418 us; a cluster per row
 // 324; clusters that stay, neighbouring tokens in one CTA 442, and dealt out in blocks 273.
